@@ -522,6 +522,100 @@ int qmoe_attention_forward(const qmoe_attention_t* attention, uint64_t stream);
 int qmoe_attention_backward(const qmoe_attention_t* attention, uint64_t stream);
 
 /* ---------------------------------------------------------------------------------------------
+ * Norm and rotation of query and key heads in one pass (no upstream counterpart: its blocks rotate unnormalised heads,
+ * src/qutai/lm/layers.py:316-349): every head of every row, x of `dim` elements,
+ *     y = R(p) (w * x / sqrt(mean(x^2) + eps)),   p = offset + starts[b] + t,
+ * R(p) turning the pairs (2 i, 2 i + 1) by p theta^(-2 i / dim) as qmoe_rope does; one weight for the query heads, one for the key
+ * heads.  Any number of rows, none included; dim a multiple of 8 up to 256; rows may lie `pitch` elements apart (a fused projection's output).
+ * ------------------------------------------------------------------------------------------- */
+typedef struct qmoe_norm_rope {
+    int64_t batch, time;
+    int32_t heads, kv_heads, dim;
+    int32_t dtype;                       /* of q, k, their outputs and gradients */
+    int64_t offset;                      /* position of row 0 of a sequence, starts[b] added where given */
+    int64_t q_pitch, k_pitch;            /* elements from a row of q (k) to the next; outputs and gradients are dense */
+    double eps, theta;
+    uint64_t q;                          /* [batch, time, heads, dim] */
+    uint64_t k;                          /* [batch, time, kv_heads, dim] */
+    uint64_t q_weight, k_weight;         /* f32 [dim] */
+    uint64_t starts;                     /* i32 [batch], or 0 */
+    uint64_t q_out, k_out;               /* forward */
+    uint64_t grad_q, grad_k;             /* backward: gradients of q_out, k_out */
+    uint64_t dq, dk;                     /* backward: dense, like q_out, k_out */
+    uint64_t d_q_weight, d_k_weight;     /* backward: f32 [dim] */
+    uint64_t partials;                   /* backward: f32 [qmoe_norm_rope_partials(...)] scratch */
+} qmoe_norm_rope_t;
+int qmoe_norm_rope_forward(const qmoe_norm_rope_t* norm_rope, uint64_t stream);
+int64_t qmoe_norm_rope_partials(int64_t batch, int64_t time, int32_t heads, int32_t kv_heads, int32_t dim);
+int qmoe_norm_rope_backward(const qmoe_norm_rope_t* norm_rope, uint64_t stream);
+
+/* ---------------------------------------------------------------------------------------------
+ * A key/value cache for decoding, and attention over it (upstream decodes without one: every token runs the whole sequence again).
+ * Keys and values lie [batch, kv_heads, capacity, dim], so that a head's positions are contiguous; sequence b holds lengths[b] of them.  In a
+ * QMOE_INT8 cache the `dim` values of a head and position are whole multiples, -127 .. 127, of a scale of their own,
+ * max |x| / 127 in f32; a value is the whole number times the scale.
+ * ------------------------------------------------------------------------------------------- */
+enum { QMOE_INT8 = 2 };                  /* dtype of a cache, beside QMOE_BF16 */
+typedef struct qmoe_cache {
+    int64_t batch, capacity;
+    int32_t kv_heads, dim;               /* dim: a multiple of 8 up to 256 */
+    int32_t dtype;                       /* QMOE_BF16 or QMOE_INT8 */
+    int32_t reserved;
+    uint64_t k, v;                       /* [batch, kv_heads, capacity, dim] */
+    uint64_t k_scale, v_scale;           /* f32 [batch, kv_heads, capacity]; 0 for QMOE_BF16 */
+    uint64_t lengths;                    /* i32 [batch], read on the device */
+} qmoe_cache_t;
+/* Rows [b, t < counts[b]] of k and v ([batch, time, kv_heads, dim], rows `pitch` elements apart; counts i32 [batch], 0: time) go to positions
+ * lengths[b] + t, and lengths_out[b] = lengths[b] + counts[b].  lengths_out is another buffer than lengths.  What would
+ * lie behind `capacity` is dropped, and lengths_out[b] ends there. */
+int qmoe_cache_append(const qmoe_cache_t* cache, uint64_t k, uint64_t v, int32_t dtype, int64_t k_pitch, int64_t v_pitch, int64_t time,
+                      uint64_t counts, uint64_t lengths_out, uint64_t stream);
+/* Positions [start, start + count) of every sequence as k_out, v_out [batch, count, kv_heads, dim]; zeros behind a sequence's length. */
+int qmoe_cache_read(const qmoe_cache_t* cache, int64_t start, int64_t count, uint64_t k_out, uint64_t v_out, int32_t dtype, uint64_t stream);
+/* New queries of a batch over a prefix that all its sequences share and over each sequence's own cache, which holds the keys
+ * of the new positions already:
+ *     out[b, t, h, :] = softmax([q . Kp^T, q . Kb^T] / sqrt(dim)) [Vp; Vb],   query t seeing the whole prefix and the first
+ * lengths[b] - time + t + 1 positions of sequence b.  A row that sees nothing gives zeros and lse = -infinity.  The prefix (a cache of batch 1) is
+ * read once for all sequences.  bf16 queries, dim 64 or 128. */
+typedef struct qmoe_prefix_attention {
+    int64_t time;                        /* new positions of every sequence */
+    int32_t heads;
+    int32_t reserved;
+    int64_t prefix_longest, longest;     /* bounds on the prefix's length and on the sequences', known to the host */
+    uint64_t q;                          /* [batch, time, heads, dim] */
+    uint64_t out;                        /* like q */
+    uint64_t lse;                        /* f32 [batch, time, heads] */
+    uint64_t scratch;                    /* qmoe_prefix_attention_scratch bytes */
+} qmoe_prefix_attention_t;
+/* prefix: null or a cache with the kv_heads, dim and dtype of `cache` */
+int64_t qmoe_prefix_attention_scratch(const qmoe_prefix_attention_t* attention, const qmoe_cache_t* cache, const qmoe_cache_t* prefix);
+int qmoe_prefix_attention(const qmoe_prefix_attention_t* attention, const qmoe_cache_t* cache, const qmoe_cache_t* prefix, uint64_t stream);
+
+/* ---------------------------------------------------------------------------------------------
+ * One token a row from given uniform numbers (no upstream counterpart on the device).  The weight of a token is
+ * exp((logit - largest) / temperature), held as a whole number of 2^-31 (a weight below 2^-32 of the largest is none), so that sums
+ * do not depend on their order.  Kept are the top_k largest logits (0 or at least vocab: all; of equal ones those of lower
+ * index), of these the shortest run from the largest that holds top_p of their weight, of these the ones of at least
+ * min_p times the largest's weight; the token is the first at which the running sum of the kept weights, by index, passes
+ * uniform * their sum.  Temperature 0 (and whatever is not above it): the first of the largest.  NaN logits count as -infinity; a row without
+ * another gives token -1.  log_prob: of the token among ALL of the row's at its temperature (at 1 for temperature 0).
+ * ------------------------------------------------------------------------------------------- */
+typedef struct qmoe_sample {
+    int64_t rows, vocab;                 /* vocab up to 2^22 */
+    int32_t dtype;                       /* of the logits */
+    int32_t top_k;
+    float temperature, top_p, min_p;     /* for every row, unless the row's own are given: */
+    float reserved;
+    uint64_t logits;                     /* [rows, vocab] */
+    uint64_t uniforms;                   /* f32 [rows], in [0, 1) */
+    uint64_t temperatures, top_ps, min_ps;   /* f32 [rows], or 0 */
+    uint64_t top_ks;                     /* i32 [rows], or 0 */
+    uint64_t tokens;                     /* i64 [rows] */
+    uint64_t log_probs;                  /* f32 [rows] */
+} qmoe_sample_t;
+int qmoe_sample(const qmoe_sample_t* sample, uint64_t stream);
+
+/* ---------------------------------------------------------------------------------------------
  * Expert parallelism (one process per GPU, NCCL over NVLink / NVSwitch).  The upstream project is
  * single-GPU (src/qutai/backends/cuda_runtime.py:82, :105), so these entry points have no upstream
  * counterpart; they keep the layer's semantics when tokens are sharded T/N per rank (contiguous

@@ -1,0 +1,346 @@
+// The norm of every query and key head and the rotation of its position, queries and keys in one pass:
+//     y = R(p) (w * x / rms(x)),   rms(x) = sqrt(mean(x^2) + eps) over the head's `dim` elements,
+// with R(p) turning every pair (2 i, 2 i + 1) by the angle p theta^(-2 i / dim), p the row's position.  Backward, from g = dL/dy:
+//     g' = R(-p) g,   dw = sum over rows and heads of g' * x / rms,   dx = (g' * w - x / rms * mean(g' * w * x / rms)) / rms.
+// The statistics are not kept from the forward: a head is in a few lanes' registers anyway.
+//
+// dim / 8 lanes (rounded up to a power of two) hold a head, eight elements each, so a warp has 32 / lanes heads at a time, and
+// goes through a chunk of a row's heads with the row's angles formed once.
+//
+// Angles.  A position times a frequency is a place on the circle, and what counts is its fraction of a turn: the frequency in
+// turns is held as a 64-bit fraction F (2^64 = one turn), so position * F modulo 2^64, an integer product, IS that fraction, exact to
+// 2^-64 * position at any position, and its upper half goes to sincospi.  (In 32 bits the angle of position 100000 is off by 4e-3.)
+// Sums over rows run in a fixed order (no atomics).
+#include "common.cuh"
+
+#include <math.h>
+
+namespace qmoe {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kWarps = kThreads / 32;
+constexpr int kMaxDim = 256;
+constexpr int kInFlight = 4;             // heads of a lane whose loads are on their way together
+
+struct NormRopeParams {
+    const void* q;
+    const void* k;
+    void* q_out;                         // backward: dq, dk
+    void* k_out;
+    const void* grad_q;
+    const void* grad_k;
+    const float* q_weight;
+    const float* k_weight;
+    const int* starts;
+    float* partials;
+    long long offset, q_pitch, k_pitch;
+    int rows, time, heads, kv_heads, dim;
+    int lane_bits, passes;               // log2 of the lanes per head; heads of a lane per chunk
+    float eps;
+    unsigned long long turns[kMaxDim / 2];
+};
+
+__device__ __forceinline__ void load8(const __nv_bfloat16* p, uint4* raw) { raw[0] = *reinterpret_cast<const uint4*>(p); }
+__device__ __forceinline__ void load8(const float* p, uint4* raw) {
+    raw[0] = *reinterpret_cast<const uint4*>(p);
+    raw[1] = *reinterpret_cast<const uint4*>(p + 4);
+}
+template <typename T> __device__ __forceinline__ void unpack8(const uint4* raw, float* f) {
+    Vec16<T>::unpack(raw[0], f);
+    if constexpr (Vec16<T>::N == 4) Vec16<T>::unpack(raw[1], f + 4);
+}
+template <typename T> __device__ __forceinline__ void store8(T* p, const float* f) {
+    *reinterpret_cast<uint4*>(p) = Vec16<T>::pack(f);
+    if constexpr (Vec16<T>::N == 4) *reinterpret_cast<uint4*>(p + 4) = Vec16<T>::pack(f + 4);
+}
+// sum over the 2^bits neighbouring lanes of a head, in every one of them
+__device__ __forceinline__ float head_sum(float v, int bits) {
+    for (int o = 1; o < 1 << bits; o <<= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+
+// What a lane keeps throughout: its place in a head, its frequencies and weights
+template <typename T> struct Lane {
+    int sub, slot, per_warp;
+    bool active;
+    unsigned long long turns[4];
+    float wq[8], wk[8];
+    __device__ __forceinline__ Lane(const NormRopeParams& p) {
+        const int lane = threadIdx.x & 31;
+        sub = lane & ((1 << p.lane_bits) - 1);
+        slot = lane >> p.lane_bits;
+        per_warp = 32 >> p.lane_bits;
+        active = sub * 8 < p.dim;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) turns[i] = active ? p.turns[4 * sub + i] : 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            wq[i] = active ? p.q_weight[8 * sub + i] : 0.f;
+            wk[i] = active ? p.k_weight[8 * sub + i] : 0.f;
+        }
+    }
+    __device__ __forceinline__ void angles(const NormRopeParams& p, int row, float* s, float* c) const {
+        const int b = row / p.time;
+        const long long position = p.offset + (p.starts ? p.starts[b] : 0) + (row - b * p.time);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int turn = (int)(((unsigned long long)position * turns[i]) >> 32);      // of 2^32
+            sincospif((float)turn * 4.656612873077392578125e-10f, &s[i], &c[i]);         // 2^-31: half turns
+        }
+    }
+};
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads)
+norm_rope_kernel(const __grid_constant__ NormRopeParams p) {
+    chain_begin();
+    const Lane<T> me(p);
+    const int total = p.heads + p.kv_heads, first = blockIdx.y * p.passes * me.per_warp + me.slot;
+    for (int row = blockIdx.x * kWarps + (threadIdx.x >> 5); row < p.rows; row += gridDim.x * kWarps) {
+        float s[4], c[4];
+        bool have = false;
+        for (int at = 0; at < p.passes; at += kInFlight) {
+            uint4 raw[kInFlight][2];
+#pragma unroll
+            for (int u = 0; u < kInFlight; ++u) {
+                const int h = first + (at + u) * me.per_warp;
+                if (me.active && at + u < p.passes && h < total)
+                    load8((h < p.heads ? (const T*)p.q + row * p.q_pitch + h * p.dim : (const T*)p.k + row * p.k_pitch + (h - p.heads) * p.dim) + 8 * me.sub,
+                          raw[u]);
+                else
+                    raw[u][0] = raw[u][1] = make_uint4(0, 0, 0, 0);
+            }
+            if (!have) {
+                me.angles(p, row, s, c);
+                have = true;
+            }
+#pragma unroll
+            for (int u = 0; u < kInFlight; ++u) {
+                const int h = first + (at + u) * me.per_warp;
+                const bool live = at + u < p.passes && h < total;
+                if (!__any_sync(0xffffffffu, live)) break;
+                float x[8], y[8], square = 0.f;
+                unpack8<T>(raw[u], x);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) square = fmaf(x[i], x[i], square);
+                const float inverse = rsqrtf(head_sum(square, p.lane_bits) / (float)p.dim + p.eps);
+                const bool query = h < p.heads;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float a = x[2 * i] * inverse * (query ? me.wq[2 * i] : me.wk[2 * i]);
+                    const float b = x[2 * i + 1] * inverse * (query ? me.wq[2 * i + 1] : me.wk[2 * i + 1]);
+                    y[2 * i] = a * c[i] - b * s[i];
+                    y[2 * i + 1] = a * s[i] + b * c[i];
+                }
+                if (live && me.active)
+                    store8((query ? (T*)p.q_out + (long long)row * p.heads * p.dim + h * p.dim
+                                  : (T*)p.k_out + (long long)row * p.kv_heads * p.dim + (h - p.heads) * p.dim) + 8 * me.sub, y);
+            }
+        }
+    }
+}
+
+// dq, dk, and this block's share of the weights' gradients: partials[block][q | k][dim]
+template <typename T>
+__global__ void __launch_bounds__(kThreads)
+norm_rope_backward_kernel(const __grid_constant__ NormRopeParams p) {
+    chain_begin();
+    const Lane<T> me(p);
+    const int total = p.heads + p.kv_heads, first = blockIdx.y * p.passes * me.per_warp + me.slot;
+    float dwq[8] = {}, dwk[8] = {};
+    for (int row = blockIdx.x * kWarps + (threadIdx.x >> 5); row < p.rows; row += gridDim.x * kWarps) {
+        float s[4], c[4];
+        bool have = false;
+        for (int at = 0; at < p.passes; at += kInFlight / 2) {
+            uint4 raw[kInFlight / 2][2], raw_g[kInFlight / 2][2];
+#pragma unroll
+            for (int u = 0; u < kInFlight / 2; ++u) {
+                const int h = first + (at + u) * me.per_warp;
+                if (me.active && at + u < p.passes && h < total) {
+                    const bool query = h < p.heads;
+                    load8((query ? (const T*)p.q + row * p.q_pitch + h * p.dim : (const T*)p.k + row * p.k_pitch + (h - p.heads) * p.dim) + 8 * me.sub, raw[u]);
+                    load8((query ? (const T*)p.grad_q + (long long)row * p.heads * p.dim + h * p.dim
+                                 : (const T*)p.grad_k + (long long)row * p.kv_heads * p.dim + (h - p.heads) * p.dim) + 8 * me.sub, raw_g[u]);
+                } else {
+                    raw[u][0] = raw[u][1] = raw_g[u][0] = raw_g[u][1] = make_uint4(0, 0, 0, 0);
+                }
+            }
+            if (!have) {
+                me.angles(p, row, s, c);
+                have = true;
+            }
+#pragma unroll
+            for (int u = 0; u < kInFlight / 2; ++u) {
+                const int h = first + (at + u) * me.per_warp;
+                const bool live = at + u < p.passes && h < total;
+                if (!__any_sync(0xffffffffu, live)) break;
+                float x[8], g[8], square = 0.f, dot = 0.f;
+                unpack8<T>(raw[u], x);
+                unpack8<T>(raw_g[u], g);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) square = fmaf(x[i], x[i], square);
+                const float inverse = rsqrtf(head_sum(square, p.lane_bits) / (float)p.dim + p.eps);
+                const bool query = h < p.heads;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {          // turned back
+                    const float a = g[2 * i], b = g[2 * i + 1];
+                    g[2 * i] = a * c[i] + b * s[i];
+                    g[2 * i + 1] = b * c[i] - a * s[i];
+                }
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    x[i] *= inverse;
+                    const float gx = g[i] * x[i];
+                    if (query) dwq[i] += gx; else dwk[i] += gx;      // zero where there is no head
+                    g[i] *= query ? me.wq[i] : me.wk[i];
+                    dot = fmaf(g[i], x[i], dot);
+                }
+                dot = head_sum(dot, p.lane_bits) / (float)p.dim;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) g[i] = inverse * (g[i] - x[i] * dot);
+                if (live && me.active)
+                    store8((query ? (T*)p.q_out + (long long)row * p.heads * p.dim + h * p.dim
+                                  : (T*)p.k_out + (long long)row * p.kv_heads * p.dim + (h - p.heads) * p.dim) + 8 * me.sub, g);
+            }
+        }
+    }
+    __shared__ float s_sum[kWarps][2][kMaxDim];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        for (int o = 1 << p.lane_bits; o < 32; o <<= 1) {
+            dwq[i] += __shfl_xor_sync(0xffffffffu, dwq[i], o);
+            dwk[i] += __shfl_xor_sync(0xffffffffu, dwk[i], o);
+        }
+        if (lane < 1 << p.lane_bits) {
+            s_sum[warp][0][8 * me.sub + i] = dwq[i];
+            s_sum[warp][1][8 * me.sub + i] = dwk[i];
+        }
+    }
+    __syncthreads();
+    float* out = p.partials + (long long)(blockIdx.y * gridDim.x + blockIdx.x) * 2 * p.dim;
+    for (int j = threadIdx.x; j < 2 * p.dim; j += kThreads) {
+        const int which = j >= p.dim, column = j - which * p.dim;
+        float sum = 0.f;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) sum += s_sum[w][which][column];
+        out[j] = sum;
+    }
+}
+
+// A warp per column of the weights' gradients: its lanes stride over the blocks' shares and meet in a fixed tree
+__global__ void __launch_bounds__(kThreads)
+norm_rope_weights_kernel(const float* __restrict__ partials, float* __restrict__ dq_weight, float* __restrict__ dk_weight, int blocks, int dim) {
+    chain_begin();
+    const int column = blockIdx.x * kWarps + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+    if (column >= 2 * dim) return;
+    float sum = 0.f;
+    for (int b = lane; b < blocks; b += 32) sum += partials[(long long)b * 2 * dim + column];
+    sum = warp_sum(sum);
+    if (lane == 0) (column < dim ? dq_weight : dk_weight - dim)[column] = sum;
+}
+
+struct Shape { int lane_bits, passes, chunks, blocks; };
+
+// Lanes per head, and how a row's heads are cut into chunks: whole rows to a warp (angles formed once) while the rows alone make
+// eight warps per SM, else shorter chunks down to one head per lane.
+Shape shape_of(long long rows, int heads, int kv_heads, int dim, int warps_per_sm) {
+    Shape s = {};
+    while ((8 << s.lane_bits) < dim) ++s.lane_bits;
+    const int per_warp = 32 >> s.lane_bits, all = ceil_div(heads + kv_heads, per_warp);
+    s.passes = all;
+    while (s.passes > 1 && rows * ceil_div(all, s.passes) < (long long)sm_count() * 8) s.passes = (s.passes + 1) / 2;
+    s.chunks = ceil_div(all, s.passes);
+    const long long blocks = (rows + kWarps - 1) / kWarps, most = (long long)sm_count() * warps_per_sm / kWarps / s.chunks;
+    s.blocks = (int)(blocks < (most > 1 ? most : 1) ? blocks : (most > 1 ? most : 1));
+    return s;
+}
+constexpr int kForwardWarps = 32, kBackwardWarps = 16;     // per SM
+
+int norm_rope_check(const qmoe_norm_rope_t* a, bool backward) {
+    if (!a) return fail_arg("norm_rope: argument is null");
+    if (a->dtype != QMOE_F32 && a->dtype != QMOE_BF16) return fail_arg("norm_rope: dtype must be QMOE_F32 or QMOE_BF16");
+    if (a->batch < 0 || a->time < 0 || a->heads <= 0 || a->kv_heads <= 0) return fail_arg("norm_rope: sizes must not be negative, head counts positive");
+    if (a->dim < 8 || a->dim > kMaxDim || a->dim % 8) return fail_arg("norm_rope: the head width must be a multiple of 8 up to %d", kMaxDim);
+    if (a->heads > (1 << 20) || a->kv_heads > (1 << 20) || (a->batch && a->time > 0x7fffffff / a->batch)) return fail_arg("norm_rope: too many rows or heads");
+    if (!(a->theta > 0) || !(a->eps >= 0) || a->theta > 1e30) return fail_arg("norm_rope: theta must be positive and eps not negative");
+    if (!a->q || !a->k || !a->q_weight || !a->k_weight) return fail_arg("norm_rope: null buffer address");
+    if (backward ? !a->grad_q || !a->grad_k || !a->dq || !a->dk || !a->d_q_weight || !a->d_k_weight || !a->partials : !a->q_out || !a->k_out)
+        return fail_arg("norm_rope: null buffer address");
+    if ((a->q | a->k | a->q_out | a->k_out | a->grad_q | a->grad_k | a->dq | a->dk) & 15u) return fail_arg("norm_rope: rows must be 16-byte aligned");
+    if ((a->q_weight | a->k_weight | a->starts | a->partials | a->d_q_weight | a->d_k_weight) & 3u) return fail_arg("norm_rope: misaligned address");
+    const long long align = a->dtype == QMOE_BF16 ? 8 : 4;
+    if (a->q_pitch % align || a->k_pitch % align || a->q_pitch < (long long)a->heads * a->dim || a->k_pitch < (long long)a->kv_heads * a->dim)
+        return fail_arg("norm_rope: a row pitch must be a multiple of 16 bytes and not below the row's width");
+    return 0;
+}
+
+void norm_rope_params(const qmoe_norm_rope_t* a, const Shape& s, NormRopeParams& p) {
+    p.q = (const void*)a->q; p.k = (const void*)a->k;
+    p.q_weight = (const float*)a->q_weight; p.k_weight = (const float*)a->k_weight;
+    p.starts = (const int*)a->starts;
+    p.offset = a->offset; p.q_pitch = a->q_pitch; p.k_pitch = a->k_pitch;
+    p.rows = (int)(a->batch * a->time); p.time = (int)a->time;
+    p.heads = a->heads; p.kv_heads = a->kv_heads; p.dim = a->dim;
+    p.lane_bits = s.lane_bits; p.passes = s.passes;
+    p.eps = (float)a->eps;
+    const long double ratio = powl((long double)a->theta, -2.0L / a->dim);
+    long double turns = 1.0L / 6.283185307179586476925286766559L;
+    for (int i = 0; i < a->dim / 2; ++i, turns *= ratio) {
+        const long double fraction = ldexpl(turns - floorl(turns), 64);
+        p.turns[i] = fraction >= 18446744073709551615.0L ? 0ull : (unsigned long long)fraction;
+    }
+}
+
+}  // namespace
+}  // namespace qmoe
+
+using namespace qmoe;
+
+extern "C" int qmoe_norm_rope_forward(const qmoe_norm_rope_t* a, uint64_t stream_) {
+    if (int rc = norm_rope_check(a, false)) return rc;
+    if (!a->batch || !a->time) return 0;
+    cudaStream_t stream = (cudaStream_t)stream_;
+    TimedScope timed(KC_ELEMENTWISE, stream);
+    const Shape s = shape_of(a->batch * a->time, a->heads, a->kv_heads, a->dim, kForwardWarps);
+    NormRopeParams p = {};
+    norm_rope_params(a, s, p);
+    p.q_out = (void*)a->q_out; p.k_out = (void*)a->k_out;
+    const dim3 grid((unsigned)s.blocks, (unsigned)s.chunks);
+    if (a->dtype == QMOE_BF16) chained(norm_rope_kernel<__nv_bfloat16>, grid, kThreads, 0, stream, p);
+    else chained(norm_rope_kernel<float>, grid, kThreads, 0, stream, p);
+    QMOE_LAUNCH_CHECK("norm_rope_kernel");
+    return 0;
+}
+
+extern "C" int64_t qmoe_norm_rope_partials(int64_t batch, int64_t time, int32_t heads, int32_t kv_heads, int32_t dim) {
+    if (batch <= 0 || time <= 0 || heads <= 0 || kv_heads <= 0 || dim < 8 || dim > kMaxDim) return 1;
+    const Shape s = shape_of(batch * time, heads, kv_heads, dim, kBackwardWarps);
+    return (int64_t)s.blocks * s.chunks * 2 * dim;
+}
+
+extern "C" int qmoe_norm_rope_backward(const qmoe_norm_rope_t* a, uint64_t stream_) {
+    if (int rc = norm_rope_check(a, true)) return rc;
+    cudaStream_t stream = (cudaStream_t)stream_;
+    TimedScope timed(KC_ELEMENTWISE, stream);
+    if (!a->batch || !a->time) {       // no rows: nothing but the weights' gradients to write
+        QMOE_CUDA(cudaMemsetAsync((void*)a->d_q_weight, 0, a->dim * sizeof(float), stream));
+        QMOE_CUDA(cudaMemsetAsync((void*)a->d_k_weight, 0, a->dim * sizeof(float), stream));
+        return 0;
+    }
+    const Shape s = shape_of(a->batch * a->time, a->heads, a->kv_heads, a->dim, kBackwardWarps);
+    NormRopeParams p = {};
+    norm_rope_params(a, s, p);
+    p.q_out = (void*)a->dq; p.k_out = (void*)a->dk;
+    p.grad_q = (const void*)a->grad_q; p.grad_k = (const void*)a->grad_k;
+    p.partials = (float*)a->partials;
+    const dim3 grid((unsigned)s.blocks, (unsigned)s.chunks);
+    if (a->dtype == QMOE_BF16) chained(norm_rope_backward_kernel<__nv_bfloat16>, grid, kThreads, 0, stream, p);
+    else chained(norm_rope_backward_kernel<float>, grid, kThreads, 0, stream, p);
+    QMOE_LAUNCH_CHECK("norm_rope_backward_kernel");
+    chained(norm_rope_weights_kernel, (unsigned)ceil_div(2 * a->dim, kWarps), kThreads, 0, stream, (const float*)a->partials, (float*)a->d_q_weight,
+            (float*)a->d_k_weight, s.blocks * s.chunks, a->dim);
+    QMOE_LAUNCH_CHECK("norm_rope_weights_kernel");
+    return 0;
+}

@@ -13,14 +13,15 @@ import threading
 from ctypes import (POINTER, Structure, byref, c_char_p, c_double, c_float, c_int, c_int32, c_int64,
                     c_uint64, c_void_p)
 
-QMOE_F32, QMOE_BF16 = 0, 1
+QMOE_F32, QMOE_BF16, QMOE_INT8 = 0, 1, 2
 ENGINE_AUTO, ENGINE_SIMT, ENGINE_TCGEN05 = 0, 1, 2
 VARIANT_SINGLE_CTA_GEMM, VARIANT_WGRAD_PER_PRODUCT, VARIANT_NARROW_SCATTER, VARIANT_PLAIN_GEMM_ON_CUDA_CORES = 0, 1, 2, 3
 VARIANT_NO_STREAM_GEMM, VARIANT_NO_FLOAT32_TILES = 4, 5
 EXPERTS_SHORT_PADS = 0x5350
 ROW_PAD, MAX_EXPERTS, MAX_TOP_K = 128, 256, 8
 DTYPE_CODES = {"float32": QMOE_F32, "bfloat16": QMOE_BF16}
-ITEM_BYTES = {"float32": 4, "bfloat16": 2, "int32": 4, "int64": 8, "float64": 8}
+CACHE_CODES = {"bfloat16": QMOE_BF16, "int8": QMOE_INT8}
+ITEM_BYTES = {"int8": 1, "float32": 4, "bfloat16": 2, "int32": 4, "int64": 8, "float64": 8}
 
 
 class Route(Structure):
@@ -85,6 +86,33 @@ class Attention(Structure):
     """``qmoe_attention_t``."""
     _fields_ = [(name, c_int32) for name in ("batch", "time", "heads", "kv_heads", "dim", "dtype")] + [(name, c_uint64) for name in (
         "q", "k", "v", "out", "lse", "grad_out", "delta", "dq", "dk", "dv")]
+
+
+class NormRope(Structure):
+    """``qmoe_norm_rope_t``."""
+    _fields_ = [("batch", c_int64), ("time", c_int64), ("heads", c_int32), ("kv_heads", c_int32), ("dim", c_int32), ("dtype", c_int32),
+                ("offset", c_int64), ("q_pitch", c_int64), ("k_pitch", c_int64), ("eps", c_double), ("theta", c_double)] + [
+        (name, c_uint64) for name in ("q", "k", "q_weight", "k_weight", "starts", "q_out", "k_out", "grad_q", "grad_k", "dq", "dk",
+                                      "d_q_weight", "d_k_weight", "partials")]
+
+
+class Cache(Structure):
+    """``qmoe_cache_t``."""
+    _fields_ = [("batch", c_int64), ("capacity", c_int64), ("kv_heads", c_int32), ("dim", c_int32), ("dtype", c_int32), ("reserved", c_int32)] + [
+        (name, c_uint64) for name in ("k", "v", "k_scale", "v_scale", "lengths")]
+
+
+class PrefixAttention(Structure):
+    """``qmoe_prefix_attention_t``."""
+    _fields_ = [("time", c_int64), ("heads", c_int32), ("reserved", c_int32), ("prefix_longest", c_int64), ("longest", c_int64)] + [
+        (name, c_uint64) for name in ("q", "out", "lse", "scratch")]
+
+
+class Sample(Structure):
+    """``qmoe_sample_t``."""
+    _fields_ = [("rows", c_int64), ("vocab", c_int64), ("dtype", c_int32), ("top_k", c_int32), ("temperature", c_float), ("top_p", c_float),
+                ("min_p", c_float), ("reserved", c_float)] + [
+        (name, c_uint64) for name in ("logits", "uniforms", "temperatures", "top_ps", "min_ps", "top_ks", "tokens", "log_probs")]
 
 
 _U, _I32, _I64 = c_uint64, c_int32, c_int64
@@ -172,6 +200,14 @@ SIGNATURES = {
     "qmoe_embedding_backward": (c_int, [_U, _I32, _U, _U, _U, _U, _I64, _I64, _I64, _I64, _U]),
     "qmoe_attention_forward": (c_int, [POINTER(Attention), _U]),
     "qmoe_attention_backward": (c_int, [POINTER(Attention), _U]),
+    "qmoe_norm_rope_forward": (c_int, [POINTER(NormRope), _U]),
+    "qmoe_norm_rope_partials": (c_int64, [_I64, _I64, _I32, _I32, _I32]),
+    "qmoe_norm_rope_backward": (c_int, [POINTER(NormRope), _U]),
+    "qmoe_cache_append": (c_int, [POINTER(Cache), _U, _U, _I32, _I64, _I64, _I64, _U, _U, _U]),
+    "qmoe_cache_read": (c_int, [POINTER(Cache), _I64, _I64, _U, _U, _I32, _U]),
+    "qmoe_prefix_attention_scratch": (c_int64, [POINTER(PrefixAttention), POINTER(Cache), POINTER(Cache)]),
+    "qmoe_prefix_attention": (c_int, [POINTER(PrefixAttention), POINTER(Cache), POINTER(Cache), _U]),
+    "qmoe_sample": (c_int, [POINTER(Sample), _U]),
     "qmoe_layer_forward": (c_int, [_LP, _U]),
     "qmoe_layer_backward": (c_int, [_LP, _U]),
     "qmoe_ep_unique_id": (c_int, [c_void_p]),

@@ -22,7 +22,7 @@ from array import array
 
 from . import lib
 
-_FORMATS = {"float32": "f", "float64": "d", "int32": "i", "int64": "q"}
+_FORMATS = {"int8": "b", "float32": "f", "float64": "d", "int32": "i", "int64": "q"}
 _cache: dict[int, list[int]] = {}
 _cached_bytes = 0
 # Freed blocks are kept for reuse up to this many bytes (a B200 has 180 GB; activations and gradients of the
