@@ -601,7 +601,7 @@ int qmoe_prefix_attention(const qmoe_prefix_attention_t* attention, const qmoe_c
  * another gives token -1.  log_prob: of the token among ALL of the row's at its temperature (at 1 for temperature 0).
  * ------------------------------------------------------------------------------------------- */
 typedef struct qmoe_sample {
-    int64_t rows, vocab;                 /* vocab up to 2^22 */
+    int64_t rows, vocab;                 /* vocab up to 2000000 */
     int32_t dtype;                       /* of the logits */
     int32_t top_k;
     float temperature, top_p, min_p;     /* for every row, unless the row's own are given: */

@@ -136,3 +136,22 @@ def test_no_rows():
 
     tokens, log_probs = sample(Tensor(DeviceStorage(0, "float32"), (0, 50)), DeviceStorage(0, "float32"))
     assert tokens.size == 0 and log_probs.size == 0
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("vocab", [700001, 1999999])
+def test_vocabularies_that_no_shared_memory_holds(vocab, dtype):
+    rng = np.random.default_rng(8)
+    check(rng.standard_normal((2, vocab)), rng.random(2), dtype, top_p=0.8, top_k=vocab - 5)
+    check(rng.standard_normal((2, vocab)) * 4, rng.random(2), dtype, top_k=100)
+    check(np.zeros((1, vocab)), rng.random(1), dtype, top_p=0.5)
+
+
+def test_more_tokens_than_there_are_with_any_weight():
+    """Half of the row masked, or too small to weigh anything: top-k beyond the rest takes all of it."""
+    rng = np.random.default_rng(10)
+    logits = rng.standard_normal((4, 3000))
+    logits[:, ::2] = -np.inf
+    logits[2:, 1::4] = -200.0
+    check(logits, rng.random(4), top_k=2000, top_p=0.9)
+    check(logits, rng.random(4), top_k=2000)
