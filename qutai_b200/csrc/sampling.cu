@@ -7,17 +7,20 @@
 // c or a higher one, for the least c with mass(above c) < p * mass; for top-k the same with counts.
 //
 // A cluster of up to eight CTAs works on a row, each with a slice of it in shared memory: the logits are read from HBM once.
-//   1  the largest logit (its place), over the cluster
+//   1  the largest logit, over the cluster
 //   2  the masses' sum, and the sum of those that min-p lets through.  Where top-p cannot cut into those any more, or nothing cuts, on to 5
 //   3  a bound on how far down the kept tokens reach, from the threads' largest logits: where k of those lie in the upper buckets of
-//      a histogram by z = (max - x) / T, so do the k largest of all; the same with p of the mass
-//   4  a histogram, counts and masses, of what lies above the bound; its crossing bucket is the only one whose members have to be told
-//      apart, and goes to a list in the first CTA, which finds the threshold there.  A bucket too full for the list (thousands
-//      of equal logits): the threshold by bisection over the places, every step a question to all CTAs
+//      a histogram by z = (max - x) / T, so do the k largest of all; the same with p of the mass.  What lies above the bound goes to a list in the
+//      first CTA; where that holds it (most rows: k or a little more), everything else is done there, each member compared with all others
+//   4  else a histogram, counts and masses, of what lies above the bound; its crossing bucket is the only one whose members have to be
+//      told apart, and goes to the list instead.  A bucket too full for that (thousands of equal logits): the threshold by bisection over
+//      the places, every step a question to all CTAs
 //   5  every CTA's kept mass; the CTA that holds the drawn number's place walks to it by sums over warps, lanes and elements
 #include "common.cuh"
 
 #include <cooperative_groups.h>
+
+#include <type_traits>
 
 namespace qmoe {
 namespace {
@@ -25,13 +28,13 @@ namespace {
 namespace cg = cooperative_groups;
 typedef unsigned long long u64;
 
-constexpr int kThreads = 512, kWarps = kThreads / 32;
 constexpr int kMaxCtas = 8;
-constexpr int kBuckets = 2048, kPerThread = kBuckets / kThreads;
-constexpr int kList = 1024;
+constexpr int kBuckets = 1024;
+constexpr int kList = 2048;
+constexpr int kTable = 2048;
 constexpr float kOne = 2147483648.f;     // 2^31: the mass of the largest logit's token
 constexpr float kLastZ = 22.25f;         // exp(-z) 2^31 < 1/2 from z = 22.2 on: no mass
-constexpr long long kMaxVocab = 2000000;         // eight slices of at most kBuckets sums of warps (Shared::table)
+constexpr long long kMaxVocab = 2000000;         // eight slices of at most kTable sums of warps
 constexpr int kMaxSlice = 160 * 1024;    // bytes of a row's slice in shared memory
 constexpr int kMaxHeld = 65536;          // its elements
 
@@ -50,14 +53,16 @@ struct SampleParams {
 
 enum { ASK_DONE = 0, ASK_LIST = 1, ASK_ABOVE = 2 };
 
-struct Shared {
-    u64 places[kMaxCtas], totals[kMaxCtas], passing[kMaxCtas], kept[kMaxCtas];   // of every CTA, in every CTA
-    u64 scratch[kWarps];
+template <int kThreads> struct Shared {
+    float tops[kMaxCtas];                // of every CTA, in every CTA
+    u64 totals[kMaxCtas], passing[kMaxCtas], kept[kMaxCtas];
+    u64 scratch[kThreads / 32];
     u64 answer_count[kMaxCtas], answer_mass[kMaxCtas];       // first CTA: answers to ASK_ABOVE
     u64 ask_place;                       // what the first CTA asks, in every CTA
     int ask, ask_bucket;
     int bound;                           // the last bucket that counts
-    unsigned listed;
+    unsigned members[kMaxCtas];          // of the list, from every CTA, in every CTA
+    u64 least, selected;
     union {
         struct {
             // this CTA's.  Masses in two halves of 16 bits, for which shared memory has an addition of its own, while 65536 of them
@@ -68,13 +73,17 @@ struct Shared {
                 u64 mass[kBuckets];
             };
         } own;
-        u64 table[kBuckets];             // step 5: sums of warps
+        struct {                         // first CTA, while no histogram is being made: places, and of a short list masses
+            u64 list[kList];
+            uint32_t list_mass[kThreads];
+        };
+        u64 table[kTable];               // step 5: sums of warps
     };
-    uint32_t count[kBuckets];            // first CTA: the cluster's, then of the buckets before
-    u64 mass[kBuckets];
-    u64 list_place[kList];
-    uint32_t list_mass[kList];
-    u64 least, selected;
+    uint32_t count[kBuckets];            // first CTA: the cluster's, of the buckets before
+    union {
+        u64 mass[kBuckets];
+        float maxima[kMaxCtas * kThreads];       // first CTA: of every thread
+    };
 };
 
 __device__ __forceinline__ uint32_t ordered(float x) {
@@ -85,61 +94,89 @@ __device__ __forceinline__ float logit_at(u64 place) {
     const uint32_t b = (uint32_t)(place >> 32);
     return __uint_as_float(b & 0x80000000u ? b & 0x7fffffffu : ~b);
 }
-__device__ __forceinline__ u64 place_of(float x, int i) { return (u64)ordered(x) << 32 | (0xffffffffu - (uint32_t)i); }
-// (x - largest) / T, in (-infinity, 0]; -infinity for a logit that is none
-__device__ __forceinline__ float exponent_of(float x, float largest, float inverse) {
+__device__ __forceinline__ u64 place_of(float x, int i) { return (u64)ordered(x + 0.f) << 32 | (0xffffffffu - (uint32_t)i); }     // + 0: one zero
+// (x - largest) / T, in (-infinity, 0]; -infinity for a logit that is none, NaN stays.  The product says all of that by itself unless the
+// largest logit is infinite or 1 / T is 0 or infinite (`odd`)
+__device__ __forceinline__ float exponent_of(float x, float largest, float inverse, bool odd) {
     const float apart = x - largest;
-    return x == largest ? 0.f : apart == -INFINITY ? -INFINITY : apart * inverse;
+    if (odd) return x == largest ? 0.f : apart == -INFINITY ? -INFINITY : apart * inverse;
+    return apart * inverse;
 }
-__device__ __forceinline__ uint32_t mass_of(float weight) { return __float2uint_rn(weight * kOne); }
+__device__ __forceinline__ uint32_t mass_of(float weight) { return __float2uint_rn(weight * kOne); }      // of NaN: 0
 __device__ __forceinline__ int bucket_of(float exponent) { return min(kBuckets - 1, (int)(exponent * (-kBuckets / kLastZ))); }
+__device__ __forceinline__ float max_of(const uint4& v, float so_far, __nv_bfloat16) {
+    const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&v);
+    const __nv_bfloat162 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+    return fmaxf(so_far, fmaxf(__low2float(m), __high2float(m)));
+}
+__device__ __forceinline__ float max_of(const uint4& v, float so_far, float) {
+    return fmaxf(so_far, fmaxf(fmaxf(__uint_as_float(v.x), __uint_as_float(v.y)), fmaxf(__uint_as_float(v.z), __uint_as_float(v.w))));
+}
 
+// over the warp, in every lane, in three parts of 24, 24 and 16 bits
 __device__ __forceinline__ u64 warp_sum64(u64 v) {
-#pragma unroll
-    for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    return v;
+    const uint32_t low = __reduce_add_sync(0xffffffffu, (uint32_t)v & 0xffffffu), mid = __reduce_add_sync(0xffffffffu, (uint32_t)(v >> 24) & 0xffffffu),
+                   high = __reduce_add_sync(0xffffffffu, (uint32_t)(v >> 48));
+    return (u64)low + ((u64)mid << 24) + ((u64)high << 48);
 }
 // over the block, in every thread
-__device__ u64 block_sum(u64 v, u64* scratch) {
+template <int kThreads> __device__ u64 block_sum(u64 v, u64* scratch) {
     v = warp_sum64(v);
     __syncthreads();
     if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = v;
     __syncthreads();
-    v = threadIdx.x % 32 < kWarps ? scratch[threadIdx.x % 32] : 0;
+    v = threadIdx.x % 32 < kThreads / 32 ? scratch[threadIdx.x % 32] : 0;
     return warp_sum64(v);
 }
-__device__ u64 block_max(u64 v, u64* scratch) {
-#pragma unroll
-    for (int o = 16; o; o >>= 1) v = max(v, __shfl_xor_sync(0xffffffffu, v, o));
+template <int kThreads> __device__ float block_max(float v, u64* scratch) {
+    float* values = reinterpret_cast<float*>(scratch);
+    v = warp_max(v);
     __syncthreads();
-    if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = v;
+    if ((threadIdx.x & 31) == 0) values[threadIdx.x >> 5] = v;
     __syncthreads();
-    v = threadIdx.x % 32 < kWarps ? scratch[threadIdx.x % 32] : 0;
-#pragma unroll
-    for (int o = 16; o; o >>= 1) v = max(v, __shfl_xor_sync(0xffffffffu, v, o));
-    return v;
+    return warp_max(values[threadIdx.x % (kThreads / 32)]);
 }
 // sum over the threads before this one
-__device__ u64 block_before(u64 v, u64* scratch) {
-    u64 upto = v;
+template <typename V> __device__ V block_before(V v, u64* scratch) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    V upto = v;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const u64 other = __shfl_up_sync(0xffffffffu, upto, o);
-        if ((int)(threadIdx.x & 31) >= o) upto += other;
+        const V other = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += other;
     }
     __syncthreads();
-    if ((threadIdx.x & 31) == 31) scratch[threadIdx.x >> 5] = upto;
+    if (lane == 31) scratch[warp] = upto;
     __syncthreads();
-    u64 before = upto - v;
-    for (int w = 0; w < (int)(threadIdx.x >> 5); ++w) before += scratch[w];
-    return before;
+    const u64 ahead = lane < warp ? scratch[lane] : 0;
+    return upto - v + (V)(sizeof(V) == 4 ? __reduce_add_sync(0xffffffffu, (uint32_t)ahead) : warp_sum64(ahead));
+}
+// list[0 .. n) in falling order; behind it zeros, up to a power of two.  Pairs at most 32 apart stay within a warp's 64 elements.
+template <int kThreads> __device__ void sort_falling(u64* list, unsigned n) {
+    unsigned padded = 64;
+    while (padded < n) padded *= 2;
+    __syncthreads();
+    for (unsigned i = n + threadIdx.x; i < padded; i += kThreads) list[i] = 0;
+    __syncthreads();
+    for (unsigned run = 2; run <= padded; run *= 2)
+        for (unsigned apart = run / 2; apart; apart /= 2) {
+            for (unsigned t = threadIdx.x; t < padded / 2; t += kThreads) {
+                const unsigned i = 2 * t - (t & (apart - 1)), j = i + apart;
+                const u64 a = list[i], b = list[j];
+                if ((a < b) == ((i & run) == 0)) { list[i] = b; list[j] = a; }
+            }
+            if (apart > 32 || (apart == 1 && run >= 64)) __syncthreads();
+            else __syncwarp();
+        }
+    __syncthreads();
 }
 
-template <typename T, bool HELD>
-__global__ void __launch_bounds__(kThreads)
+template <typename T, bool HELD, int kThreads>
+__global__ void __launch_bounds__(kThreads, 1024 / kThreads)
 sample_kernel(const __grid_constant__ SampleParams p) {
     chain_begin();
-    constexpr int N = Vec16<T>::N;
+    constexpr int N = Vec16<T>::N, kWarps = kThreads / 32, kPerThread = kBuckets / kThreads;
+    using Shared = Shared<kThreads>;
     extern __shared__ __align__(16) uint8_t smem[];
     Shared& s = *reinterpret_cast<Shared*>(smem);
     uint4* held = reinterpret_cast<uint4*>(smem + (sizeof(Shared) + 15) / 16 * 16);
@@ -147,25 +184,24 @@ sample_kernel(const __grid_constant__ SampleParams p) {
     const int ctas = (int)cluster.num_blocks(), rank = (int)cluster.block_rank(), lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const long long row = blockIdx.x / ctas;
     cluster.barrier_arrive();            // waited for ahead of the first store to another CTA: by then all of them run
-    // the row in pieces of 16 bytes from the 16-byte boundary at or before its start: element i of piece v is token N v + i - lead
+    // the row in pieces of 16 bytes from the 16-byte boundary at or before its start: element i of piece v is token N v + i - lead.  A
+    // thread has the same pieces throughout.
     const T* const x = (const T*)p.logits + row * p.vocab;
     const int lead = (int)(((uintptr_t)x & 15u) / sizeof(T));
     const int first_piece = rank * (p.slice / N), pieces = p.slice / N;
-    auto fetch = [&](int v, float* f) {
-        const int at = (first_piece + v) * N - lead;
-        if (at >= 0 && at + N <= p.vocab) {
-            Vec16<T>::unpack(*reinterpret_cast<const uint4*>(x + at), f);
-        } else {
+    auto token_of = [&](int v, int i) { return (first_piece + v) * N + i - lead; };
+    auto inside = [&](int v) { return token_of(v, 0) >= 0 && token_of(v, N) <= p.vocab; };
+    auto gather = [&](int v) {           // a piece at the row's ends, or beyond: -infinity where there is no token
+        float f[N];
 #pragma unroll
-            for (int i = 0; i < N; ++i) f[i] = at + i >= 0 && at + i < p.vocab ? Act<T>::load(x + at + i) : -INFINITY;
-        }
-#pragma unroll
-        for (int i = 0; i < N; ++i) f[i] = isnan(f[i]) ? -INFINITY : f[i] + 0.f;      // + 0: one zero
+        for (int i = 0; i < N; ++i) f[i] = token_of(v, i) >= 0 && token_of(v, i) < p.vocab ? Act<T>::load(x + token_of(v, i)) : -INFINITY;
+        return Vec16<T>::pack(f);
     };
-    auto piece = [&](int v, float* f) {
-        if constexpr (HELD) Vec16<T>::unpack(held[v], f);
-        else fetch(v, f);
+    auto raw = [&](int v) -> uint4 {
+        if constexpr (HELD) return held[v];
+        else return inside(v) ? *reinterpret_cast<const uint4*>(x + token_of(v, 0)) : gather(v);
     };
+    auto piece = [&](int v, float* f) { Vec16<T>::unpack(raw(v), f); };
     auto add = [&](int b, uint32_t mass) {
         atomicAdd(&s.own.count[b], 1u);
         if constexpr (HELD) {
@@ -175,62 +211,104 @@ sample_kernel(const __grid_constant__ SampleParams p) {
             atomicAdd(&s.own.mass[b], (u64)mass);
         }
     };
-    auto token_of = [&](int v, int i) { return (first_piece + v) * N + i - lead; };
-
+    auto own_mass = [&](const Shared* of, int b) -> u64 {
+        if constexpr (HELD) return (u64)of->own.low[b] + ((u64)of->own.high[b] << 16);
+        else return of->own.mass[b];
+    };
+    if constexpr (HELD) {
+        for (int v = threadIdx.x; v < pieces; v += kThreads) {
+            if (inside(v)) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(held + v)), "l"(x + token_of(v, 0)) : "memory");
+            else held[v] = gather(v);
+        }
+    }
     const float temperature = p.temperatures ? p.temperatures[row] : p.temperature;
     const float top_p = p.top_ps ? p.top_ps[row] : p.top_p, min_p = fminf(p.min_ps ? p.min_ps[row] : p.min_p, 1.f);
     const bool greedy = !(temperature > 0.f);
     const float inverse = greedy ? 1.f : __fdiv_rn(1.f, temperature);
     const int top_k = greedy ? 1 : p.top_ks ? p.top_ks[row] : p.top_k;
+    const bool one = top_k == 1, by_count = top_k > 1 && top_k < p.vocab, by_mass = !one && !(top_p >= 1.f);
+    const float uniform = p.uniforms[row];
+    if (by_count || by_mass)
+        for (int b = threadIdx.x; b < kBuckets; b += kThreads) s.own.count[b] = s.own.low[b] = s.own.high[b] = 0;
+    if constexpr (HELD) asm volatile("cp.async.wait_all;" ::: "memory");
 
     // 1
-    float most = -INFINITY;
-    int most_at = 0;
-    for (int v = threadIdx.x; v < pieces; v += kThreads) {
-        float f[N];
-        fetch(v, f);
-        if constexpr (HELD) held[v] = Vec16<T>::pack(f);
-#pragma unroll
-        for (int i = 0; i < N; ++i)
-            if (f[i] > most) { most = f[i]; most_at = token_of(v, i); }
-    }
-    u64 place = block_max(place_of(most, most_at), s.scratch);
+    Shared* const first_cta = cluster.map_shared_rank(&s, 0);
+    float largest = -INFINITY;
+    for (int v = threadIdx.x; v < pieces; v += kThreads) largest = max_of(raw(v), largest, T());
     cluster.barrier_wait();
-    if (threadIdx.x < ctas) cluster.map_shared_rank(&s, threadIdx.x)->places[rank] = place;
-    for (int b = threadIdx.x; b < kBuckets; b += kThreads) s.own.count[b] = s.own.low[b] = s.own.high[b] = 0;
-    if (threadIdx.x == 0) s.listed = 0;
+    if (by_count || by_mass) first_cta->maxima[rank * kThreads + threadIdx.x] = largest;
+    largest = block_max<kThreads>(largest, s.scratch);
+    if (threadIdx.x < ctas) cluster.map_shared_rank(&s, threadIdx.x)->tops[rank] = largest;
     cluster.sync();
-    for (int c = 0; c < ctas; ++c) place = max(place, s.places[c]);
-    const float largest = logit_at(place);
+    for (int c = 0; c < ctas; ++c) largest = fmaxf(largest, s.tops[c]);
     if (largest == -INFINITY) {
         if (rank == 0 && threadIdx.x == 0) { p.tokens[row] = -1; p.log_probs[row] = -INFINITY; }
-        cluster.sync();
         return;
     }
+    const bool odd = largest == INFINITY || inverse == INFINITY || inverse == 0.f;
+    auto exponent = [&](float f) { return exponent_of(f, largest, inverse, odd); };
     // 2
     u64 total = 0, passing = 0;
-    for (int v = threadIdx.x; v < pieces; v += kThreads) {
-        float f[N];
-        piece(v, f);
+    auto weigh = [&](auto any_odd, auto any_min) {
+        for (int v = threadIdx.x; v < pieces; v += kThreads) {
+            float f[N];
+            piece(v, f);
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const float weight = expf(exponent_of(f[i], largest, inverse));
-            const uint32_t mass = mass_of(weight);
-            total += mass;
-            if (!(weight < min_p)) passing += mass;
+            for (int i = 0; i < N; ++i) {
+                const float weight = expf(exponent_of(f[i], largest, inverse, any_odd.value));
+                const uint32_t mass = mass_of(weight);
+                total += mass;
+                if (any_min.value && !(weight < min_p)) passing += mass;
+            }
         }
-    }
-    const bool one = top_k == 1, by_count = top_k > 1 && top_k < p.vocab, by_mass = !one && !(top_p >= 1.f);
-    if (by_count || by_mass) {
-        const float exponent = exponent_of(most, largest, inverse);
-        const uint32_t mass = mass_of(expf(exponent));
-        if (mass) {
-            const int b = bucket_of(exponent);
-            add(b, mass);
+    };
+    // 3: the first CTA; top-k's bound needs no masses' sum and comes along with it
+    auto find_bound = [&]() {
+        for (int i = threadIdx.x; i < ctas * kThreads; i += kThreads) {
+            const float e = exponent(s.maxima[i]);
+            if (!(e > -kLastZ)) continue;
+            const uint32_t mass = mass_of(expf(e));
+            if (!mass) continue;
+            if (by_count) atomicAdd(&s.own.count[bucket_of(e)], 1u);
+            else add(bucket_of(e), mass);
         }
-    }
-    total = block_sum(total, s.scratch);
-    passing = block_sum(passing, s.scratch);
+        __syncthreads();
+        // a thread's buckets: the first that reaches what is wanted, together with all before
+        uint32_t count[kPerThread], counts = 0;
+        u64 mass[kPerThread], masses = 0;
+#pragma unroll
+        for (int i = 0; i < kPerThread; ++i) {
+            counts += count[i] = s.own.count[threadIdx.x * kPerThread + i];
+            if (!by_count) masses += mass[i] = own_mass(&s, threadIdx.x * kPerThread + i);
+        }
+        const uint32_t mine = counts;
+        counts = block_before(counts, s.scratch);
+        if (!by_count) masses = block_before(masses, s.scratch);
+        // no bound: all tokens, if few threads have one with a mass, or no list
+        if (threadIdx.x == kThreads - 1) s.bound = counts + mine <= kList / 8 ? kBuckets - 1 : kBuckets;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < kPerThread; ++i) {
+            counts += count[i];
+            if (!by_count) masses += mass[i];
+            if (by_count ? counts >= (uint32_t)top_k : (double)masses >= (double)top_p * (double)total) {
+                atomicMin(&s.bound, threadIdx.x * kPerThread + i);
+                break;
+            }
+        }
+        __syncthreads();
+        if (threadIdx.x < ctas) cluster.map_shared_rank(&s, threadIdx.x)->bound = s.bound;
+    };
+    if (by_count && rank == 0) find_bound();
+    using Yes = std::true_type;
+    using No = std::false_type;
+    if (odd) weigh(Yes(), Yes());
+    else if (min_p > 0.f) weigh(No(), Yes());
+    else weigh(No(), No());
+    if (odd || min_p > 0.f) passing = block_sum<kThreads>(passing, s.scratch);
+    total = block_sum<kThreads>(total, s.scratch);
+    if (!odd && !(min_p > 0.f)) passing = total;
     if (threadIdx.x < ctas) {
         Shared* other = cluster.map_shared_rank(&s, threadIdx.x);
         other->totals[rank] = total;
@@ -239,79 +317,235 @@ sample_kernel(const __grid_constant__ SampleParams p) {
     cluster.sync();
     total = passing = 0;
     for (int c = 0; c < ctas; ++c) { total += s.totals[c]; passing += s.passing[c]; }
+    auto finish = [&](int token, float f) {
+        p.tokens[row] = token;
+        p.log_probs[row] = (float)((double)exponent(f) - log((double)total / (double)kOne));
+    };
+    auto target_of = [&](u64 all) -> u64 {
+        const long long drawn = (long long)((double)uniform * (double)all);
+        return one ? 0 : (u64)max(0ll, min(drawn, (long long)all - 1));
+    };
 
-    u64 first = one ? place : 0;         // the least place that is kept
+    u64 first = one ? (u64)ordered(largest + 0.f) << 32 : 0;         // the least place that is kept
     // top-p cuts into what min-p lets through only if that holds more than p of the mass
     const bool cut = by_count || (by_mass && !((double)passing <= (double)top_p * (double)total));
     if (cut) {
-        Shared* lead_cta = cluster.map_shared_rank(&s, 0);
-        // the cluster's histogram, an eighth of it by every CTA, and in the first CTA the sums of the buckets before
-        auto merge = [&]() {
-            const int share = kBuckets / ctas;
-            for (int b = rank * share + threadIdx.x; b < (rank + 1) * share; b += kThreads) {
-                uint32_t count = 0;
-                u64 mass = 0;
-                for (int c = 0; c < ctas; ++c) {
-                    const Shared* other = cluster.map_shared_rank(&s, c);
-                    count += other->own.count[b];
-                    if constexpr (HELD) mass += (u64)other->own.low[b] + ((u64)other->own.high[b] << 16);
-                    else mass += other->own.mass[b];
+        // 3, by mass
+        if (!by_count) {
+            if (rank == 0) find_bound();
+            cluster.sync();
+        }
+        const int bound = s.bound;
+        // The members of bucket `only`, or of all up to the bound, to the first CTA's list, if it holds them: counted first, so that everyone
+        // knows their place.  Their number.
+        auto enlist = [&](int only) -> unsigned {
+            auto member = [&](float e) {
+                if (!(e > -kLastZ)) return false;
+                const int b = bucket_of(e);
+                return (only < 0 ? b <= bound : b == only) && mass_of(expf(e)) != 0;
+            };
+            unsigned mine = 0;
+            for (int v = threadIdx.x; v < pieces; v += kThreads) {
+                float f[N];
+                piece(v, f);
+#pragma unroll
+                for (int i = 0; i < N; ++i) mine += member(exponent(f[i]));
+            }
+            unsigned to = block_before(mine, s.scratch);
+            if (threadIdx.x == kThreads - 1)
+#pragma unroll
+                for (int c = 0; c < kMaxCtas; ++c)
+                    if (c < ctas) cluster.map_shared_rank(&s, c)->members[rank] = to + mine;
+            cluster.sync();
+            unsigned n = 0;
+#pragma unroll
+            for (int c = 0; c < kMaxCtas; ++c) {
+                if (c == rank) to += n;
+                if (c < ctas) n += s.members[c];
+            }
+            if (n <= kList && mine) {
+                for (int v = threadIdx.x; v < pieces; v += kThreads) {
+                    float f[N];
+                    piece(v, f);
+#pragma unroll
+                    for (int i = 0; i < N; ++i) {
+                        const float e = exponent(f[i]);
+                        if (!member(e)) continue;
+                        first_cta->list[to++] = place_of(f[i], token_of(v, i));
+                    }
                 }
-                lead_cta->count[b] = count;
-                lead_cta->mass[b] = mass;
             }
             cluster.sync();
-            if (rank == 0) {
-                u64 counts = 0, masses = 0;
-                for (int i = 0; i < kPerThread; ++i) { counts += s.count[threadIdx.x * kPerThread + i]; masses += s.mass[threadIdx.x * kPerThread + i]; }
-                counts = block_before(counts, s.scratch);
-                masses = block_before(masses, s.scratch);
-                for (int i = 0; i < kPerThread; ++i) {
-                    const int b = threadIdx.x * kPerThread + i;
-                    const uint32_t count = s.count[b];
-                    const u64 mass = s.mass[b];
-                    s.count[b] = (uint32_t)counts;
-                    s.mass[b] = masses;
-                    counts += count;
-                    masses += mass;
-                }
-                __syncthreads();
-            }
+            return n;
         };
-        merge();
-        // 3
-        if (rank == 0) {
-            if (threadIdx.x == 0) s.bound = kBuckets - 1;
+        auto weight_at = [&](u64 at) { return expf(exponent(logit_at(at))); };
+        // Of the first CTA's sorted list: kept by count, the number before (and `base` of them ahead of the list) below `limit`; by mass, the mass
+        // before 0 or below `threshold`.  The least place that is kept, all ones for none; `selected` becomes the kept members' mass.
+        constexpr int EACH = kList / kThreads;
+        auto least_kept = [&](unsigned n, bool counts, u64 base, u64 limit, double threshold) {
+            if (threadIdx.x == 0) { s.least = ~0ull; s.selected = 0; }
+            u64 mass[EACH], sum = 0;
+            const unsigned begin = threadIdx.x * EACH;
+#pragma unroll
+            for (int i = 0; i < EACH; ++i) sum += mass[i] = begin + i < n ? mass_of(weight_at(s.list[begin + i])) : 0;
+            const u64 mass_before = block_before(sum, s.scratch);
+            u64 before = mass_before;
+            int kept = 0;
+#pragma unroll
+            for (int i = 0; i < EACH; ++i) {
+                const u64 so_far = base + (counts ? begin + i : before);
+                if (begin + i < n && (counts ? so_far < limit : so_far == 0 || (double)so_far < threshold)) {
+                    before += mass[i];
+                    ++kept;
+                }
+            }
+            // what is kept is a run from the front: its last member says where it ends
+            if (kept && (kept < EACH || begin + EACH >= n)) { s.least = s.list[begin + kept - 1]; s.selected = before; }
+            if (kept == EACH && begin + EACH < n) {
+                const u64 so_far = base + (counts ? begin + EACH : before);
+                if (!(counts ? so_far < limit : (double)so_far < threshold)) { s.least = s.list[begin + EACH - 1]; s.selected = before; }
+            }
             __syncthreads();
-            for (int b = threadIdx.x; b < kBuckets - 1; b += kThreads)
-                if (by_count ? s.count[b + 1] >= (uint32_t)top_k : (double)s.mass[b + 1] >= (double)top_p * (double)total) atomicMin(&s.bound, b);
-            __syncthreads();
-            if (threadIdx.x < ctas) cluster.map_shared_rank(&s, threadIdx.x)->bound = s.bound;
+        };
+        if (bound < kBuckets) {          // everything that can be kept, if the list holds it
+            const unsigned n = enlist(-1);
+            if (n <= kList) {            // the first CTA alone goes on
+                if (rank) return;
+                if (n <= kThreads) {     // a short list: every member compared with all others, by as many lanes as there are for each
+                    int bits = 0;
+                    while (bits < 5 && n << (bits + 1) <= kThreads) ++bits;
+                    const unsigned me = threadIdx.x >> bits, of = 1u << bits;
+                    const u64 at = me < n ? s.list[me] : 0;
+                    const float weight = me < n ? weight_at(at) : 0.f;
+                    const uint32_t mass = mass_of(weight);
+                    const bool leads = me < n && (threadIdx.x & (of - 1)) == 0;
+                    if (leads) s.list_mass[me] = mass;
+                    __syncthreads();
+                    unsigned ahead = 0;
+                    u64 mass_ahead = 0, behind = 0;
+                    for (unsigned j = threadIdx.x & (of - 1); j < n; j += of)
+                        if (s.list[j] > at) {
+                            ++ahead;
+                            mass_ahead += s.list_mass[j];
+                        }
+                    for (unsigned o = 1; o < of; o <<= 1) {
+                        ahead += __shfl_xor_sync(0xffffffffu, ahead, o);
+                        mass_ahead += __shfl_xor_sync(0xffffffffu, mass_ahead, o);
+                    }
+                    bool keep = !by_count || ahead < (unsigned)top_k;
+                    if (by_mass) {
+                        const u64 whole = by_count ? block_sum<kThreads>(leads && keep ? mass : 0u, s.scratch) : total;
+                        keep = keep && (mass_ahead == 0 || (double)mass_ahead < (double)top_p * (double)whole);
+                    }
+                    const uint32_t kept = leads && keep && !(weight < min_p) ? mass : 0u;
+                    const u64 target = target_of(block_sum<kThreads>(kept, s.scratch));
+                    if (leads) s.list_mass[me] = kept;
+                    __syncthreads();
+                    for (unsigned j = threadIdx.x & (of - 1); j < n; j += of)      // by index: the places' lower halves fall with it
+                        if ((uint32_t)s.list[j] > (uint32_t)at) behind += s.list_mass[j];
+                    for (unsigned o = 1; o < of; o <<= 1) behind += __shfl_xor_sync(0xffffffffu, behind, o);
+                    if (kept && target >= behind && target < behind + kept) finish((int)(0xffffffffu - (uint32_t)at), logit_at(at));
+                    return;
+                }
+                sort_falling<kThreads>(s.list, n);
+                u64 whole = total;
+                if (by_count) {
+                    least_kept(n, true, 0, (u64)top_k, 0.0);
+                    first = s.least;
+                    whole = s.selected;
+                    __syncthreads();
+                }
+                if (by_mass) {
+                    least_kept(n, false, 0, 0, (double)top_p * (double)whole);
+                    first = max(first, s.least);
+                    __syncthreads();
+                }
+                // the kept ones by index: their places' lower halves fall with it.  A place turned about, upper half for lower
+                for (unsigned i = threadIdx.x; i < n; i += kThreads) {
+                    const u64 at = s.list[i];
+                    s.list[i] = at >= first && !(weight_at(at) < min_p) ? at << 32 | at >> 32 : 0;
+                }
+                sort_falling<kThreads>(s.list, n);
+                u64 sum = 0;
+                uint32_t mass[EACH];
+                const unsigned begin = threadIdx.x * EACH;
+#pragma unroll
+                for (int i = 0; i < EACH; ++i) {
+                    const u64 turned = begin + i < n ? s.list[begin + i] : 0;
+                    sum += mass[i] = turned ? mass_of(weight_at(turned << 32)) : 0u;
+                }
+                u64 before = block_before(sum, s.scratch);
+                if (threadIdx.x == kThreads - 1) s.selected = before + sum;
+                __syncthreads();
+                const u64 target = target_of(s.selected);
+#pragma unroll
+                for (int i = 0; i < EACH; ++i) {
+                    if (target >= before && target < before + mass[i]) {
+                        const u64 turned = s.list[begin + i];
+                        finish((int)(0xffffffffu - (uint32_t)(turned >> 32)), logit_at(turned << 32));
+                    }
+                    before += mass[i];
+                }
+                return;
+            }
         }
-        cluster.sync();
-        const int bound = s.bound;
+        // 4
+        // sums of the buckets before, in place
+        auto accumulate = [&]() {
+            __syncthreads();
+            u64 counts = 0, masses = 0, mass[kPerThread];
+            uint32_t count[kPerThread];
+#pragma unroll
+            for (int i = 0; i < kPerThread; ++i) {
+                counts += count[i] = s.count[threadIdx.x * kPerThread + i];
+                masses += mass[i] = s.mass[threadIdx.x * kPerThread + i];
+            }
+            counts = block_before(counts, s.scratch);
+            masses = block_before(masses, s.scratch);
+#pragma unroll
+            for (int i = 0; i < kPerThread; ++i) {
+                const int b = threadIdx.x * kPerThread + i;
+                s.count[b] = (uint32_t)counts;
+                s.mass[b] = masses;
+                counts += count[i];
+                masses += mass[i];
+            }
+            __syncthreads();
+        };
+        __syncthreads();
         for (int b = threadIdx.x; b < kBuckets; b += kThreads) s.own.count[b] = s.own.low[b] = s.own.high[b] = 0;
         __syncthreads();
-        // 4
         for (int v = threadIdx.x; v < pieces; v += kThreads) {
             float f[N];
             piece(v, f);
 #pragma unroll
             for (int i = 0; i < N; ++i) {
-                const float exponent = exponent_of(f[i], largest, inverse);
-                if (!(exponent > -kLastZ)) continue;
-                const int b = bucket_of(exponent);
+                const float e = exponent(f[i]);
+                if (!(e > -kLastZ)) continue;
+                const int b = bucket_of(e);
                 if (b > bound) continue;
-                const uint32_t mass = mass_of(expf(exponent));
-                if (!mass) continue;
-                add(b, mass);
+                const uint32_t mass = mass_of(expf(e));
+                if (mass) add(b, mass);
             }
         }
         cluster.sync();
-        merge();
+        // the cluster's, an equal share of the buckets by every CTA
+        for (int b = rank * (kBuckets / ctas) + threadIdx.x; b < (rank + 1) * (kBuckets / ctas); b += kThreads) {
+            uint32_t count = 0;
+            u64 mass = 0;
+#pragma unroll
+            for (int c = 0; c < kMaxCtas; ++c)
+                if (c < ctas) {
+                    const Shared* other = cluster.map_shared_rank(&s, c);
+                    count += other->own.count[b];
+                    mass += own_mass(other, b);
+                }
+            first_cta->count[b] = count;
+            first_cta->mass[b] = mass;
+        }
+        cluster.sync();
         // The first CTA leads: it asks for a bucket's members, or what lies above a place, until it knows the threshold.
         auto ask = [&](int what, int bucket, u64 at) {          // by the first CTA; every CTA then answers in `answer`
-            if (threadIdx.x == 0) s.listed = 0;
             if (threadIdx.x < ctas) {
                 Shared* other = cluster.map_shared_rank(&s, threadIdx.x);
                 other->ask = what;
@@ -319,48 +553,40 @@ sample_kernel(const __grid_constant__ SampleParams p) {
                 other->ask_place = at;
             }
         };
+        unsigned listed = 0;
         auto answer = [&]() {
             cluster.sync();
-            const int what = s.ask, bucket = s.ask_bucket;
-            const u64 at = s.ask_place;
+            const int what = s.ask;
             if (what == ASK_DONE) return false;
-            u64 count = 0, mass = 0;
-            for (int v = threadIdx.x; v < pieces; v += kThreads) {
-                float f[N];
-                piece(v, f);
+            if (what == ASK_LIST) {
+                listed = enlist(s.ask_bucket);
+            } else {
+                const u64 at = s.ask_place;
+                u64 count = 0, mass = 0;
+                for (int v = threadIdx.x; v < pieces; v += kThreads) {
+                    float f[N];
+                    piece(v, f);
 #pragma unroll
-                for (int i = 0; i < N; ++i) {
-                    const float exponent = exponent_of(f[i], largest, inverse);
-                    if (!(exponent > -kLastZ)) continue;
-                    if (what == ASK_LIST) {
-                        if (bucket_of(exponent) != bucket) continue;
-                        const uint32_t m = mass_of(expf(exponent));
-                        if (!m) continue;
-                        const unsigned to = atomicAdd(&lead_cta->listed, 1u);
-                        if (to < kList) {
-                            lead_cta->list_place[to] = place_of(f[i], token_of(v, i));
-                            lead_cta->list_mass[to] = m;
-                        }
-                    } else if (place_of(f[i], token_of(v, i)) > at) {
-                        const uint32_t m = mass_of(expf(exponent));
+                    for (int i = 0; i < N; ++i) {
+                        const float e = exponent(f[i]);
+                        if (!(e > -kLastZ) || place_of(f[i], token_of(v, i)) <= at) continue;
+                        const uint32_t m = mass_of(expf(e));
                         count += m != 0;
                         mass += m;
                     }
                 }
+                count = block_sum<kThreads>(count, s.scratch);
+                mass = block_sum<kThreads>(mass, s.scratch);
+                if (threadIdx.x == 0) { first_cta->answer_count[rank] = count; first_cta->answer_mass[rank] = mass; }
+                cluster.sync();
             }
-            if (what == ASK_ABOVE) {
-                count = block_sum(count, s.scratch);
-                mass = block_sum(mass, s.scratch);
-                if (threadIdx.x == 0) { lead_cta->answer_count[rank] = count; lead_cta->answer_mass[rank] = mass; }
-            }
-            cluster.sync();
             return true;
         };
         if (rank == 0) {
+            accumulate();
             u64 whole = total;           // of what top-k keeps
             int listed_bucket = -1;
-            // kept by count: the number before is below `limit`; by mass: the mass before is 0 or below `threshold`
-            auto threshold_of = [&](bool counts, u64 limit, double threshold) {
+            auto threshold_of = [&](bool counts, u64 limit, double threshold) -> u64 {
                 auto keeps = [&](u64 before) { return counts ? before < limit : before == 0 || (double)before < threshold; };
                 // the last bucket whose first member is kept
                 if (threadIdx.x == 0) s.bound = 0;
@@ -378,42 +604,28 @@ sample_kernel(const __grid_constant__ SampleParams p) {
                     answer();
                     listed_bucket = bucket;
                 }
-                const unsigned n = s.listed;
+                const unsigned n = listed;
                 if (n > kList) {         // too many to compare with one another
-                    u64 c = 0, above = 0;
+                    u64 c = 0;
                     for (int bit = 63; bit >= 0; --bit) {
                         ask(ASK_ABOVE, 0, c | ((1ull << bit) - 1));
                         answer();
-                        u64 count = 0, mass = 0;
-                        for (int r = 0; r < ctas; ++r) { count += s.answer_count[r]; mass += s.answer_mass[r]; }
-                        if (!keeps(counts ? count : mass)) c |= 1ull << bit;
-                        else above = mass;
+                        u64 before = 0;
+                        for (int r = 0; r < ctas; ++r) before += counts ? s.answer_count[r] : s.answer_mass[r];
+                        if (!keeps(before)) c |= 1ull << bit;
                     }
                     listed_bucket = -1;
                     if (counts && c) {   // the mass that is kept: of the places from c on
                         ask(ASK_ABOVE, 0, c - 1);
                         answer();
-                        above = 0;
-                        for (int r = 0; r < ctas; ++r) above += s.answer_mass[r];
-                        whole = above;
+                        whole = 0;
+                        for (int r = 0; r < ctas; ++r) whole += s.answer_mass[r];
                     }
                     return c;
                 }
-                if (threadIdx.x == 0) { s.least = ~0ull; s.selected = 0; }
-                __syncthreads();
-                const u64 count_before = s.count[bucket], mass_before = s.mass[bucket];
-                for (unsigned i = threadIdx.x; i < n; i += kThreads) {
-                    const u64 mine = s.list_place[i];
-                    u64 before = counts ? count_before : mass_before;
-                    for (unsigned j = 0; j < n; ++j)
-                        if (s.list_place[j] > mine) before += counts ? 1u : s.list_mass[j];
-                    if (keeps(before)) {
-                        atomicMin(&s.least, mine);
-                        atomicAdd(&s.selected, (u64)s.list_mass[i]);
-                    }
-                }
-                __syncthreads();
-                if (counts) whole = mass_before + s.selected;
+                sort_falling<kThreads>(s.list, n);
+                least_kept(n, counts, counts ? (u64)s.count[bucket] : s.mass[bucket], limit, threshold);
+                if (counts) whole = s.mass[bucket] + s.selected;
                 const u64 c = n ? s.least : 0;      // an empty last bucket: everything is kept
                 __syncthreads();
                 return c;
@@ -429,9 +641,9 @@ sample_kernel(const __grid_constant__ SampleParams p) {
     }
     // 5
     auto kept_of = [&](float f, int v, int i) -> uint32_t {
-        const float exponent = exponent_of(f, largest, inverse);
-        if (!(exponent > -kLastZ) || place_of(f, token_of(v, i)) < first) return 0u;
-        const float weight = expf(exponent);
+        const float e = exponent(f);
+        if (!(e > -kLastZ) || place_of(f, token_of(v, i)) < first) return 0u;
+        const float weight = expf(e);
         return weight < min_p ? 0u : mass_of(weight);
     };
     u64 sum = 0, before = 0, all = 0;
@@ -442,7 +654,7 @@ sample_kernel(const __grid_constant__ SampleParams p) {
 #pragma unroll
             for (int i = 0; i < N; ++i) sum += kept_of(f[i], v, i);
         }
-        sum = block_sum(sum, s.scratch);
+        sum = block_sum<kThreads>(sum, s.scratch);
         if (threadIdx.x < ctas) cluster.map_shared_rank(&s, threadIdx.x)->kept[rank] = sum;
         cluster.sync();
     }
@@ -451,80 +663,68 @@ sample_kernel(const __grid_constant__ SampleParams p) {
         if (c == rank) { before = all; sum = share; }
         all += share;
     }
-    long long drawn = (long long)((double)p.uniforms[row] * (double)all);
-    drawn = max(0ll, min(drawn, (long long)all - 1));
-    const u64 target = (u64)drawn;
-    if (target >= before && target < before + sum) {         // the same for the whole CTA
-        const int rounds = (pieces + kThreads - 1) / kThreads;
-        for (int r = 0; r < rounds; ++r) {
-            const int v = r * kThreads + threadIdx.x;
-            u64 mine = 0;
-            if (v < pieces) {
-                float f[N];
-                piece(v, f);
+    const u64 target = target_of(all);
+    if (target < before || target >= before + sum) return;          // another CTA's
+    const int rounds = (pieces + kThreads - 1) / kThreads;
+    for (int r = 0; r < rounds; ++r) {
+        const int v = r * kThreads + threadIdx.x;
+        u64 mine = 0;
+        if (v < pieces) {
+            float f[N];
+            piece(v, f);
 #pragma unroll
-                for (int i = 0; i < N; ++i) mine += kept_of(f[i], v, i);
-            }
-            mine = warp_sum64(mine);
-            if (lane == 0) s.table[r * kWarps + warp] = mine;
+            for (int i = 0; i < N; ++i) mine += kept_of(f[i], v, i);
         }
-        __syncthreads();
-        if (warp == 0) {
-            // the warp's share of the table: 32 sums at a time
-            for (int at = 0; at < rounds * kWarps; at += 32) {
-                const u64 mine = at + lane < rounds * kWarps ? s.table[at + lane] : 0;
-                u64 upto = mine;
-#pragma unroll
-                for (int o = 1; o < 32; o <<= 1) {
-                    const u64 other = __shfl_up_sync(0xffffffffu, upto, o);
-                    if (lane >= o) upto += other;
-                }
-                const unsigned hit = __ballot_sync(0xffffffffu, before + upto > target);
-                if (!hit) {
-                    before += __shfl_sync(0xffffffffu, upto, 31);
-                    continue;
-                }
-                const int which = __ffs(hit) - 1;
-                before += __shfl_sync(0xffffffffu, upto - mine, which);
-                const int entry = at + which, v = entry / kWarps * kThreads + entry % kWarps * 32 + lane;
-                float f[N];
-                uint32_t masses[N];
-                u64 lane_sum = 0;
-#pragma unroll
-                for (int i = 0; i < N; ++i) masses[i] = 0;
-                if (v < pieces) {
-                    piece(v, f);
-#pragma unroll
-                    for (int i = 0; i < N; ++i) lane_sum += masses[i] = kept_of(f[i], v, i);
-                }
-                u64 lane_upto = lane_sum;
-#pragma unroll
-                for (int o = 1; o < 32; o <<= 1) {
-                    const u64 other = __shfl_up_sync(0xffffffffu, lane_upto, o);
-                    if (lane >= o) lane_upto += other;
-                }
-                u64 running = before + lane_upto - lane_sum;
-                if (target >= running && target < running + lane_sum) {
-#pragma unroll
-                    for (int i = 0; i < N; ++i) {
-                        if (target >= running && target < running + masses[i]) {
-                            p.tokens[row] = token_of(v, i);
-                            p.log_probs[row] = (float)((double)exponent_of(f[i], largest, inverse) - log((double)total / (double)kOne));
-                        }
-                        running += masses[i];
-                    }
-                }
-                break;
-            }
-        }
+        mine = warp_sum64(mine);
+        if (lane == 0) s.table[r * kWarps + warp] = mine;
     }
-    cluster.sync();                      // nobody leaves while its shared memory is being read
+    __syncthreads();
+    if (warp) return;
+    // the warp's share of the table: 32 sums at a time
+    for (int at = 0; at < rounds * kWarps; at += 32) {
+        const u64 mine = at + lane < rounds * kWarps ? s.table[at + lane] : 0;
+        u64 upto = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const u64 other = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += other;
+        }
+        const unsigned hit = __ballot_sync(0xffffffffu, before + upto > target);
+        if (!hit) {
+            before += __shfl_sync(0xffffffffu, upto, 31);
+            continue;
+        }
+        const int which = __ffs(hit) - 1;
+        before += __shfl_sync(0xffffffffu, upto - mine, which);
+        const int entry = at + which, v = entry / kWarps * kThreads + entry % kWarps * 32 + lane;
+        float f[N];
+        uint32_t masses[N];
+        u64 lane_sum = 0;
+        if (v < pieces) piece(v, f);
+#pragma unroll
+        for (int i = 0; i < N; ++i) lane_sum += masses[i] = v < pieces ? kept_of(f[i], v, i) : 0u;
+        u64 running = lane_sum;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const u64 other = __shfl_up_sync(0xffffffffu, running, o);
+            if (lane >= o) running += other;
+        }
+        running += before - lane_sum;
+        if (target >= running && target < running + lane_sum) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                if (target >= running && target < running + masses[i]) finish(token_of(v, i), f[i]);
+                running += masses[i];
+            }
+        }
+        return;
+    }
 }
 
-template <typename T, bool HELD>
+template <typename T, bool HELD, int kThreads>
 int launch(const SampleParams& p, int ctas, long long rows, cudaStream_t stream) {
-    const size_t shared = (sizeof(Shared) + 15) / 16 * 16 + (HELD ? (size_t)p.slice * sizeof(T) : 0);
-    QMOE_CUDA(cudaFuncSetAttribute(sample_kernel<T, HELD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)shared));
+    const size_t shared = (sizeof(Shared<kThreads>) + 15) / 16 * 16 + (HELD ? (size_t)p.slice * sizeof(T) : 0);
+    QMOE_CUDA(cudaFuncSetAttribute(sample_kernel<T, HELD, kThreads>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)shared));
     cudaLaunchAttribute attributes[2] = {chain_attribute(), {}};
     attributes[1].id = cudaLaunchAttributeClusterDimension;
     attributes[1].val.clusterDim.x = ctas;
@@ -536,7 +736,7 @@ int launch(const SampleParams& p, int ctas, long long rows, cudaStream_t stream)
     config.stream = stream;
     config.attrs = attributes;
     config.numAttrs = 2;
-    (void)cudaLaunchKernelEx(&config, sample_kernel<T, HELD>, p);
+    (void)cudaLaunchKernelEx(&config, sample_kernel<T, HELD, kThreads>, p);
     QMOE_LAUNCH_CHECK("sample_kernel");
     return 0;
 }
@@ -564,13 +764,17 @@ extern "C" int qmoe_sample(const qmoe_sample_t* a, uint64_t stream_) {
     p.temperatures = (const float*)a->temperatures; p.top_ps = (const float*)a->top_ps; p.min_ps = (const float*)a->min_ps; p.top_ks = (const int*)a->top_ks;
     p.tokens = (long long*)a->tokens; p.log_probs = (float*)a->log_probs;
     p.vocab = (int)a->vocab; p.top_k = a->top_k; p.temperature = a->temperature; p.top_p = a->top_p; p.min_p = a->min_p;
-    // As many CTAs to a row as have 2048 tokens each, and for few rows up to eight, so that the slices' 32 KB leave room for two CTAs on an SM
+    // Few rows: as many CTAs to a row as have 2048 tokens each and find an SM of their own, up to eight, with 512 threads.  Many rows: as
+    // few as hold the row in slices of 40 KB, with 256 threads, because what a warp does beside its tokens is half of the work
     const int size = a->dtype == QMOE_BF16 ? 2 : 4;
     const long long padded = a->vocab + 15;          // a row may start anywhere in its first 16 bytes
     int ctas = 1;
-    while (ctas < kMaxCtas && padded > 2048ll * ctas && (a->rows * ctas < 2 * sm_count() || padded * size > 40 * 1024ll * ctas)) ctas *= 2;
+    while (ctas < kMaxCtas && padded > 2048ll * ctas && (a->rows * ctas <= sm_count() || padded * size > 40 * 1024ll * ctas)) ctas *= 2;
     p.slice = (int)((padded + 16 * ctas - 1) / (16 * ctas) * 16);
-    const bool held = (long long)p.slice * size <= kMaxSlice && p.slice <= kMaxHeld;
-    if (a->dtype == QMOE_BF16) return held ? launch<__nv_bfloat16, true>(p, ctas, a->rows, stream) : launch<__nv_bfloat16, false>(p, ctas, a->rows, stream);
-    return held ? launch<float, true>(p, ctas, a->rows, stream) : launch<float, false>(p, ctas, a->rows, stream);
+    const bool held = (long long)p.slice * size <= kMaxSlice && p.slice <= kMaxHeld, many = a->rows * ctas > 2 * sm_count();
+    if (a->dtype == QMOE_BF16)
+        return !held ? launch<__nv_bfloat16, false, 512>(p, ctas, a->rows, stream) : many ? launch<__nv_bfloat16, true, 256>(p, ctas, a->rows, stream)
+                                                                                          : launch<__nv_bfloat16, true, 512>(p, ctas, a->rows, stream);
+    return !held ? launch<float, false, 512>(p, ctas, a->rows, stream) : many ? launch<float, true, 256>(p, ctas, a->rows, stream)
+                                                                              : launch<float, true, 512>(p, ctas, a->rows, stream);
 }
