@@ -25,7 +25,7 @@
 // forward: 72, 37 and 32.
 // Every wait is bounded; on expiry the CTA records a code in the library's status word and leaves.
 #include "common.cuh"
-#include "tc_ptx.cuh"
+#include "attention_ptx.cuh"
 
 namespace qmoe {
 namespace {
@@ -36,8 +36,6 @@ constexpr int TILE_BYTES = BLOCK * D * 2;          // 16 KiB: 128 rows x 128 byt
 constexpr int THREADS = 192;              // forward, dq: TMA warp, MMA warp, four row warps
 // Row warps per 32 rows of the dk, dv kernel, which share the columns of a block between them
 constexpr int DKV_PARTS = 2, DKV_THREADS = 64 + 128 * DKV_PARTS;
-constexpr float LOG2E = 1.4426950408889634f;
-enum { STATUS_ATTENTION_WAIT = 301 };
 
 struct alignas(64) AttentionParams {
     CUtensorMap map_q, map_k, map_v, map_do;     // 3-D [batch][time][heads * 64] bf16, boxes of 64 x 128 x 1
@@ -53,25 +51,6 @@ struct alignas(64) AttentionParams {
     int split;                    // backward for dk, dv: CTAs per key block (cluster size)
 };
 
-__device__ __forceinline__ void tma_load_3d(const CUtensorMap* map, uint32_t dst, uint32_t bar, int c0, int c1, int c2) {
-    asm volatile(
-        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
-        ::"r"(dst), "l"(map), "r"(bar), "r"(c0), "r"(c1), "r"(c2) : "memory");
-}
-__device__ __forceinline__ uint32_t pack2(float a, float b) {
-    __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
-    return *reinterpret_cast<uint32_t*>(&h);
-}
-__device__ __forceinline__ float exp2_fast(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-__device__ __forceinline__ float max3(float a, float b, float c) {      // like fmaxf: a number rather than a NaN
-    float y;
-    asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
-    return y;
-}
 // 32 accumulator columns of one row, scaled, as 64 bytes of bf16
 __device__ __forceinline__ void store_row32(uint4* dst, const uint32_t* r, float scale) {
     auto two = [&](int c) { return pack2(__uint_as_float(r[c]) * scale, __uint_as_float(r[c + 1]) * scale); };
@@ -87,25 +66,6 @@ __device__ __forceinline__ void load_cluster4(uint32_t at, float* v) {
 // Where the 16 contraction elements [16 kk, 16 kk + 16) of a bf16 operand start that the rows wrote over the scores they had
 // read: a thread keeps to its own COLS columns, P (or the only operand) in their first half, dS in their second
 template <int COLS> __device__ __forceinline__ constexpr uint32_t p_column(int kk) { return (uint32_t)(kk * 16 / COLS * COLS + kk * 16 % COLS / 2); }
-
-struct Wait {   // bounded waits of one thread; the first that runs out marks the CTA
-    volatile int* abort_flag;
-    int* status;
-    __device__ __forceinline__ bool operator()(uint32_t bar, uint32_t parity) const {
-        if (mbar_wait(bar, parity, abort_flag)) return true;
-        if (!*abort_flag) { *abort_flag = 1; atomicExch(status, STATUS_ATTENTION_WAIT); }
-        return false;
-    }
-    // the same for a whole warp: all lanes go on, or none does
-    __device__ __forceinline__ bool all(uint32_t bar, uint32_t parity) const { return __all_sync(0xffffffffu, (*this)(bar, parity)); }
-};
-
-// a CTA that gave up leaves its copies and MMAs in flight a bounded time to land before its shared memory and TMEM go away
-__device__ __forceinline__ void linger_after_abort(const volatile int* abort_flag) {
-    if (!*abort_flag) return;
-    const unsigned long long start = global_ns();
-    while (global_ns() - start < 2000000ull) __nanosleep(1000);
-}
 
 // ------------------------------------------------------------------------------------------------
 // forward

@@ -1021,14 +1021,14 @@ int make_map_2d(CUtensorMap* out, uint64_t ptr, uint64_t inner, uint64_t outer, 
 // 3-D bf16 tensor [outer][mid][inner] (dense), box {64, box_mid, 1}, 128-byte swizzle: the attention kernels' view of
 // [batch][time][heads * 64], in which a box never crosses from one sequence into the next and positions past the end
 // of a sequence arrive as zeros.
-int make_map_3d(CUtensorMap* out, uint64_t ptr, uint64_t inner, uint64_t mid, uint64_t outer, uint32_t box_mid) {
+int make_map_3d(CUtensorMap* out, uint64_t ptr, uint64_t inner, uint64_t mid, uint64_t outer, uint32_t box_mid, uint32_t box_outer) {
     EncodeTiledFn fn = encode_fn();
     if (!fn) { set_error("cuTensorMapEncodeTiled is not available from the driver"); return QMOE_ERR_STATE; }
     if (ptr & 15u) return fail_arg("tensor-core operand address must be 16-byte aligned");
     if ((inner * 2) % 16) return fail_arg("tensor-core operand row pitch must be a multiple of 16 bytes");
     cuuint64_t dims[3] = {inner, mid, outer};
     cuuint64_t strides[2] = {inner * 2, inner * mid * 2};
-    cuuint32_t box[3] = {64, box_mid, 1};
+    cuuint32_t box[3] = {64, box_mid, box_outer};
     cuuint32_t estr[3] = {1, 1, 1};
     CUresult rc = fn(out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, (void*)ptr, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
                      CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);

@@ -7,7 +7,7 @@
 // key/value head, for a sequence's own cache its time * group.  An item is one key/value head, a tile of rows, and a chunk of the
 // keys; a chunk of several is joined with the others of its row by prefix_join_kernel.
 #include "common.cuh"
-#include "tc_ptx.cuh"
+#include "attention_ptx.cuh"
 
 namespace qmoe {
 
@@ -18,7 +18,6 @@ namespace {
 constexpr int kWarps = 4, kThreads = 32 * kWarps;
 constexpr int kKeys = 64;                // keys of a tile
 constexpr int kStages = 3;
-constexpr float kLog2e = 1.4426950408889634f;
 
 struct Keys {                            // the prefix, or the sequences' caches
     const uint8_t* k;
@@ -45,15 +44,6 @@ struct PrefixParams {
     float scale;                         // 1 / sqrt(dim)
 };
 
-__device__ __forceinline__ float exp2_fast(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-__device__ __forceinline__ uint32_t pack2(float a, float b) {
-    __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
-    return *reinterpret_cast<uint32_t*>(&h);
-}
 // two numbers as bf16, and what that leaves of them
 __device__ __forceinline__ void split2(float a, float b, uint32_t& high, uint32_t& rest) {
     high = pack2(a, b);
@@ -167,7 +157,7 @@ __device__ __forceinline__ void attend(const PrefixParams& p, const Keys& keys, 
 #pragma unroll
     for (int c = 0; c < COLS; ++c) o[c][0] = o[c][1] = o[c][2] = o[c][3] = 0.f;
     const int tiles = end > begin ? (end - begin + kKeys - 1) / kKeys : 0;
-    const float scale2 = p.scale * kLog2e;
+    const float scale2 = p.scale * LOG2E;
 #pragma unroll
     for (int s = 0; s < kStages - 1; ++s) {
         if (s < tiles) fetch(s);
@@ -369,6 +359,256 @@ prefix_attention_kernel(const __grid_constant__ PrefixParams p) {
     }
 }
 
+// ------------------------------------------------------------------------------------------------
+// The prefix on the tcgen05 tensor cores, for rows that fill their tiles: 128 rows (whole groups of heads of 128 / group sequences) against
+// blocks of 64 keys.  Warp 0 asks TMA for the tiles, warp 1 issues the MMAs, four row warps own a TMEM lane (a row) per thread:
+//     S = Q K^T -> rows: max, exp2, sum, P as two bf16 numbers, put back over the scores -> O += P V, twice, accumulated in tensor memory.
+// The scores of the next block go to the other of two buffers meanwhile.  What bounds it: the exponential unit, 512 cycles for a block and SM (the
+// products take 384, 256 of them the two of P V), which two CTAs to an SM share: one's exponentials run beside the other's waits.
+// ------------------------------------------------------------------------------------------------
+constexpr int kTcKeys = 64, kTcThreads = 192, kTcColumns = 256;
+
+template <int DIM> struct TcTile {
+    static constexpr int kHalves = DIM / 64;                       // a row of 64 elements is the 128 bytes of a swizzle
+    static constexpr int kQHalf = 128 * 128, kKeyHalf = kTcKeys * 128;
+    static constexpr int kQ = kHalves * kQHalf, kKey = kHalves * kKeyHalf;
+    static constexpr int kStages = DIM == 64 ? 3 : 2;
+    static constexpr int kTiles = kQ + 2 * kStages * kKey;
+    static constexpr int kShared = kTiles + 256;
+};
+
+struct alignas(64) PrefixTcParams {
+    CUtensorMap map_q, map_k, map_v;
+    PrefixParams p;
+    int* status;
+    int sequences;                       // of batch * time, in a tile
+};
+
+template <int DIM>
+__global__ void __launch_bounds__(kTcThreads, 2)
+prefix_tensor_kernel(const __grid_constant__ PrefixTcParams tc) {
+    using L = TcTile<DIM>;
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    const PrefixParams& p = tc.p;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int split = (int)blockIdx.x % p.prefix.splits, tile = (int)blockIdx.x / p.prefix.splits;
+    const int g = tile % p.kv_heads, first_sequence = tile / p.kv_heads * tc.sequences;
+    const uint32_t base = smem_u32(smem_raw), q_tile = base, k_tile = base + L::kQ, v_tile = k_tile + L::kStages * L::kKey, bars = base + L::kTiles;
+    enum { Q_FULL = 0, K_FULL = 1, K_EMPTY = K_FULL + L::kStages, V_FULL = K_EMPTY + L::kStages, V_EMPTY = V_FULL + L::kStages, S_FULL = V_EMPTY + L::kStages,
+           P_FULL = S_FULL + 2, BARS = P_FULL + 2 };
+    static_assert(8 * BARS + 8 <= L::kShared - L::kTiles, "the barriers fit");
+    auto bar = [&](int which) { return bars + 8u * which; };
+    uint32_t& s_tmem_base = *reinterpret_cast<uint32_t*>(smem_raw + L::kTiles + 8 * BARS);
+    volatile int& s_abort = *reinterpret_cast<volatile int*>(smem_raw + L::kTiles + 8 * BARS + 4);
+    if (base & 1023u) {                  // the operand tiles need the alignment the declaration asks for
+        chain_wait();
+        if (threadIdx.x == 0) atomicExch(tc.status, STATUS_ATTENTION_WAIT + 1);
+        return;
+    }
+    if (threadIdx.x == 0) {
+        s_abort = 0;
+        for (int w = 0; w < BARS; ++w) mbar_init(bar(w), w >= P_FULL ? 4 : 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        prefetch_map(&tc.map_q); prefetch_map(&tc.map_k); prefetch_map(&tc.map_v);
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s_tmem_base)), "r"(kTcColumns) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    chain_wait();
+    chain_next();                        // the tensor memory is this block's
+    const uint32_t tmem = s_tmem_base, tmem_o = tmem + 2 * kTcKeys;      // two buffers of scores, O behind them
+    const int length = min(max(p.prefix.lengths[0], 0), p.prefix.longest);
+    const int begin = split * p.prefix.chunk, end = min(length, begin + p.prefix.chunk);
+    const int n = end > begin ? (end - begin + kTcKeys - 1) / kTcKeys : 0;
+    const Wait wait{&s_abort, tc.status};
+
+    if (warp == 0) {
+        if (lane == 0 && n) {
+            mbar_expect_tx(bar(Q_FULL), p.group * tc.sequences * DIM * 2);
+            for (int half = 0; half < L::kHalves; ++half) tma_load_3d(&tc.map_q, q_tile + half * L::kQHalf, bar(Q_FULL), half * 64, g * p.group, first_sequence);
+            int st = 0;
+            uint32_t parity = 1;
+            for (int j = 0; j < n && !s_abort; ++j) {
+                if (!wait(bar(K_EMPTY + st), parity)) break;
+                mbar_expect_tx(bar(K_FULL + st), L::kKey);
+                for (int half = 0; half < L::kHalves; ++half)
+                    tma_load_3d(&tc.map_k, k_tile + st * L::kKey + half * L::kKeyHalf, bar(K_FULL + st), half * 64, begin + j * kTcKeys, g);
+                if (!wait(bar(V_EMPTY + st), parity)) break;
+                mbar_expect_tx(bar(V_FULL + st), L::kKey);
+                for (int half = 0; half < L::kHalves; ++half)
+                    tma_load_3d(&tc.map_v, v_tile + st * L::kKey + half * L::kKeyHalf, bar(V_FULL + st), half * 64, begin + j * kTcKeys, g);
+                if (++st == L::kStages) { st = 0; parity ^= 1u; }
+            }
+        }
+    } else if (warp == 1) {
+        constexpr uint32_t idesc_s = make_idesc<false, false, 128>(kTcKeys), idesc_o = make_idesc<false, true, 128>(64);
+        auto scores = [&](int j) {       // S = Q K^T of block j into its buffer
+            const int st = j % L::kStages;
+            if (!wait.all(bar(K_FULL + st), (uint32_t)(j / L::kStages) & 1u)) return false;
+            tc_fence_after();
+            if (elect_one()) {
+#pragma unroll
+                for (int kk = 0; kk < DIM / 16; ++kk)
+                    umma_bf16(tmem + (uint32_t)(j & 1) * kTcKeys, make_desc(q_tile + kk / 4 * L::kQHalf + kk % 4 * 32, 16, 1024),
+                              make_desc(k_tile + st * L::kKey + kk / 4 * L::kKeyHalf + kk % 4 * 32, 16, 1024), idesc_s, kk ? 1u : 0u);
+                umma_commit(bar(S_FULL + (j & 1)));
+                umma_commit(bar(K_EMPTY + st));
+            }
+            __syncwarp();
+            return true;
+        };
+        bool ok = n && wait.all(bar(Q_FULL), 0) && scores(0);
+        for (int j = 0; ok && j < n; ++j) {
+            const int st = j % L::kStages;
+            // the scores of the next block into the other buffer, once the product that reads the P of block j - 1 there is done
+            if (j > 0) ok = wait.all(bar(V_EMPTY + (j - 1) % L::kStages), (uint32_t)((j - 1) / L::kStages) & 1u);
+            if (ok && j + 1 < n) ok = scores(j + 1);
+            if (ok) ok = wait.all(bar(V_FULL + st), (uint32_t)(j / L::kStages) & 1u);
+            if (ok) ok = wait.all(bar(P_FULL + (j & 1)), (uint32_t)(j >> 1) & 1u);
+            if (!ok) break;
+            tc_fence_after();
+            // O += P V, the larger part of P and what it left: P from tensor memory, V as it lies in memory (rows = keys) is the
+            // MN-major operand
+            if (elect_one()) {
+#pragma unroll
+                for (int kk = 0; kk < kTcKeys / 16; ++kk)
+#pragma unroll
+                    for (int part = 0; part < 2; ++part)
+#pragma unroll
+                        for (int half = 0; half < L::kHalves; ++half)
+                            umma_bf16_ts(tmem_o + half * 64, tmem + (uint32_t)(j & 1) * kTcKeys + part * (kTcKeys / 2) + kk * 8,
+                                         make_desc(v_tile + st * L::kKey + half * L::kKeyHalf + kk * 2048, 8192, 1024), idesc_o, (j | kk | part) ? 1u : 0u);
+                umma_commit(bar(V_EMPTY + st));
+            }
+            __syncwarp();
+        }
+        // the last commit has arrived before this CTA's shared memory can go to another one
+        if (ok) wait.all(bar(V_EMPTY + (n - 1) % L::kStages), (uint32_t)((n - 1) / L::kStages) & 1u);
+    } else {
+        const int quad = warp & 3, row = quad * 32 + lane;
+        const int sequence = first_sequence + row / p.group;
+        const bool live = row < p.group * tc.sequences && sequence < p.batch * p.time;
+        const long long at = ((long long)sequence * p.kv_heads + g) * p.group + row % p.group;
+        const uint32_t lane_base = (uint32_t)(quad * 32) << 16;
+        const float scale2 = p.scale * LOG2E;
+        const uint64_t scale_pair = pair2(scale2, scale2);
+        float m = -INFINITY, l = 0.f;
+        bool ok = true;
+        for (int j = 0; ok && j < n; ++j) {
+            const uint32_t tmem_s = tmem + (uint32_t)(j & 1) * kTcKeys + lane_base;
+            const int there = end - begin - j * kTcKeys;            // keys of the block
+            ok = wait.all(bar(S_FULL + (j & 1)), (uint32_t)(j >> 1) & 1u);
+            if (!ok) break;
+            tc_fence_after();
+            uint32_t s[kTcKeys];
+            tmem_ld32(tmem_s, s);
+            tmem_ld32(tmem_s + 32, s + 32);
+            tmem_ld_wait();
+            if (there < kTcKeys) {
+#pragma unroll
+                for (int c = 0; c < kTcKeys; ++c)
+                    if (c >= there) s[c] = 0xff800000u;             // -inf
+                // Whatever lies behind the prefix must not meet a probability of zero as a NaN: its values become zeros.
+                const int st = j % L::kStages;
+                ok = wait.all(bar(V_FULL + st), (uint32_t)(j / L::kStages) & 1u);
+                if (!ok) break;
+                for (int i = threadIdx.x - 64; i < L::kHalves * kTcKeys * 8; i += 128)
+                    if (i / 8 % kTcKeys >= there)
+                        *reinterpret_cast<uint4*>(smem_raw + (v_tile - base) + st * L::kKey + i / 8 / kTcKeys * L::kKeyHalf + i / 8 % kTcKeys * 128 + i % 8 * 16) = make_uint4(0, 0, 0, 0);
+                fence_async_shared();
+            }
+            float peak4[4] = {__uint_as_float(s[0]), __uint_as_float(s[1]), __uint_as_float(s[2]), __uint_as_float(s[3])};
+#pragma unroll
+            for (int c = 4; c < kTcKeys; c += 2) peak4[(c >> 1) & 3] = max3(peak4[(c >> 1) & 3], __uint_as_float(s[c]), __uint_as_float(s[c + 1]));
+            const float next = fmaxf(m, fmaxf(max3(peak4[0], peak4[1], peak4[2]), peak4[3])), from = next == -INFINITY ? 0.f : next;
+            const float alpha = j ? exp2_fast((m - from) * scale2) : 1.f;
+            m = next;
+            l *= alpha;
+            const uint64_t minus_m = pair2(-from, -from);
+            uint64_t total2[2] = {0, 0};
+            uint32_t high[kTcKeys / 2], rest[kTcKeys / 2];
+#pragma unroll
+            for (int c = 0; c < kTcKeys; c += 2) {
+                float x0, x1;
+                unpair2(mul2(add2(pair2(__uint_as_float(s[c]), __uint_as_float(s[c + 1])), minus_m), scale_pair), x0, x1);
+                const float p0 = exp2_fast(x0), p1 = exp2_fast(x1);
+                total2[(c >> 1) & 1] = add2(total2[(c >> 1) & 1], pair2(p0, p1));
+                split2(p0, p1, high[c >> 1], rest[c >> 1]);
+            }
+            if (j > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
+                // O is whole once the product of the block before is done
+                ok = wait.all(bar(V_EMPTY + (j - 1) % L::kStages), (uint32_t)((j - 1) / L::kStages) & 1u);
+                if (!ok) break;
+                tc_fence_after();
+                const uint64_t alpha_pair = pair2(alpha, alpha);
+#pragma unroll
+                for (int e = 0; e < DIM; e += 32) {
+                    uint32_t o[32];
+                    tmem_ld32(tmem_o + lane_base + e, o);
+                    tmem_ld_wait();
+#pragma unroll
+                    for (int c = 0; c < 32; c += 2) {
+                        float o0, o1;
+                        unpair2(mul2(pair2(__uint_as_float(o[c]), __uint_as_float(o[c + 1])), alpha_pair), o0, o1);
+                        o[c] = __float_as_uint(o0);
+                        o[c + 1] = __float_as_uint(o1);
+                    }
+                    tmem_st32(tmem_o + lane_base + e, o);
+                }
+            }
+            tmem_st32(tmem_s, high);
+            tmem_st32(tmem_s + 32, rest);
+            tmem_st_wait();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar(P_FULL + (j & 1)));
+            float t0, t1;
+            unpair2(add2(total2[0], total2[1]), t0, t1);
+            l += t0 + t1;
+        }
+        if (ok && n) ok = wait.all(bar(V_EMPTY + (n - 1) % L::kStages), (uint32_t)((n - 1) / L::kStages) & 1u);
+        if (ok) {
+            const bool whole = p.slots == 1;
+            const long long slot = (long long)(p.prefix.first_slot + split) * p.rows + at;
+            const float inverse = l > 0.f ? 1.f / l : 0.f;
+            if (live) {
+                if (whole) p.lse[at] = l > 0.f ? m * p.scale + logf(l) : -INFINITY;
+                else p.part_ml[slot] = make_float2(m, l);
+            }
+            if (n || whole) {
+                tc_fence_after();
+#pragma unroll 1
+                for (int e = 0; e < DIM; e += 32) {
+                    uint32_t o[32];
+                    tmem_ld32(tmem_o + lane_base + e, o);
+                    tmem_ld_wait();
+                    if (!live) continue;
+                    auto value = [&](int c) { return n ? __uint_as_float(o[c]) : 0.f; };
+                    if (whole) {
+                        auto two = [&](int c) { return pack2(value(c) * inverse, value(c + 1) * inverse); };
+#pragma unroll
+                        for (int c = 0; c < 32; c += 8) *reinterpret_cast<uint4*>(p.out + at * DIM + e + c) = make_uint4(two(c), two(c + 2), two(c + 4), two(c + 6));
+                    } else {
+#pragma unroll
+                        for (int c = 0; c < 32; c += 4) *reinterpret_cast<float4*>(p.part_o + slot * DIM + e + c) = make_float4(value(c), value(c + 1), value(c + 2), value(c + 3));
+                    }
+                }
+            }
+        }
+    }
+    linger_after_abort(&s_abort);
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTcColumns) : "memory");
+    }
+}
+
 // A warp per row: the parts' weights, then their weighted sum
 template <int DIM>
 __global__ void __launch_bounds__(kThreads)
@@ -377,7 +617,7 @@ prefix_join_kernel(const __grid_constant__ PrefixParams p) {
     const long long row = (long long)blockIdx.x * kWarps + (threadIdx.x >> 5);
     const int lane = threadIdx.x & 31;
     if (row >= p.rows) return;
-    const float scale2 = p.scale * kLog2e;
+    const float scale2 = p.scale * LOG2E;
     float top = -INFINITY, total = 0.f;
     for (int s = lane; s < p.slots; s += 32) top = fmaxf(top, p.part_ml[s * p.rows + row].x);
     top = warp_max(top);
@@ -406,24 +646,31 @@ prefix_join_kernel(const __grid_constant__ PrefixParams p) {
     if (lane == 0) p.lse[row] = total > 0.f ? top * p.scale + logf(total) : -INFINITY;
 }
 
-struct Plan { Keys prefix, own; int slots; long long prefix_items, own_items; bool prefix_by_keys, own_by_keys; };
+struct Plan { Keys prefix, own; int slots; long long prefix_items, own_items; bool tensor, prefix_by_keys, own_by_keys; };
 
 // Chunks of keys: as long as they leave four items to an SM, but not below two tiles.
 Plan plan_of(const qmoe_prefix_attention_t* a, const qmoe_cache_t* c) {
     Plan plan = {};
     const long long group = a->heads / c->kv_heads, own_rows = a->time * group, all_rows = c->batch * own_rows;
+    plan.tensor = c->dtype == QMOE_BF16 && group <= 128 && all_rows > 64 && a->prefix_longest >= 2 * kTcKeys;
     plan.prefix_by_keys = all_rows <= 16;
     plan.own_by_keys = own_rows <= 16;
-    plan.prefix.row_tiles = ceil_div(all_rows, plan.prefix_by_keys ? 16 : 64);
+    plan.prefix.row_tiles = plan.tensor ? ceil_div(c->batch * a->time, 128 / group) : ceil_div(all_rows, plan.prefix_by_keys ? 16 : 64);
     plan.own.row_tiles = ceil_div(own_rows, plan.own_by_keys ? 16 : 64);
     const long long prefix_tiles = ceil_div(a->prefix_longest, kKeys), own_tiles = ceil_div(a->longest, kKeys), wanted = (long long)sm_count() * 4;
     const long long prefix_heads = (long long)plan.prefix.row_tiles * c->kv_heads, own_heads = (long long)plan.own.row_tiles * c->kv_heads * c->batch;
-    long long chunk = prefix_tiles > own_tiles ? prefix_tiles : own_tiles;
-    auto items = [&](long long tiles) { return prefix_heads * ceil_div(prefix_tiles, tiles) + own_heads * ceil_div(own_tiles, tiles); };
+    const long long prefix_mma = plan.tensor ? 0 : prefix_tiles;
+    long long chunk = prefix_mma > own_tiles ? prefix_mma : own_tiles;
+    auto items = [&](long long tiles) { return prefix_heads * ceil_div(prefix_mma, tiles) + own_heads * ceil_div(own_tiles, tiles); };
     while (chunk > 2 && items(chunk) < wanted) chunk = (chunk + 1) / 2;
     if (chunk < 1) chunk = 1;
     plan.prefix.chunk = plan.own.chunk = (int)chunk * kKeys;
-    plan.prefix.splits = ceil_div(prefix_tiles, chunk);
+    if (plan.tensor) {                   // one round of the two CTAs that an SM holds, but no chunk below four blocks
+        long long splits = 2ll * sm_count() / prefix_heads;
+        if (splits > prefix_tiles / 4) splits = prefix_tiles / 4;
+        plan.prefix.chunk = ceil_div(prefix_tiles, splits > 1 ? splits : 1) * kKeys;
+    }
+    plan.prefix.splits = ceil_div(a->prefix_longest, plan.prefix.chunk);
     plan.own.splits = ceil_div(own_tiles, chunk);
     if (!plan.prefix.splits && !plan.own.splits) plan.own.splits = 1;        // nothing to see: zeros are written all the same
     plan.own.first_slot = plan.prefix.splits;
@@ -455,17 +702,42 @@ int prefix_attention_check(const qmoe_prefix_attention_t* a, const qmoe_cache_t*
     return 0;
 }
 
+template <int DIM>
+int launch_tensor(const PrefixParams& p, const Plan& plan, const qmoe_cache_t* prefix, cudaStream_t stream) {
+    PrefixTcParams tc = {};
+    const uint32_t group = (uint32_t)p.group, sequences = 128 / group;
+    if (int rc = make_map_3d(&tc.map_q, (uint64_t)p.q, DIM, (uint64_t)group * p.kv_heads, (uint64_t)p.batch * p.time, group, sequences)) return rc;
+    if (int rc = make_map_3d(&tc.map_k, prefix->k, DIM, (uint64_t)prefix->capacity, (uint64_t)p.kv_heads, kTcKeys)) return rc;
+    if (int rc = make_map_3d(&tc.map_v, prefix->v, DIM, (uint64_t)prefix->capacity, (uint64_t)p.kv_heads, kTcKeys)) return rc;
+    tc.p = p;
+    tc.status = device_status_address();
+    tc.sequences = (int)sequences;
+    QMOE_CUDA(cudaFuncSetAttribute(prefix_tensor_kernel<DIM>, cudaFuncAttributeMaxDynamicSharedMemorySize, TcTile<DIM>::kShared));
+    chained(prefix_tensor_kernel<DIM>, (unsigned)plan.prefix_items, kTcThreads, TcTile<DIM>::kShared, stream, tc);
+    count_tensor_core_launch();
+    QMOE_LAUNCH_CHECK("prefix_tensor_kernel");
+    return 0;
+}
+
 template <int DIM, bool INT8>
-int launch(const PrefixParams& p, const Plan& plan, cudaStream_t stream) {
+int launch(PrefixParams& p, const Plan& plan, const qmoe_cache_t* prefix, cudaStream_t stream) {
     constexpr int SHARED = Tile<DIM, INT8>::kShared;
+    long long items = plan.prefix_items + plan.own_items;
+    if (plan.tensor) {
+        if constexpr (!INT8)
+            if (int rc = launch_tensor<DIM>(p, plan, prefix, stream)) return rc;
+        p.prefix_items = 0;
+        items = plan.own_items;
+    }
     auto go = [&](auto kernel) -> int {
         QMOE_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SHARED));
-        chained(kernel, (unsigned)(plan.prefix_items + plan.own_items), kThreads, SHARED, stream, p);
+        chained(kernel, (unsigned)items, kThreads, SHARED, stream, p);
         QMOE_LAUNCH_CHECK("prefix_attention_kernel");
         return 0;
     };
-    int rc;
-    if (plan.prefix_by_keys) rc = go(prefix_attention_kernel<DIM, INT8, true, true>);        // few rows in all: few in a sequence
+    int rc = 0;
+    if (!items) {}
+    else if (plan.prefix_by_keys) rc = go(prefix_attention_kernel<DIM, INT8, true, true>);        // few rows in all: few in a sequence
     else if (plan.own_by_keys) rc = go(prefix_attention_kernel<DIM, INT8, false, true>);
     else rc = go(prefix_attention_kernel<DIM, INT8, false, false>);
     if (rc || plan.slots == 1) return rc;
@@ -505,6 +777,6 @@ extern "C" int qmoe_prefix_attention(const qmoe_prefix_attention_t* a, const qmo
     p.batch = (int)c->batch; p.time = (int)a->time; p.kv_heads = c->kv_heads; p.group = a->heads / c->kv_heads; p.slots = plan.slots;
     p.prefix_items = (int)plan.prefix_items;
     p.scale = 1.f / sqrtf((float)c->dim);
-    if (c->dim == 64) return c->dtype == QMOE_INT8 ? launch<64, true>(p, plan, stream) : launch<64, false>(p, plan, stream);
-    return c->dtype == QMOE_INT8 ? launch<128, true>(p, plan, stream) : launch<128, false>(p, plan, stream);
+    if (c->dim == 64) return c->dtype == QMOE_INT8 ? launch<64, true>(p, plan, prefix, stream) : launch<64, false>(p, plan, prefix, stream);
+    return c->dtype == QMOE_INT8 ? launch<128, true>(p, plan, prefix, stream) : launch<128, false>(p, plan, prefix, stream);
 }
