@@ -18,6 +18,7 @@ namespace {
 constexpr int kWarps = 4, kThreads = 32 * kWarps;
 constexpr int kKeys = 64;                // keys of a tile
 constexpr int kStages = 3;
+constexpr float LN2 = 0.6931471805599453f;
 
 struct Keys {                            // the prefix, or the sequences' caches
     const uint8_t* k;
@@ -36,7 +37,7 @@ struct PrefixParams {
     const __nv_bfloat16* q;
     __nv_bfloat16* out;
     float* lse;
-    float2* part_ml;                     // [slots][rows]: m in raw scores, l
+    float2* part_ml;                     // [slots][rows]: m as an exponent of 2, l
     float* part_o;                       // [slots][rows][dim]
     long long rows;                      // batch * time * heads
     int batch, time, kv_heads, group, slots;
@@ -44,10 +45,14 @@ struct PrefixParams {
     float scale;                         // 1 / sqrt(dim)
 };
 
-// two numbers as bf16, and what that leaves of them
+// Two numbers that are not negative as bf16, cut off and not rounded (the upper halves as they are), and what that leaves of them, rounded: 2^-16
+// of a number is lost at most.
 __device__ __forceinline__ void split2(float a, float b, uint32_t& high, uint32_t& rest) {
-    high = pack2(a, b);
-    rest = pack2(a - __uint_as_float(high << 16), b - __uint_as_float(high & 0xffff0000u));
+    high = __byte_perm(__float_as_uint(a), __float_as_uint(b), 0x7632);
+    float a_rest, b_rest;
+    unpair2(add2(pair2(a, b), pair2(__uint_as_float((__float_as_uint(a) & 0xffff0000u) | 0x80000000u),
+                                    __uint_as_float((__float_as_uint(b) & 0xffff0000u) | 0x80000000u))), a_rest, b_rest);
+    rest = pack2(a_rest, b_rest);
 }
 // 16 bytes into shared memory, zeros where there is nothing to read
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool there) {
@@ -310,7 +315,7 @@ __device__ __forceinline__ void attend(const PrefixParams& p, const Keys& keys, 
         const float inverse = total > 0.f ? 1.f / total : 0.f;
         if (piece == 0) {
             if (whole) p.lse[to] = total > 0.f ? top * p.scale + logf(total) : -INFINITY;
-            else p.part_ml[slot] = make_float2(top, total);
+            else p.part_ml[slot] = make_float2(top * scale2, total);
         }
         for (int d = piece * 4; d < DIM; d += 32) {
             float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -330,7 +335,7 @@ __device__ __forceinline__ void attend(const PrefixParams& p, const Keys& keys, 
             const float inverse = l[i] > 0.f ? 1.f / l[i] : 0.f;
             if (t4 == 0) {
                 if (p.slots == 1) p.lse[at[i]] = l[i] > 0.f ? m[i] * p.scale + logf(l[i]) : -INFINITY;
-                else p.part_ml[slot] = make_float2(m[i], l[i]);
+                else p.part_ml[slot] = make_float2(m[i] * scale2, l[i]);
             }
 #pragma unroll
             for (int c = 0; c < COLS; ++c)
@@ -363,40 +368,58 @@ prefix_attention_kernel(const __grid_constant__ PrefixParams p) {
 // The prefix on the tcgen05 tensor cores, for rows that fill their tiles: 128 rows (whole groups of heads of 128 / group sequences) against
 // blocks of 64 keys.  Warp 0 asks TMA for the tiles, warp 1 issues the MMAs, four row warps own a TMEM lane (a row) per thread:
 //     S = Q K^T -> rows: max, exp2, sum, P as two bf16 numbers, put back over the scores -> O += P V, twice, accumulated in tensor memory.
-// The scores of the next block go to the other of two buffers meanwhile.  What bounds it: the exponential unit, 512 cycles for a block and SM (the
-// products take 384, 256 of them the two of P V), which two CTAs to an SM share: one's exponentials run beside the other's waits.
+// The scores of the next blocks go to other buffers meanwhile.  Keys and values of 8 bits come through two more warps, which load them
+// and put them into shared memory as bf16, exactly, in the order in which TMA would have; their scales go to the rows, the key's into
+// the score, the value's into the probability.
+// What bounds it: the exponential unit, 512 cycles for a block and SM (the products take 384, 256 of them the two of P V), which two CTAs to
+// an SM share: one's exponentials run beside the other's waits.
 // ------------------------------------------------------------------------------------------------
-constexpr int kTcKeys = 64, kTcThreads = 192, kTcColumns = 256;
+constexpr int kTcKeys = 64, kTcColumns = 256, kTcConverters = 2;
 
-template <int DIM> struct TcTile {
+template <int DIM, bool INT8> struct TcTile {
+    static constexpr int kThreads = 192 + (INT8 ? 32 * kTcConverters : 0);
     static constexpr int kHalves = DIM / 64;                       // a row of 64 elements is the 128 bytes of a swizzle
     static constexpr int kQHalf = 128 * 128, kKeyHalf = kTcKeys * 128;
     static constexpr int kQ = kHalves * kQHalf, kKey = kHalves * kKeyHalf;
     static constexpr int kStages = DIM == 64 ? 3 : 2;
+    static constexpr int kBuffers = DIM == 64 ? 3 : 2;             // of scores: with O all of a CTA's 256 columns
     static constexpr int kTiles = kQ + 2 * kStages * kKey;
-    static constexpr int kShared = kTiles + 256;
+    static constexpr int kScales = INT8 ? kStages * 2 * kTcKeys * 4 : 0;
+    static constexpr int kShared = kTiles + 256 + kScales;
 };
 
 struct alignas(64) PrefixTcParams {
-    CUtensorMap map_q, map_k, map_v;
+    CUtensorMap map_q, map_k, map_v;     // k, v: of a bf16 prefix
     PrefixParams p;
     int* status;
     int sequences;                       // of batch * time, in a tile
 };
 
-template <int DIM>
-__global__ void __launch_bounds__(kTcThreads, 2)
+// 16 signed bytes as 16 bf16 numbers, to two neighbouring pieces of a swizzled row
+__device__ __forceinline__ void store_bytes(uint32_t row, int piece, int key, const uint4& v) {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const uint32_t a = bytes_to_bf16(__byte_perm(w[2 * i], 0, 0x4140)), b = bytes_to_bf16(__byte_perm(w[2 * i], 0, 0x4342));
+        const uint32_t c = bytes_to_bf16(__byte_perm(w[2 * i + 1], 0, 0x4140)), d = bytes_to_bf16(__byte_perm(w[2 * i + 1], 0, 0x4342));
+        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(row + (((2 * piece + i) ^ (key & 7)) << 4)), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+    }
+}
+
+template <int DIM, bool INT8>
+__global__ void __launch_bounds__(TcTile<DIM, INT8>::kThreads, 2)
 prefix_tensor_kernel(const __grid_constant__ PrefixTcParams tc) {
-    using L = TcTile<DIM>;
+    using L = TcTile<DIM, INT8>;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     const PrefixParams& p = tc.p;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int split = (int)blockIdx.x % p.prefix.splits, tile = (int)blockIdx.x / p.prefix.splits;
     const int g = tile % p.kv_heads, first_sequence = tile / p.kv_heads * tc.sequences;
     const uint32_t base = smem_u32(smem_raw), q_tile = base, k_tile = base + L::kQ, v_tile = k_tile + L::kStages * L::kKey, bars = base + L::kTiles;
-    enum { Q_FULL = 0, K_FULL = 1, K_EMPTY = K_FULL + L::kStages, V_FULL = K_EMPTY + L::kStages, V_EMPTY = V_FULL + L::kStages, S_FULL = V_EMPTY + L::kStages,
-           P_FULL = S_FULL + 2, BARS = P_FULL + 2 };
-    static_assert(8 * BARS + 8 <= L::kShared - L::kTiles, "the barriers fit");
+    enum { Q_FULL = 0, K_FULL = 1, V_FULL = K_FULL + L::kStages, K_EMPTY = V_FULL + L::kStages, V_EMPTY = K_EMPTY + L::kStages, S_FULL = V_EMPTY + L::kStages,
+           P_FULL = S_FULL + L::kBuffers, BARS = P_FULL + L::kBuffers };
+    static_assert(8 * BARS + 8 <= 256, "the barriers fit");
+    float* const scales = reinterpret_cast<float*>(smem_raw + L::kTiles + 256);      // INT8: [stage][key, value][64]
     auto bar = [&](int which) { return bars + 8u * which; };
     uint32_t& s_tmem_base = *reinterpret_cast<uint32_t*>(smem_raw + L::kTiles + 8 * BARS);
     volatile int& s_abort = *reinterpret_cast<volatile int*>(smem_raw + L::kTiles + 8 * BARS + 4);
@@ -407,9 +430,10 @@ prefix_tensor_kernel(const __grid_constant__ PrefixTcParams tc) {
     }
     if (threadIdx.x == 0) {
         s_abort = 0;
-        for (int w = 0; w < BARS; ++w) mbar_init(bar(w), w >= P_FULL ? 4 : 1);
+        for (int w = 0; w < BARS; ++w) mbar_init(bar(w), w >= P_FULL ? 4 : INT8 && w >= K_FULL && w < K_EMPTY ? kTcConverters : 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-        prefetch_map(&tc.map_q); prefetch_map(&tc.map_k); prefetch_map(&tc.map_v);
+        prefetch_map(&tc.map_q);
+        if (!INT8) { prefetch_map(&tc.map_k); prefetch_map(&tc.map_v); }
     }
     if (warp == 1) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s_tmem_base)), "r"(kTcColumns) : "memory");
@@ -420,7 +444,7 @@ prefix_tensor_kernel(const __grid_constant__ PrefixTcParams tc) {
     tc_fence_after();
     chain_wait();
     chain_next();                        // the tensor memory is this block's
-    const uint32_t tmem = s_tmem_base, tmem_o = tmem + 2 * kTcKeys;      // two buffers of scores, O behind them
+    const uint32_t tmem = s_tmem_base, tmem_o = tmem + L::kBuffers * kTcKeys;      // the buffers of scores, O behind them
     const int length = min(max(p.prefix.lengths[0], 0), p.prefix.longest);
     const int begin = split * p.prefix.chunk, end = min(length, begin + p.prefix.chunk);
     const int n = end > begin ? (end - begin + kTcKeys - 1) / kTcKeys : 0;
@@ -432,7 +456,7 @@ prefix_tensor_kernel(const __grid_constant__ PrefixTcParams tc) {
             for (int half = 0; half < L::kHalves; ++half) tma_load_3d(&tc.map_q, q_tile + half * L::kQHalf, bar(Q_FULL), half * 64, g * p.group, first_sequence);
             int st = 0;
             uint32_t parity = 1;
-            for (int j = 0; j < n && !s_abort; ++j) {
+            for (int j = 0; !INT8 && j < n && !s_abort; ++j) {
                 if (!wait(bar(K_EMPTY + st), parity)) break;
                 mbar_expect_tx(bar(K_FULL + st), L::kKey);
                 for (int half = 0; half < L::kHalves; ++half)
@@ -446,126 +470,205 @@ prefix_tensor_kernel(const __grid_constant__ PrefixTcParams tc) {
         }
     } else if (warp == 1) {
         constexpr uint32_t idesc_s = make_idesc<false, false, 128>(kTcKeys), idesc_o = make_idesc<false, true, 128>(64);
+        // descriptors of the first tiles; an offset in bytes goes into their address field in units of 16
+        const uint64_t q_desc = make_desc(q_tile, 16, 1024), k_desc = make_desc(k_tile, 16, 1024), v_desc = make_desc(v_tile, 8192, 1024);
         auto scores = [&](int j) {       // S = Q K^T of block j into its buffer
             const int st = j % L::kStages;
             if (!wait.all(bar(K_FULL + st), (uint32_t)(j / L::kStages) & 1u)) return false;
             tc_fence_after();
             if (elect_one()) {
+                const uint64_t k_at = k_desc + (uint32_t)(st * (L::kKey >> 4));
+                const uint32_t to = tmem + (uint32_t)(j % L::kBuffers) * kTcKeys;
 #pragma unroll
                 for (int kk = 0; kk < DIM / 16; ++kk)
-                    umma_bf16(tmem + (uint32_t)(j & 1) * kTcKeys, make_desc(q_tile + kk / 4 * L::kQHalf + kk % 4 * 32, 16, 1024),
-                              make_desc(k_tile + st * L::kKey + kk / 4 * L::kKeyHalf + kk % 4 * 32, 16, 1024), idesc_s, kk ? 1u : 0u);
-                umma_commit(bar(S_FULL + (j & 1)));
+                    umma_bf16(to, q_desc + ((kk / 4 * L::kQHalf + kk % 4 * 32) >> 4), k_at + ((kk / 4 * L::kKeyHalf + kk % 4 * 32) >> 4), idesc_s, kk ? 1u : 0u);
+                umma_commit(bar(S_FULL + j % L::kBuffers));
                 umma_commit(bar(K_EMPTY + st));
             }
             __syncwarp();
             return true;
         };
-        bool ok = n && wait.all(bar(Q_FULL), 0) && scores(0);
+        // the scores are formed as many blocks ahead as there are buffers but one
+        bool ok = n && wait.all(bar(Q_FULL), 0);
+        for (int j = 0; ok && j < L::kBuffers - 1 && j < n; ++j) ok = scores(j);
         for (int j = 0; ok && j < n; ++j) {
-            const int st = j % L::kStages;
-            // the scores of the next block into the other buffer, once the product that reads the P of block j - 1 there is done
+            const int st = j % L::kStages, next = j + L::kBuffers - 1;
+            // into the buffer of the block before, once the product that reads its P there is done
             if (j > 0) ok = wait.all(bar(V_EMPTY + (j - 1) % L::kStages), (uint32_t)((j - 1) / L::kStages) & 1u);
-            if (ok && j + 1 < n) ok = scores(j + 1);
+            if (ok && next < n) ok = scores(next);
             if (ok) ok = wait.all(bar(V_FULL + st), (uint32_t)(j / L::kStages) & 1u);
-            if (ok) ok = wait.all(bar(P_FULL + (j & 1)), (uint32_t)(j >> 1) & 1u);
+            if (ok) ok = wait.all(bar(P_FULL + j % L::kBuffers), (uint32_t)(j / L::kBuffers) & 1u);
             if (!ok) break;
             tc_fence_after();
             // O += P V, the larger part of P and what it left: P from tensor memory, V as it lies in memory (rows = keys) is the
             // MN-major operand
             if (elect_one()) {
+                const uint64_t v_at = v_desc + (uint32_t)(st * (L::kKey >> 4));
+                const uint32_t from = tmem + (uint32_t)(j % L::kBuffers) * kTcKeys;
 #pragma unroll
                 for (int kk = 0; kk < kTcKeys / 16; ++kk)
 #pragma unroll
                     for (int part = 0; part < 2; ++part)
 #pragma unroll
                         for (int half = 0; half < L::kHalves; ++half)
-                            umma_bf16_ts(tmem_o + half * 64, tmem + (uint32_t)(j & 1) * kTcKeys + part * (kTcKeys / 2) + kk * 8,
-                                         make_desc(v_tile + st * L::kKey + half * L::kKeyHalf + kk * 2048, 8192, 1024), idesc_o, (j | kk | part) ? 1u : 0u);
+                            umma_bf16_ts(tmem_o + half * 64, from + kk / 2 * 32 + part * 16 + kk % 2 * 8, v_at + ((half * L::kKeyHalf + kk * 2048) >> 4), idesc_o, (j | kk | part) ? 1u : 0u);
                 umma_commit(bar(V_EMPTY + st));
             }
             __syncwarp();
         }
         // the last commit has arrived before this CTA's shared memory can go to another one
         if (ok) wait.all(bar(V_EMPTY + (n - 1) % L::kStages), (uint32_t)((n - 1) / L::kStages) & 1u);
+    } else if (INT8 && warp >= 6) {
+        // pieces of 16 values, a thread's EACH of a tile: piece i of the tile is piece i % PIECES of key i / PIECES
+        constexpr int PIECES = DIM / 16, EACH = kTcKeys * PIECES / (32 * kTcConverters);
+        const int mine = threadIdx.x - 192;
+        const long long head = (long long)g * p.prefix.capacity + begin;
+        uint4 k[EACH], v[EACH];
+        float k_scale = 0.f, v_scale = 0.f;
+        auto fetch = [&](int j) {        // behind `end` zeros, whatever lies there
+#pragma unroll
+            for (int i = 0; i < EACH; ++i) {
+                const int at = i * 32 * kTcConverters + mine, key = j * kTcKeys + at / PIECES;
+                const bool there = begin + key < end;
+                const long long from = (head + key) * DIM + at % PIECES * 16;
+                k[i] = there ? *reinterpret_cast<const uint4*>(p.prefix.k + from) : make_uint4(0, 0, 0, 0);
+                v[i] = there ? *reinterpret_cast<const uint4*>(p.prefix.v + from) : make_uint4(0, 0, 0, 0);
+            }
+            const bool there = begin + j * kTcKeys + mine < end;
+            k_scale = there ? p.prefix.k_scale[head + j * kTcKeys + mine] : 0.f;
+            v_scale = there ? p.prefix.v_scale[head + j * kTcKeys + mine] : 0.f;
+        };
+        if (n) fetch(0);
+        bool ok = true;
+        for (int j = 0; ok && j < n; ++j) {
+            const int st = j % L::kStages;
+            const uint32_t parity = (uint32_t)(j / L::kStages) & 1u ^ 1u;
+            auto put = [&](uint32_t to, const uint4* values) {
+#pragma unroll
+                for (int i = 0; i < EACH; ++i) {
+                    const int at = i * 32 * kTcConverters + mine, key = at / PIECES, piece = at % PIECES;
+                    store_bytes(to + piece / 4 * L::kKeyHalf + key * 128, piece % 4, key, values[i]);
+                }
+            };
+            ok = wait.all(bar(K_EMPTY + st), parity);
+            if (!ok) break;
+            put(k_tile + st * L::kKey, k);
+            fence_async_shared();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar(K_FULL + st));
+            ok = wait.all(bar(V_EMPTY + st), parity);
+            if (!ok) break;
+            put(v_tile + st * L::kKey, v);
+            scales[st * 2 * kTcKeys + mine] = k_scale;
+            scales[st * 2 * kTcKeys + kTcKeys + mine] = v_scale;
+            if (j + 1 < n) fetch(j + 1);
+            fence_async_shared();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar(V_FULL + st));
+        }
     } else {
         const int quad = warp & 3, row = quad * 32 + lane;
         const int sequence = first_sequence + row / p.group;
         const bool live = row < p.group * tc.sequences && sequence < p.batch * p.time;
         const long long at = ((long long)sequence * p.kv_heads + g) * p.group + row % p.group;
         const uint32_t lane_base = (uint32_t)(quad * 32) << 16;
+        // Scores in the exponent of 2.  x = s * scale2 - m with m, a maximum, rounded there: what that is off by is in numerator and sum alike.
         const float scale2 = p.scale * LOG2E;
         const uint64_t scale_pair = pair2(scale2, scale2);
         float m = -INFINITY, l = 0.f;
         bool ok = true;
         for (int j = 0; ok && j < n; ++j) {
-            const uint32_t tmem_s = tmem + (uint32_t)(j & 1) * kTcKeys + lane_base;
-            const int there = end - begin - j * kTcKeys;            // keys of the block
-            ok = wait.all(bar(S_FULL + (j & 1)), (uint32_t)(j >> 1) & 1u);
+            const int st = j % L::kStages, there = end - begin - j * kTcKeys;            // keys of the block
+            const uint32_t tmem_s = tmem + (uint32_t)(j % L::kBuffers) * kTcKeys + lane_base;
+            ok = wait.all(bar(S_FULL + j % L::kBuffers), (uint32_t)(j / L::kBuffers) & 1u);
+            if (ok && (INT8 || there < kTcKeys)) ok = wait.all(bar(V_FULL + st), (uint32_t)(j / L::kStages) & 1u);
             if (!ok) break;
             tc_fence_after();
             uint32_t s[kTcKeys];
             tmem_ld32(tmem_s, s);
             tmem_ld32(tmem_s + 32, s + 32);
             tmem_ld_wait();
+            if constexpr (INT8) {
+                const float4* by = reinterpret_cast<const float4*>(scales + st * 2 * kTcKeys);
+#pragma unroll
+                for (int c = 0; c < kTcKeys; c += 4) {
+                    const float4 f = by[c / 4];
+                    float x[4];
+                    unpair2(mul2(pair2(__uint_as_float(s[c]), __uint_as_float(s[c + 1])), pair2(f.x, f.y)), x[0], x[1]);
+                    unpair2(mul2(pair2(__uint_as_float(s[c + 2]), __uint_as_float(s[c + 3])), pair2(f.z, f.w)), x[2], x[3]);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) s[c + i] = __float_as_uint(x[i]);
+                }
+            }
             if (there < kTcKeys) {
 #pragma unroll
                 for (int c = 0; c < kTcKeys; ++c)
                     if (c >= there) s[c] = 0xff800000u;             // -inf
-                // Whatever lies behind the prefix must not meet a probability of zero as a NaN: its values become zeros.
-                const int st = j % L::kStages;
-                ok = wait.all(bar(V_FULL + st), (uint32_t)(j / L::kStages) & 1u);
-                if (!ok) break;
-                for (int i = threadIdx.x - 64; i < L::kHalves * kTcKeys * 8; i += 128)
-                    if (i / 8 % kTcKeys >= there)
-                        *reinterpret_cast<uint4*>(smem_raw + (v_tile - base) + st * L::kKey + i / 8 / kTcKeys * L::kKeyHalf + i / 8 % kTcKeys * 128 + i % 8 * 16) = make_uint4(0, 0, 0, 0);
-                fence_async_shared();
+                if constexpr (!INT8) {
+                    // Whatever lies behind the prefix must not meet a probability of zero as a NaN: its values become zeros.
+                    for (int i = threadIdx.x - 64; i < L::kHalves * kTcKeys * 8; i += 128)
+                        if (i / 8 % kTcKeys >= there)
+                            *reinterpret_cast<uint4*>(smem_raw + (v_tile - base) + st * L::kKey + i / 8 / kTcKeys * L::kKeyHalf + i / 8 % kTcKeys * 128 + i % 8 * 16) = make_uint4(0, 0, 0, 0);
+                    fence_async_shared();
+                }
             }
             float peak4[4] = {__uint_as_float(s[0]), __uint_as_float(s[1]), __uint_as_float(s[2]), __uint_as_float(s[3])};
 #pragma unroll
             for (int c = 4; c < kTcKeys; c += 2) peak4[(c >> 1) & 3] = max3(peak4[(c >> 1) & 3], __uint_as_float(s[c]), __uint_as_float(s[c + 1]));
-            const float next = fmaxf(m, fmaxf(max3(peak4[0], peak4[1], peak4[2]), peak4[3])), from = next == -INFINITY ? 0.f : next;
-            const float alpha = j ? exp2_fast((m - from) * scale2) : 1.f;
-            m = next;
+            const float next = fmaxf(max3(peak4[0], peak4[1], peak4[2]), peak4[3]) * scale2;
+            // The base of the exponentials follows the maximum only when it is 2^8 behind: a new maximum somewhere in 32 rows comes with every other block,
+            // and rescaling O for it took a fifth of the rows' time.  Probabilities up to 2^8 keep their relative precision in the two bf16 numbers.
+            const bool moves = next > m + 8.f;
+            const float alpha = moves && j ? exp2_fast(m - next) : 1.f;
+            if (moves) m = next;
+            const float from = m == -INFINITY ? 0.f : m;
             l *= alpha;
-            const uint64_t minus_m = pair2(-from, -from);
-            uint64_t total2[2] = {0, 0};
-            uint32_t high[kTcKeys / 2], rest[kTcKeys / 2];
-#pragma unroll
-            for (int c = 0; c < kTcKeys; c += 2) {
-                float x0, x1;
-                unpair2(mul2(add2(pair2(__uint_as_float(s[c]), __uint_as_float(s[c + 1])), minus_m), scale_pair), x0, x1);
-                const float p0 = exp2_fast(x0), p1 = exp2_fast(x1);
-                total2[(c >> 1) & 1] = add2(total2[(c >> 1) & 1], pair2(p0, p1));
-                split2(p0, p1, high[c >> 1], rest[c >> 1]);
-            }
             if (j > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
                 // O is whole once the product of the block before is done
                 ok = wait.all(bar(V_EMPTY + (j - 1) % L::kStages), (uint32_t)((j - 1) / L::kStages) & 1u);
                 if (!ok) break;
                 tc_fence_after();
                 const uint64_t alpha_pair = pair2(alpha, alpha);
-#pragma unroll
-                for (int e = 0; e < DIM; e += 32) {
-                    uint32_t o[32];
-                    tmem_ld32(tmem_o + lane_base + e, o);
+#pragma unroll 1
+                for (int e = 0; e < DIM; e += 16) {
+                    uint32_t o[16];
+                    tmem_ld16(tmem_o + lane_base + e, o);
                     tmem_ld_wait();
 #pragma unroll
-                    for (int c = 0; c < 32; c += 2) {
+                    for (int c = 0; c < 16; c += 2) {
                         float o0, o1;
                         unpair2(mul2(pair2(__uint_as_float(o[c]), __uint_as_float(o[c + 1])), alpha_pair), o0, o1);
                         o[c] = __float_as_uint(o0);
                         o[c + 1] = __float_as_uint(o1);
                     }
-                    tmem_st32(tmem_o + lane_base + e, o);
+                    tmem_st16(tmem_o + lane_base + e, o);
                 }
             }
-            tmem_st32(tmem_s, high);
-            tmem_st32(tmem_s + 32, rest);
+            const uint64_t minus_m = pair2(-from, -from);
+            uint64_t total2[2] = {0, 0};
+            // 32 keys at a time, back over their scores: the larger parts of their probabilities, then the rest
+#pragma unroll
+            for (int h = 0; h < kTcKeys; h += 32) {
+                uint32_t high[16], rest[16];
+#pragma unroll
+                for (int c = 0; c < 32; c += 2) {
+                    float x0, x1;
+                    unpair2(fma2(pair2(__uint_as_float(s[h + c]), __uint_as_float(s[h + c + 1])), scale_pair, minus_m), x0, x1);
+                    float p0 = exp2_fast(x0), p1 = exp2_fast(x1);
+                    total2[(c >> 1) & 1] = add2(total2[(c >> 1) & 1], pair2(p0, p1));
+                    if constexpr (INT8) {
+                        const float2 f = *reinterpret_cast<const float2*>(scales + (st * 2 + 1) * kTcKeys + h + c);
+                        unpair2(mul2(pair2(p0, p1), pair2(f.x, f.y)), p0, p1);
+                    }
+                    split2(p0, p1, high[c >> 1], rest[c >> 1]);
+                }
+                tmem_st16(tmem_s + h, high);
+                tmem_st16(tmem_s + h + 16, rest);
+            }
             tmem_st_wait();
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(bar(P_FULL + (j & 1)));
+            if (lane == 0) mbar_arrive(bar(P_FULL + j % L::kBuffers));
             float t0, t1;
             unpair2(add2(total2[0], total2[1]), t0, t1);
             l += t0 + t1;
@@ -576,7 +679,7 @@ prefix_tensor_kernel(const __grid_constant__ PrefixTcParams tc) {
             const long long slot = (long long)(p.prefix.first_slot + split) * p.rows + at;
             const float inverse = l > 0.f ? 1.f / l : 0.f;
             if (live) {
-                if (whole) p.lse[at] = l > 0.f ? m * p.scale + logf(l) : -INFINITY;
+                if (whole) p.lse[at] = l > 0.f ? (m + log2f(l)) * LN2 : -INFINITY;
                 else p.part_ml[slot] = make_float2(m, l);
             }
             if (n || whole) {
@@ -617,7 +720,6 @@ prefix_join_kernel(const __grid_constant__ PrefixParams p) {
     const long long row = (long long)blockIdx.x * kWarps + (threadIdx.x >> 5);
     const int lane = threadIdx.x & 31;
     if (row >= p.rows) return;
-    const float scale2 = p.scale * LOG2E;
     float top = -INFINITY, total = 0.f;
     for (int s = lane; s < p.slots; s += 32) top = fmaxf(top, p.part_ml[s * p.rows + row].x);
     top = warp_max(top);
@@ -628,7 +730,7 @@ prefix_join_kernel(const __grid_constant__ PrefixParams p) {
     for (int s = lane / LANES; s < p.slots; s += TOGETHER) {
         const float2 ml = p.part_ml[s * p.rows + row];
         if (ml.y == 0.f) continue;                               // saw no key: its values were not written
-        const float factor = exp2_fast((ml.x - from) * scale2);
+        const float factor = exp2_fast(ml.x - from);
         const float4 v = *reinterpret_cast<const float4*>(p.part_o + (s * p.rows + row) * DIM + lane % LANES * 4);
         total += factor * ml.y;
         sum.x += factor * v.x; sum.y += factor * v.y; sum.z += factor * v.z; sum.w += factor * v.w;
@@ -643,7 +745,7 @@ prefix_join_kernel(const __grid_constant__ PrefixParams p) {
     }
     const float inverse = total > 0.f ? 1.f / total : 0.f;
     if (lane < LANES) *reinterpret_cast<uint2*>(p.out + row * DIM + lane * 4) = make_uint2(pack2(sum.x * inverse, sum.y * inverse), pack2(sum.z * inverse, sum.w * inverse));
-    if (lane == 0) p.lse[row] = total > 0.f ? top * p.scale + logf(total) : -INFINITY;
+    if (lane == 0) p.lse[row] = total > 0.f ? (top + log2f(total)) * LN2 : -INFINITY;
 }
 
 struct Plan { Keys prefix, own; int slots; long long prefix_items, own_items; bool tensor, prefix_by_keys, own_by_keys; };
@@ -652,7 +754,7 @@ struct Plan { Keys prefix, own; int slots; long long prefix_items, own_items; bo
 Plan plan_of(const qmoe_prefix_attention_t* a, const qmoe_cache_t* c) {
     Plan plan = {};
     const long long group = a->heads / c->kv_heads, own_rows = a->time * group, all_rows = c->batch * own_rows;
-    plan.tensor = c->dtype == QMOE_BF16 && group <= 128 && all_rows > 64 && a->prefix_longest >= 2 * kTcKeys;
+    plan.tensor = group <= 128 && all_rows > 64 && a->prefix_longest >= 2 * kTcKeys;
     plan.prefix_by_keys = all_rows <= 16;
     plan.own_by_keys = own_rows <= 16;
     plan.prefix.row_tiles = plan.tensor ? ceil_div(c->batch * a->time, 128 / group) : ceil_div(all_rows, plan.prefix_by_keys ? 16 : 64);
@@ -702,18 +804,21 @@ int prefix_attention_check(const qmoe_prefix_attention_t* a, const qmoe_cache_t*
     return 0;
 }
 
-template <int DIM>
+template <int DIM, bool INT8>
 int launch_tensor(const PrefixParams& p, const Plan& plan, const qmoe_cache_t* prefix, cudaStream_t stream) {
+    using L = TcTile<DIM, INT8>;
     PrefixTcParams tc = {};
     const uint32_t group = (uint32_t)p.group, sequences = 128 / group;
     if (int rc = make_map_3d(&tc.map_q, (uint64_t)p.q, DIM, (uint64_t)group * p.kv_heads, (uint64_t)p.batch * p.time, group, sequences)) return rc;
-    if (int rc = make_map_3d(&tc.map_k, prefix->k, DIM, (uint64_t)prefix->capacity, (uint64_t)p.kv_heads, kTcKeys)) return rc;
-    if (int rc = make_map_3d(&tc.map_v, prefix->v, DIM, (uint64_t)prefix->capacity, (uint64_t)p.kv_heads, kTcKeys)) return rc;
+    if (!INT8) {
+        if (int rc = make_map_3d(&tc.map_k, prefix->k, DIM, (uint64_t)prefix->capacity, (uint64_t)p.kv_heads, kTcKeys)) return rc;
+        if (int rc = make_map_3d(&tc.map_v, prefix->v, DIM, (uint64_t)prefix->capacity, (uint64_t)p.kv_heads, kTcKeys)) return rc;
+    }
     tc.p = p;
     tc.status = device_status_address();
     tc.sequences = (int)sequences;
-    QMOE_CUDA(cudaFuncSetAttribute(prefix_tensor_kernel<DIM>, cudaFuncAttributeMaxDynamicSharedMemorySize, TcTile<DIM>::kShared));
-    chained(prefix_tensor_kernel<DIM>, (unsigned)plan.prefix_items, kTcThreads, TcTile<DIM>::kShared, stream, tc);
+    QMOE_CUDA(cudaFuncSetAttribute(prefix_tensor_kernel<DIM, INT8>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kShared));
+    chained(prefix_tensor_kernel<DIM, INT8>, (unsigned)plan.prefix_items, L::kThreads, L::kShared, stream, tc);
     count_tensor_core_launch();
     QMOE_LAUNCH_CHECK("prefix_tensor_kernel");
     return 0;
@@ -724,8 +829,7 @@ int launch(PrefixParams& p, const Plan& plan, const qmoe_cache_t* prefix, cudaSt
     constexpr int SHARED = Tile<DIM, INT8>::kShared;
     long long items = plan.prefix_items + plan.own_items;
     if (plan.tensor) {
-        if constexpr (!INT8)
-            if (int rc = launch_tensor<DIM>(p, plan, prefix, stream)) return rc;
+        if (int rc = launch_tensor<DIM, INT8>(p, plan, prefix, stream)) return rc;
         p.prefix_items = 0;
         items = plan.own_items;
     }
