@@ -17,7 +17,6 @@ namespace {
 
 constexpr int kWarps = 4, kThreads = 32 * kWarps;
 constexpr int kKeys = 64;                // keys of a tile
-constexpr int kStages = 3;
 constexpr float LN2 = 0.6931471805599453f;
 
 struct Keys {                            // the prefix, or the sequences' caches
@@ -97,6 +96,7 @@ template <int DIM, bool INT8> struct Tile {
     static constexpr int kRowBytes = INT8 ? DIM : 2 * DIM;
     static constexpr int kPitch = kRowBytes + 16;                  // 16 more: no two of the rows read together share a bank
     static constexpr int kBytes = kKeys * kPitch;
+    static constexpr int kStages = DIM == 128 && !INT8 ? 2 : 3;    // the wide ones as many as leave room for two blocks on an SM
     static constexpr int kStage = 2 * kBytes + (INT8 ? 2 * kKeys * 4 : 0);
     static constexpr int kJoin = kWarps * 16 * (DIM + 4) * 4;      // the warps' parts, where they share the keys
     static constexpr int kShared = kStages * kStage > kJoin ? kStages * kStage : kJoin;
@@ -104,6 +104,9 @@ template <int DIM, bool INT8> struct Tile {
 
 // Rows of a tile: 16 to a warp (BY_KEYS false: 64 rows, every warp walks all keys) or the same 16 for all warps (BY_KEYS: a
 // quarter of every tile of keys each, joined at the end), for the few rows of one sequence.
+// of the threads that attend, in whatever block
+__device__ __forceinline__ void attend_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kThreads) : "memory"); }
+
 template <int DIM, bool INT8, bool BY_KEYS>
 __device__ __forceinline__ void attend(const PrefixParams& p, const Keys& keys, uint8_t* smem, int b, int g, int row_tile, int split, bool own) {
     using L = Tile<DIM, INT8>;
@@ -140,7 +143,7 @@ __device__ __forceinline__ void attend(const PrefixParams& p, const Keys& keys, 
     const uint32_t base = smem_u32(smem);
     const long long head = ((own ? (long long)b * p.kv_heads : 0) + g) * keys.capacity;
     auto fetch = [&](int tile) {         // keys begin + 64 tile ..; behind `end` zeros, whatever lies there
-        const uint32_t stage = base + (tile % kStages) * L::kStage;
+        const uint32_t stage = base + (tile % L::kStages) * L::kStage;
         const int first = begin + tile * kKeys;
         constexpr int PIECES = L::kRowBytes / 16;
 #pragma unroll
@@ -164,16 +167,16 @@ __device__ __forceinline__ void attend(const PrefixParams& p, const Keys& keys, 
     const int tiles = end > begin ? (end - begin + kKeys - 1) / kKeys : 0;
     const float scale2 = p.scale * LOG2E;
 #pragma unroll
-    for (int s = 0; s < kStages - 1; ++s) {
+    for (int s = 0; s < L::kStages - 1; ++s) {
         if (s < tiles) fetch(s);
         copies_commit();
     }
     for (int j = 0; j < tiles; ++j) {
-        copies_wait<kStages - 2>();
-        __syncthreads();                 // tile j is here, and nobody reads the stage that is filled next
-        if (j + kStages - 1 < tiles) fetch(j + kStages - 1);
+        copies_wait<L::kStages - 2>();
+        attend_sync();                 // tile j is here, and nobody reads the stage that is filled next
+        if (j + L::kStages - 1 < tiles) fetch(j + L::kStages - 1);
         copies_commit();
-        const uint32_t k_tile = base + (j % kStages) * L::kStage, v_tile = k_tile + L::kBytes, scales = k_tile + 2 * L::kBytes;
+        const uint32_t k_tile = base + (j % L::kStages) * L::kStage, v_tile = k_tile + L::kBytes, scales = k_tile + 2 * L::kBytes;
         const int key0 = BY_KEYS ? warp * 16 : 0, first = begin + j * kKeys + key0;
         float s[NT][4];
 #pragma unroll
@@ -284,7 +287,7 @@ __device__ __forceinline__ void attend(const PrefixParams& p, const Keys& keys, 
     if constexpr (BY_KEYS) {
         // rows [warp][16][DIM + 4] with m and l behind the row's DIM values
         float* part = reinterpret_cast<float*>(smem);
-        __syncthreads();
+        attend_sync();
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             float* row = part + (warp * 16 + quad + 8 * i) * (DIM + 4);
@@ -295,7 +298,7 @@ __device__ __forceinline__ void attend(const PrefixParams& p, const Keys& keys, 
             }
             if (t4 == 0) { row[DIM] = m[i]; row[DIM + 1] = l[i]; }
         }
-        __syncthreads();
+        attend_sync();
         // eight lanes to a row
         const int r = threadIdx.x >> 3, piece = threadIdx.x & 7, mine = row_tile * ROWS + r;
         if (mine >= rows) return;
@@ -385,7 +388,7 @@ template <int DIM, bool INT8> struct TcTile {
     static constexpr int kBuffers = DIM == 64 ? 3 : 2;             // of scores: with O all of a CTA's 256 columns
     static constexpr int kTiles = kQ + 2 * kStages * kKey;
     static constexpr int kScales = INT8 ? kStages * 2 * kTcKeys * 4 : 0;
-    static constexpr int kShared = kTiles + 256 + kScales;
+    static constexpr int kNeeded = kTiles + 256 + kScales, kShared = kNeeded > Tile<DIM, INT8>::kShared ? kNeeded : Tile<DIM, INT8>::kShared;
 };
 
 struct alignas(64) PrefixTcParams {
@@ -406,12 +409,21 @@ __device__ __forceinline__ void store_bytes(uint32_t row, int piece, int key, co
     }
 }
 
-template <int DIM, bool INT8>
+// The blocks behind the prefix's items see the sequences' own caches, as in prefix_attention_kernel, one launch for both.
+template <int DIM, bool INT8, bool OWN_BY_KEYS>
 __global__ void __launch_bounds__(TcTile<DIM, INT8>::kThreads, 2)
 prefix_tensor_kernel(const __grid_constant__ PrefixTcParams tc) {
     using L = TcTile<DIM, INT8>;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     const PrefixParams& p = tc.p;
+    if ((int)blockIdx.x >= p.prefix_items) {
+        chain_wait();
+        chain_next();
+        if (threadIdx.x >= kThreads) return;
+        const int item = (int)blockIdx.x - p.prefix_items, split = item % p.own.splits, tile = item / p.own.splits, head = tile / p.own.row_tiles;
+        attend<DIM, INT8, OWN_BY_KEYS>(p, p.own, smem_raw, head / p.kv_heads, head % p.kv_heads, tile % p.own.row_tiles, split, true);
+        return;
+    }
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int split = (int)blockIdx.x % p.prefix.splits, tile = (int)blockIdx.x / p.prefix.splits;
     const int g = tile % p.kv_heads, first_sequence = tile / p.kv_heads * tc.sequences;
@@ -577,11 +589,13 @@ prefix_tensor_kernel(const __grid_constant__ PrefixTcParams tc) {
         const uint64_t scale_pair = pair2(scale2, scale2);
         float m = -INFINITY, l = 0.f;
         bool ok = true;
+        int st = 0, buffer = 0;          // of the block, and how often they have come round
+        uint32_t st_round = 0, buffer_round = 0;
         for (int j = 0; ok && j < n; ++j) {
-            const int st = j % L::kStages, there = end - begin - j * kTcKeys;            // keys of the block
-            const uint32_t tmem_s = tmem + (uint32_t)(j % L::kBuffers) * kTcKeys + lane_base;
-            ok = wait.all(bar(S_FULL + j % L::kBuffers), (uint32_t)(j / L::kBuffers) & 1u);
-            if (ok && (INT8 || there < kTcKeys)) ok = wait.all(bar(V_FULL + st), (uint32_t)(j / L::kStages) & 1u);
+            const int there = end - begin - j * kTcKeys;            // keys of the block
+            const uint32_t tmem_s = tmem + (uint32_t)buffer * kTcKeys + lane_base;
+            ok = wait.all(bar(S_FULL + buffer), buffer_round);
+            if (ok && (INT8 || there < kTcKeys)) ok = wait.all(bar(V_FULL + st), st_round);
             if (!ok) break;
             tc_fence_after();
             uint32_t s[kTcKeys];
@@ -668,7 +682,9 @@ prefix_tensor_kernel(const __grid_constant__ PrefixTcParams tc) {
             tmem_st_wait();
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(bar(P_FULL + j % L::kBuffers));
+            if (lane == 0) mbar_arrive(bar(P_FULL + buffer));
+            if (++st == L::kStages) { st = 0; st_round ^= 1u; }
+            if (++buffer == L::kBuffers) { buffer = 0; buffer_round ^= 1u; }
             float t0, t1;
             unpair2(add2(total2[0], total2[1]), t0, t1);
             l += t0 + t1;
@@ -712,7 +728,7 @@ prefix_tensor_kernel(const __grid_constant__ PrefixTcParams tc) {
     }
 }
 
-// A warp per row: the parts' weights, then their weighted sum
+// A warp per row: the parts' weights, a lane each, then their weighted sum, eight parts' values on their way together
 template <int DIM>
 __global__ void __launch_bounds__(kThreads)
 prefix_join_kernel(const __grid_constant__ PrefixParams p) {
@@ -720,24 +736,33 @@ prefix_join_kernel(const __grid_constant__ PrefixParams p) {
     const long long row = (long long)blockIdx.x * kWarps + (threadIdx.x >> 5);
     const int lane = threadIdx.x & 31;
     if (row >= p.rows) return;
+    constexpr int LANES = DIM / 4, TOGETHER = 32 / LANES, DEEP = 8 / TOGETHER;        // lanes of a part's row, parts at a time, such loads in flight
     float top = -INFINITY, total = 0.f;
-    for (int s = lane; s < p.slots; s += 32) top = fmaxf(top, p.part_ml[s * p.rows + row].x);
-    top = warp_max(top);
-    const float from = top == -INFINITY ? 0.f : top;
-    constexpr int LANES = DIM / 4, TOGETHER = 32 / LANES;        // lanes of a part's row, parts at a time
     float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-    for (int s = lane / LANES; s < p.slots; s += TOGETHER) {
-        const float2 ml = p.part_ml[s * p.rows + row];
-        if (ml.y == 0.f) continue;                               // saw no key: its values were not written
-        const float factor = exp2_fast(ml.x - from);
-        const float4 v = *reinterpret_cast<const float4*>(p.part_o + (s * p.rows + row) * DIM + lane % LANES * 4);
-        total += factor * ml.y;
-        sum.x += factor * v.x; sum.y += factor * v.y; sum.z += factor * v.z; sum.w += factor * v.w;
+    for (int first = 0; first < p.slots; first += 32) {
+        const float2 ml = first + lane < p.slots ? p.part_ml[(first + lane) * p.rows + row] : make_float2(-INFINITY, 0.f);
+        const float next = fmaxf(top, warp_max(ml.x)), from = next == -INFINITY ? 0.f : next, alpha = exp2_fast(top - from);
+        const float factor = ml.y == 0.f ? 0.f : exp2_fast(ml.x - from);             // 0: saw no key, its values were not written
+        top = next;
+        total = total * alpha + warp_sum(factor * ml.y);
+        sum.x *= alpha; sum.y *= alpha; sum.z *= alpha; sum.w *= alpha;
+        const int many = min(32, p.slots - first);
+        for (int s = 0; s < many; s += TOGETHER * DEEP) {
+            float4 v[DEEP];
+            float f[DEEP];
+#pragma unroll
+            for (int i = 0; i < DEEP; ++i) {
+                const int slot = s + i * TOGETHER + lane / LANES;
+                f[i] = __shfl_sync(0xffffffffu, factor, slot & 31);
+                if (slot >= many) f[i] = 0.f;
+                v[i] = f[i] != 0.f ? *reinterpret_cast<const float4*>(p.part_o + ((first + slot) * p.rows + row) * DIM + lane % LANES * 4) : make_float4(0.f, 0.f, 0.f, 0.f);
+            }
+#pragma unroll
+            for (int i = 0; i < DEEP; ++i) { sum.x += f[i] * v[i].x; sum.y += f[i] * v[i].y; sum.z += f[i] * v[i].z; sum.w += f[i] * v[i].w; }
+        }
     }
 #pragma unroll
     for (int o = LANES; o < 32; o <<= 1) {
-        total += __shfl_xor_sync(0xffffffffu, total, o);
         sum.x += __shfl_xor_sync(0xffffffffu, sum.x, o);
         sum.y += __shfl_xor_sync(0xffffffffu, sum.y, o);
         sum.z += __shfl_xor_sync(0xffffffffu, sum.z, o);
@@ -748,9 +773,9 @@ prefix_join_kernel(const __grid_constant__ PrefixParams p) {
     if (lane == 0) p.lse[row] = total > 0.f ? (top + log2f(total)) * LN2 : -INFINITY;
 }
 
-struct Plan { Keys prefix, own; int slots; long long prefix_items, own_items; bool tensor, prefix_by_keys, own_by_keys; };
+struct Plan { Keys prefix, own; int slots; long long prefix_items, own_items; bool tensor, together, prefix_by_keys, own_by_keys; };
 
-// Chunks of keys: as long as they leave four items to an SM, but not below two tiles.
+// Chunks of keys: as long as they leave three items to an SM, but not below two tiles.
 Plan plan_of(const qmoe_prefix_attention_t* a, const qmoe_cache_t* c) {
     Plan plan = {};
     const long long group = a->heads / c->kv_heads, own_rows = a->time * group, all_rows = c->batch * own_rows;
@@ -759,7 +784,7 @@ Plan plan_of(const qmoe_prefix_attention_t* a, const qmoe_cache_t* c) {
     plan.own_by_keys = own_rows <= 16;
     plan.prefix.row_tiles = plan.tensor ? ceil_div(c->batch * a->time, 128 / group) : ceil_div(all_rows, plan.prefix_by_keys ? 16 : 64);
     plan.own.row_tiles = ceil_div(own_rows, plan.own_by_keys ? 16 : 64);
-    const long long prefix_tiles = ceil_div(a->prefix_longest, kKeys), own_tiles = ceil_div(a->longest, kKeys), wanted = (long long)sm_count() * 4;
+    const long long prefix_tiles = ceil_div(a->prefix_longest, kKeys), own_tiles = ceil_div(a->longest, kKeys), wanted = (long long)sm_count() * 3;
     const long long prefix_heads = (long long)plan.prefix.row_tiles * c->kv_heads, own_heads = (long long)plan.own.row_tiles * c->kv_heads * c->batch;
     const long long prefix_mma = plan.tensor ? 0 : prefix_tiles;
     long long chunk = prefix_mma > own_tiles ? prefix_mma : own_tiles;
@@ -779,6 +804,9 @@ Plan plan_of(const qmoe_prefix_attention_t* a, const qmoe_cache_t* c) {
     plan.slots = plan.prefix.splits + plan.own.splits;
     plan.prefix_items = prefix_heads * plan.prefix.splits;
     plan.own_items = own_heads * plan.own.splits;
+    // One launch for both while the sequences' items are few.  Many of them are better off with a launch of their own, whose blocks are small and
+    // three to four on an SM (128 sequences, 8 heads: 110 us, in one launch 117; 64 sequences, 4 heads: 27, in one launch 24).
+    plan.together = plan.own_items <= 4ll * sm_count();
     return plan;
 }
 
@@ -804,7 +832,7 @@ int prefix_attention_check(const qmoe_prefix_attention_t* a, const qmoe_cache_t*
     return 0;
 }
 
-template <int DIM, bool INT8>
+template <int DIM, bool INT8, bool OWN_BY_KEYS>
 int launch_tensor(const PrefixParams& p, const Plan& plan, const qmoe_cache_t* prefix, cudaStream_t stream) {
     using L = TcTile<DIM, INT8>;
     PrefixTcParams tc = {};
@@ -817,8 +845,9 @@ int launch_tensor(const PrefixParams& p, const Plan& plan, const qmoe_cache_t* p
     tc.p = p;
     tc.status = device_status_address();
     tc.sequences = (int)sequences;
-    QMOE_CUDA(cudaFuncSetAttribute(prefix_tensor_kernel<DIM, INT8>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kShared));
-    chained(prefix_tensor_kernel<DIM, INT8>, (unsigned)plan.prefix_items, L::kThreads, L::kShared, stream, tc);
+    const auto kernel = prefix_tensor_kernel<DIM, INT8, OWN_BY_KEYS>;
+    QMOE_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kShared));
+    chained(kernel, (unsigned)(plan.prefix_items + (plan.together ? plan.own_items : 0)), L::kThreads, L::kShared, stream, tc);
     count_tensor_core_launch();
     QMOE_LAUNCH_CHECK("prefix_tensor_kernel");
     return 0;
@@ -826,14 +855,14 @@ int launch_tensor(const PrefixParams& p, const Plan& plan, const qmoe_cache_t* p
 
 template <int DIM, bool INT8>
 int launch(PrefixParams& p, const Plan& plan, const qmoe_cache_t* prefix, cudaStream_t stream) {
-    constexpr int SHARED = Tile<DIM, INT8>::kShared;
     long long items = plan.prefix_items + plan.own_items;
     if (plan.tensor) {
-        if (int rc = launch_tensor<DIM, INT8>(p, plan, prefix, stream)) return rc;
+        if (int rc = plan.own_by_keys ? launch_tensor<DIM, INT8, true>(p, plan, prefix, stream) : launch_tensor<DIM, INT8, false>(p, plan, prefix, stream)) return rc;
+        items = plan.together ? 0 : plan.own_items;
         p.prefix_items = 0;
-        items = plan.own_items;
     }
     auto go = [&](auto kernel) -> int {
+        constexpr int SHARED = Tile<DIM, INT8>::kShared;
         QMOE_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SHARED));
         chained(kernel, (unsigned)items, kThreads, SHARED, stream, p);
         QMOE_LAUNCH_CHECK("prefix_attention_kernel");
@@ -841,7 +870,7 @@ int launch(PrefixParams& p, const Plan& plan, const qmoe_cache_t* prefix, cudaSt
     };
     int rc = 0;
     if (!items) {}
-    else if (plan.prefix_by_keys) rc = go(prefix_attention_kernel<DIM, INT8, true, true>);        // few rows in all: few in a sequence
+    else if (plan.own_by_keys && (plan.tensor || plan.prefix_by_keys)) rc = go(prefix_attention_kernel<DIM, INT8, true, true>);
     else if (plan.own_by_keys) rc = go(prefix_attention_kernel<DIM, INT8, false, true>);
     else rc = go(prefix_attention_kernel<DIM, INT8, false, false>);
     if (rc || plan.slots == 1) return rc;
