@@ -6,8 +6,10 @@
 // bf16, so the attention that reads them can hand them to the tensor cores as they are.  The division is the rounded one
 // of IEEE, not a product with the reciprocal: x / s then lies on the same side of a tie everywhere.
 //
-// dim / 8 lanes (rounded up to a power of two) hold a head of one position, eight values each.
+// dim / 16 lanes (rounded up to a power of two) hold a head of one position, 16 values each.
 #include "common.cuh"
+
+#include <type_traits>
 
 namespace qmoe {
 namespace {
@@ -15,13 +17,17 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kMaxDim = 256;
 
+// Values of a lane: 16, so that its 8-bit ones are one 16-byte access; 8 where the head width is no multiple of that
+int lane_values(const qmoe_cache_t* c) { return c->dim % 16 ? 8 : 16; }
+
 struct CacheParams {
     void* k;
     void* v;
     float* k_scale;
     float* v_scale;
     const int* lengths;
-    long long capacity, units;           // units: heads of positions, keys and values counted once
+    long long capacity;
+    unsigned units;                      // heads of positions, keys and values counted once
     int batch, kv_heads, dim, lane_bits;
     // append
     const void* k_in;
@@ -36,13 +42,13 @@ struct CacheParams {
     long long start, count;
 };
 
-template <typename T> __device__ __forceinline__ void load_values(const T* p, float* f) {
+template <int V, typename T> __device__ __forceinline__ void load_values(const T* p, float* f) {
 #pragma unroll
-    for (int i = 0; i < 8; i += Vec16<T>::N) Vec16<T>::unpack(*reinterpret_cast<const uint4*>(p + i), f + i);
+    for (int i = 0; i < V; i += Vec16<T>::N) Vec16<T>::unpack(*reinterpret_cast<const uint4*>(p + i), f + i);
 }
-template <typename T> __device__ __forceinline__ void store_values(T* p, const float* f) {
+template <int V, typename T> __device__ __forceinline__ void store_values(T* p, const float* f) {
 #pragma unroll
-    for (int i = 0; i < 8; i += Vec16<T>::N) *reinterpret_cast<uint4*>(p + i) = Vec16<T>::pack(f + i);
+    for (int i = 0; i < V; i += Vec16<T>::N) *reinterpret_cast<uint4*>(p + i) = Vec16<T>::pack(f + i);
 }
 __device__ __forceinline__ float max_or_nan(float a, float b) {      // a NaN among the values ends in the scale, not under the carpet
     float r;
@@ -54,76 +60,79 @@ __device__ __forceinline__ uint32_t pack_bytes(const int* q) {
     return (uint32_t)(q[0] & 255) | (uint32_t)(q[1] & 255) << 8 | (uint32_t)(q[2] & 255) << 16 | (uint32_t)q[3] << 24;
 }
 
-// Keys in blockIdx.y = 0, values in 1.
-template <typename T, bool INT8>
+template <int V> struct Bytes;           // V of them as one access
+template <> struct Bytes<8> { using type = uint2; };
+template <> struct Bytes<16> { using type = uint4; };
+
+// Keys in blockIdx.y = 0, values in 1.  V values to a lane; a thread has its part of one head of one position.
+template <typename T, bool INT8, int V>
 __global__ void __launch_bounds__(kThreads)
 cache_append_kernel(const __grid_constant__ CacheParams p) {
     chain_begin();
     const bool key = blockIdx.y == 0;
     const int lanes = 1 << p.lane_bits, sub = threadIdx.x & (lanes - 1);
-    const long long stride = (long long)gridDim.x * (kThreads >> p.lane_bits);
     if (key)
         for (long long b = (long long)blockIdx.x * kThreads + threadIdx.x; b < p.batch; b += (long long)gridDim.x * kThreads) {
             const int n = p.counts ? min(max(p.counts[b], 0), p.time) : p.time;
             p.lengths_out[b] = (int)min(p.capacity, (long long)p.lengths[b] + n);
         }
-    // a warp's lanes go round together: the shuffles below need all of them
-    for (long long unit = (long long)blockIdx.x * (kThreads >> p.lane_bits) + (threadIdx.x >> p.lane_bits);
-         __any_sync(0xffffffffu, unit < p.units); unit += stride) {
-        const bool in = unit < p.units;
-        const long long row = in ? unit / p.kv_heads : 0;
-        const int h = in ? (int)(unit - row * p.kv_heads) : 0, b = (int)(row / p.time), t = (int)(row - (long long)b * p.time);
-        const long long position = (long long)p.lengths[b] + t;
-        const bool live = in && t < (p.counts ? min(p.counts[b], p.time) : p.time) && position >= 0 && position < p.capacity;
-        const bool active = live && sub * 8 < p.dim;
-        float f[8] = {};
-        if (active) load_values((key ? (const T*)p.k_in + row * p.k_pitch : (const T*)p.v_in + row * p.v_pitch) + h * p.dim + 8 * sub, f);
-        const long long at = ((long long)b * p.kv_heads + h) * p.capacity + position;
-        if constexpr (INT8) {
-            float most = 0.f;
+    const unsigned unit = blockIdx.x * (kThreads >> p.lane_bits) + (threadIdx.x >> p.lane_bits);
+    const bool in = unit < p.units;      // (the shuffles below need all of a warp's lanes)
+    const unsigned row = in ? unit / (unsigned)p.kv_heads : 0, b = row / (unsigned)p.time;
+    const int h = in ? (int)(unit - row * p.kv_heads) : 0, t = (int)(row - b * p.time);
+    const long long position = (long long)p.lengths[b] + t;
+    const bool live = in && t < (p.counts ? min(p.counts[b], p.time) : p.time) && position >= 0 && position < p.capacity;
+    const bool active = live && sub * V < p.dim;
+    float f[V] = {};
+    if (active) load_values<V>((key ? (const T*)p.k_in + row * p.k_pitch : (const T*)p.v_in + row * p.v_pitch) + h * p.dim + V * sub, f);
+    const long long at = ((long long)b * p.kv_heads + h) * p.capacity + position;
+    if constexpr (INT8) {
+        float most = 0.f;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) most = max_or_nan(most, fabsf(f[i]));
-            for (int o = 1; o < lanes; o <<= 1) most = max_or_nan(most, __shfl_xor_sync(0xffffffffu, most, o));
-            const float scale = __fdiv_rn(most, 127.f);
-            int q[8];
+        for (int i = 0; i < V; ++i) most = max_or_nan(most, fabsf(f[i]));
+        for (int o = 1; o < lanes; o <<= 1) most = max_or_nan(most, __shfl_xor_sync(0xffffffffu, most, o));
+        const float scale = __fdiv_rn(most, 127.f);
+        if (!active) return;
+        uint32_t words[V / 4];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) q[i] = scale > 0.f ? min(max(__float2int_rn(__fdiv_rn(f[i], scale)), -127), 127) : 0;
-            if (active) {
-                *reinterpret_cast<uint2*>((int8_t*)(key ? p.k : p.v) + at * p.dim + 8 * sub) = make_uint2(pack_bytes(q), pack_bytes(q + 4));
-                if (sub == 0) (key ? p.k_scale : p.v_scale)[at] = scale;
-            }
-        } else if (active) {
-            store_values((__nv_bfloat16*)(key ? p.k : p.v) + at * p.dim + 8 * sub, f);
+        for (int i = 0; i < V; i += 4) {
+            int q[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) q[e] = scale > 0.f ? min(max(__float2int_rn(__fdiv_rn(f[i + e], scale)), -127), 127) : 0;
+            words[i / 4] = pack_bytes(q);
         }
+        *reinterpret_cast<typename Bytes<V>::type*>((int8_t*)(key ? p.k : p.v) + at * p.dim + V * sub) = *reinterpret_cast<const typename Bytes<V>::type*>(words);
+        if (sub == 0) (key ? p.k_scale : p.v_scale)[at] = scale;
+    } else if (active) {
+        store_values<V>((__nv_bfloat16*)(key ? p.k : p.v) + at * p.dim + V * sub, f);
     }
 }
 
-template <typename T, bool INT8>
+template <typename T, bool INT8, int V>
 __global__ void __launch_bounds__(kThreads)
 cache_read_kernel(const __grid_constant__ CacheParams p) {
     chain_begin();
     const bool key = blockIdx.y == 0;
     const int sub = threadIdx.x & ((1 << p.lane_bits) - 1);
-    if (sub * 8 >= p.dim) return;
-    const long long stride = (long long)gridDim.x * (kThreads >> p.lane_bits);
-    for (long long unit = (long long)blockIdx.x * (kThreads >> p.lane_bits) + (threadIdx.x >> p.lane_bits); unit < p.units; unit += stride) {
-        const long long row = unit / p.kv_heads, b = row / p.count, position = p.start + row - b * p.count;
-        const int h = (int)(unit - row * p.kv_heads);
-        float f[8] = {};
-        if (position < p.lengths[b] && position < p.capacity) {
-            const long long at = (b * p.kv_heads + h) * p.capacity + position;
-            if constexpr (INT8) {
-                const uint2 raw = *reinterpret_cast<const uint2*>((const int8_t*)(key ? p.k : p.v) + at * p.dim + 8 * sub);
-                const float scale = (key ? p.k_scale : p.v_scale)[at];
-                const uint32_t w[2] = {raw.x, raw.y};
+    const unsigned unit = blockIdx.x * (kThreads >> p.lane_bits) + (threadIdx.x >> p.lane_bits);
+    if (unit >= p.units || sub * V >= p.dim) return;
+    const unsigned row = unit / (unsigned)p.kv_heads, b = row / (unsigned)p.count;
+    const int h = (int)(unit - row * p.kv_heads);
+    const long long position = p.start + (row - b * (unsigned)p.count);
+    float f[V] = {};
+    if (position < p.lengths[b] && position < p.capacity) {
+        const long long at = ((long long)b * p.kv_heads + h) * p.capacity + position;
+        if constexpr (INT8) {
+            const typename Bytes<V>::type raw = *reinterpret_cast<const typename Bytes<V>::type*>((const int8_t*)(key ? p.k : p.v) + at * p.dim + V * sub);
+            const float scale = (key ? p.k_scale : p.v_scale)[at];
+            const uint32_t* w = reinterpret_cast<const uint32_t*>(&raw);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) f[i] = (float)(int8_t)(w[i >> 2] >> (8 * (i & 3))) * scale;
-            } else {
-                load_values((const __nv_bfloat16*)(key ? p.k : p.v) + at * p.dim + 8 * sub, f);
-            }
+            for (int i = 0; i < V; ++i) f[i] = (float)(int8_t)(w[i >> 2] >> (8 * (i & 3))) * scale;
+        } else {
+            load_values<V>((const __nv_bfloat16*)(key ? p.k : p.v) + at * p.dim + V * sub, f);
         }
-        store_values((T*)(key ? p.k_read : p.v_read) + (row * p.kv_heads + h) * p.dim + 8 * sub, f);
     }
+    store_values<V>((T*)(key ? p.k_read : p.v_read) + ((long long)row * p.kv_heads + h) * p.dim + V * sub, f);
 }
 
 CacheParams cache_params(const qmoe_cache_t* c) {
@@ -131,13 +140,31 @@ CacheParams cache_params(const qmoe_cache_t* c) {
     p.k = (void*)c->k; p.v = (void*)c->v; p.k_scale = (float*)c->k_scale; p.v_scale = (float*)c->v_scale;
     p.lengths = (const int*)c->lengths;
     p.capacity = c->capacity; p.batch = (int)c->batch; p.kv_heads = c->kv_heads; p.dim = c->dim;
-    while ((8 << p.lane_bits) < c->dim) ++p.lane_bits;
+    while ((lane_values(c) << p.lane_bits) < c->dim) ++p.lane_bits;
     return p;
 }
 
-dim3 cache_grid(const CacheParams& p) {
-    const long long blocks = (p.units + (kThreads >> p.lane_bits) - 1) / (kThreads >> p.lane_bits), most = (long long)sm_count() * 8;
-    return dim3((unsigned)(blocks < most ? blocks : most), 2);
+template <bool APPEND> int launch(CacheParams& p, const qmoe_cache_t* c, long long units, int dtype, cudaStream_t stream) {
+    if (units > 0x7fffffff / kThreads) return fail_arg("cache: too many positions in one call");
+    p.units = (unsigned)units;
+    const dim3 grid((unsigned)ceil_div(units, kThreads >> p.lane_bits), 2);
+    auto go = [&](auto value, auto int8, auto values) {
+        using T = decltype(value);
+        if constexpr (APPEND) chained(cache_append_kernel<T, decltype(int8)::value, decltype(values)::value>, grid, kThreads, 0, stream, p);
+        else chained(cache_read_kernel<T, decltype(int8)::value, decltype(values)::value>, grid, kThreads, 0, stream, p);
+    };
+    auto by_width = [&](auto value, auto int8) {
+        if (lane_values(c) == 16) go(value, int8, std::integral_constant<int, 16>());
+        else go(value, int8, std::integral_constant<int, 8>());
+    };
+    auto by_cache = [&](auto value) {
+        if (c->dtype == QMOE_INT8) by_width(value, std::true_type());
+        else by_width(value, std::false_type());
+    };
+    if (dtype == QMOE_BF16) by_cache(__nv_bfloat16());
+    else by_cache(float());
+    QMOE_LAUNCH_CHECK(APPEND ? "cache_append_kernel" : "cache_read_kernel");
+    return 0;
 }
 
 }  // namespace
@@ -178,17 +205,7 @@ extern "C" int qmoe_cache_append(const qmoe_cache_t* c, uint64_t k, uint64_t v, 
     CacheParams p = cache_params(c);
     p.k_in = (const void*)k; p.v_in = (const void*)v; p.k_pitch = k_pitch; p.v_pitch = v_pitch;
     p.counts = (const int*)counts; p.lengths_out = (int*)lengths_out; p.time = (int)time;
-    p.units = c->batch * time * c->kv_heads;
-    const dim3 grid = cache_grid(p);
-    if (c->dtype == QMOE_INT8) {
-        if (dtype == QMOE_BF16) chained(cache_append_kernel<__nv_bfloat16, true>, grid, kThreads, 0, stream, p);
-        else chained(cache_append_kernel<float, true>, grid, kThreads, 0, stream, p);
-    } else {
-        if (dtype == QMOE_BF16) chained(cache_append_kernel<__nv_bfloat16, false>, grid, kThreads, 0, stream, p);
-        else chained(cache_append_kernel<float, false>, grid, kThreads, 0, stream, p);
-    }
-    QMOE_LAUNCH_CHECK("cache_append_kernel");
-    return 0;
+    return launch<true>(p, c, c->batch * time * c->kv_heads, dtype, stream);
 }
 
 extern "C" int qmoe_cache_read(const qmoe_cache_t* c, int64_t start, int64_t count, uint64_t k_out, uint64_t v_out, int32_t dtype, uint64_t stream_) {
@@ -201,15 +218,5 @@ extern "C" int qmoe_cache_read(const qmoe_cache_t* c, int64_t start, int64_t cou
     TimedScope timed(KC_ELEMENTWISE, stream);
     CacheParams p = cache_params(c);
     p.k_read = (void*)k_out; p.v_read = (void*)v_out; p.start = start; p.count = count;
-    p.units = c->batch * count * c->kv_heads;
-    const dim3 grid = cache_grid(p);
-    if (c->dtype == QMOE_INT8) {
-        if (dtype == QMOE_BF16) chained(cache_read_kernel<__nv_bfloat16, true>, grid, kThreads, 0, stream, p);
-        else chained(cache_read_kernel<float, true>, grid, kThreads, 0, stream, p);
-    } else {
-        if (dtype == QMOE_BF16) chained(cache_read_kernel<__nv_bfloat16, false>, grid, kThreads, 0, stream, p);
-        else chained(cache_read_kernel<float, false>, grid, kThreads, 0, stream, p);
-    }
-    QMOE_LAUNCH_CHECK("cache_read_kernel");
-    return 0;
+    return launch<false>(p, c, c->batch * count * c->kv_heads, dtype, stream);
 }

@@ -5,7 +5,7 @@
 // The statistics are not kept from the forward: a head is in a few lanes' registers anyway.
 //
 // dim / 8 lanes (rounded up to a power of two) hold a head, eight elements each, so a warp has 32 / lanes heads at a time, and
-// goes through a chunk of a row's heads with the row's angles formed once.
+// goes through a chunk of a row's heads.  The row's angles are formed once, a pair to a lane, and handed on through shared memory.
 //
 // Angles.  A position times a frequency is a place on the circle, and what counts is its fraction of a turn: the frequency in
 // turns is held as a 64-bit fraction F (2^64 = one turn), so position * F modulo 2^64, an integer product, IS that fraction, exact to
@@ -36,8 +36,8 @@ struct NormRopeParams {
     float* partials;
     long long offset, q_pitch, k_pitch;
     int rows, time, heads, kv_heads, dim;
-    int lane_bits, passes;               // log2 of the lanes per head; heads of a lane per chunk
-    float eps;
+    int lane_bits, all_passes, passes;   // log2 of the lanes per head; passes of a row, of a chunk of it
+    float eps, one_over_dim;
     unsigned long long turns[kMaxDim / 2];
 };
 
@@ -60,128 +60,153 @@ __device__ __forceinline__ float head_sum(float v, int bits) {
     return v;
 }
 
-// What a lane keeps throughout: its place in a head, its frequencies and weights
-template <typename T> struct Lane {
-    int sub, slot, per_warp;
+// What a warp of a block has: its lanes' place in a head, the weights of query and key heads and the angles of its row in shared memory.  The
+// row's heads go by in passes of `per_warp` heads, the query heads' passes first, the key heads' behind them.
+template <typename T> struct Warp {
+    const NormRopeParams& p;
+    float2* angles;                      // cosine and sine of the row's dim / 2 angles
+    const float* weights;                // [query, key][dim]
+    int sub, slot, per_warp, query_passes;
     bool active;
-    unsigned long long turns[4];
-    float wq[8], wk[8];
-    __device__ __forceinline__ Lane(const NormRopeParams& p) {
+    __device__ __forceinline__ Warp(const NormRopeParams& p_, float2 (*s_angles)[kMaxDim / 2], float* s_weights) : p(p_) {
         const int lane = threadIdx.x & 31;
+        angles = s_angles[threadIdx.x >> 5];
+        weights = s_weights;
         sub = lane & ((1 << p.lane_bits) - 1);
         slot = lane >> p.lane_bits;
         per_warp = 32 >> p.lane_bits;
+        query_passes = (p.heads + per_warp - 1) >> (5 - p.lane_bits);
         active = sub * 8 < p.dim;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) turns[i] = active ? p.turns[4 * sub + i] : 0;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            wq[i] = active ? p.q_weight[8 * sub + i] : 0.f;
-            wk[i] = active ? p.k_weight[8 * sub + i] : 0.f;
-        }
+        for (int i = threadIdx.x; i < 2 * p.dim; i += kThreads) s_weights[i] = i < p.dim ? p.q_weight[i] : p.k_weight[i - p.dim];
+        __syncthreads();
     }
-    __device__ __forceinline__ void angles(const NormRopeParams& p, int row, float* s, float* c) const {
+    // a lane's part of its head in a pass, or -1
+    __device__ __forceinline__ int head(int pass) const {
+        const int h = (pass < query_passes ? pass : pass - query_passes) * per_warp + slot;
+        return active && h < (pass < query_passes ? p.heads : p.kv_heads) ? h : -1;
+    }
+    // every pair once in the warp, and from there to the lanes of all heads
+    __device__ __forceinline__ void turn(int row) const {
         const int b = row / p.time;
         const long long position = p.offset + (p.starts ? p.starts[b] : 0) + (row - b * p.time);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int turn = (int)(((unsigned long long)position * turns[i]) >> 32);      // of 2^32
-            sincospif((float)turn * 4.656612873077392578125e-10f, &s[i], &c[i]);         // 2^-31: half turns
+        __syncwarp();                    // the row before is done with them
+        for (int i = threadIdx.x & 31; i < p.dim / 2; i += 32) {
+            const int turns = (int)(((unsigned long long)position * p.turns[i]) >> 32);       // of 2^32
+            float2 v;
+            sincospif((float)turns * 4.656612873077392578125e-10f, &v.y, &v.x);              // 2^-31: half turns
+            angles[i] = v;
         }
+        __syncwarp();
+    }
+    __device__ __forceinline__ void angle(float* c, float* s) const {
+        const float4* from = reinterpret_cast<const float4*>(angles + (active ? 4 * sub : 0));
+        const float4 a = from[0], b = from[1];
+        c[0] = a.x; s[0] = a.y; c[1] = a.z; s[1] = a.w;
+        c[2] = b.x; s[2] = b.y; c[3] = b.z; s[3] = b.w;
+    }
+    __device__ __forceinline__ void weight(int pass, float* w) const {
+        const float4* from = reinterpret_cast<const float4*>(weights + (pass < query_passes ? 0 : p.dim) + (active ? 8 * sub : 0));
+        const float4 a = from[0], b = from[1];
+        w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w;
+        w[4] = b.x; w[5] = b.y; w[6] = b.z; w[7] = b.w;
+    }
+    __device__ __forceinline__ const T* in(int pass, int row, int h) const {
+        return (pass < query_passes ? (const T*)p.q + row * p.q_pitch : (const T*)p.k + row * p.k_pitch) + h * p.dim + 8 * sub;
+    }
+    __device__ __forceinline__ long long dense(int pass, int row, int h) const {
+        return ((long long)row * (pass < query_passes ? p.heads : p.kv_heads) + h) * p.dim + 8 * sub;
     }
 };
 
+// a row's chunk of heads to a warp
 template <typename T>
 __global__ void __launch_bounds__(kThreads)
 norm_rope_kernel(const __grid_constant__ NormRopeParams p) {
     chain_begin();
-    const Lane<T> me(p);
-    const int total = p.heads + p.kv_heads, first = blockIdx.y * p.passes * me.per_warp + me.slot;
-    for (int row = blockIdx.x * kWarps + (threadIdx.x >> 5); row < p.rows; row += gridDim.x * kWarps) {
-        float s[4], c[4];
-        bool have = false;
-        for (int at = 0; at < p.passes; at += kInFlight) {
-            uint4 raw[kInFlight][2];
+    __shared__ __align__(16) float2 s_angles[kWarps][kMaxDim / 2];
+    __shared__ __align__(16) float s_weights[2 * kMaxDim];
+    const Warp<T> me(p, s_angles, s_weights);
+    const int row = blockIdx.x * kWarps + (threadIdx.x >> 5), last = min(p.all_passes, (int)(blockIdx.y + 1) * p.passes);
+    if (row >= p.rows) return;
+    float s[4], c[4];
+    bool turned = false;
+    for (int at = blockIdx.y * p.passes; at < last; at += kInFlight) {
+        uint4 raw[kInFlight][2];
 #pragma unroll
-            for (int u = 0; u < kInFlight; ++u) {
-                const int h = first + (at + u) * me.per_warp;
-                if (me.active && at + u < p.passes && h < total)
-                    load8((h < p.heads ? (const T*)p.q + row * p.q_pitch + h * p.dim : (const T*)p.k + row * p.k_pitch + (h - p.heads) * p.dim) + 8 * me.sub,
-                          raw[u]);
-                else
-                    raw[u][0] = raw[u][1] = make_uint4(0, 0, 0, 0);
+        for (int u = 0; u < kInFlight; ++u) {
+            const int h = at + u < last ? me.head(at + u) : -1;
+            if (h >= 0) load8(me.in(at + u, row, h), raw[u]);
+            else raw[u][0] = raw[u][1] = make_uint4(0, 0, 0, 0);
+        }
+        if (!turned) {
+            me.turn(row);
+            me.angle(c, s);
+            turned = true;
+        }
+#pragma unroll
+        for (int u = 0; u < kInFlight; ++u) {
+            if (at + u >= last) break;
+            const int h = me.head(at + u);
+            float x[8], y[8], w[8], square = 0.f;
+            unpack8<T>(raw[u], x);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) square = fmaf(x[i], x[i], square);
+            const float inverse = rsqrtf(head_sum(square, p.lane_bits) * p.one_over_dim + p.eps);
+            me.weight(at + u, w);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float a = x[2 * i] * inverse * w[2 * i], b = x[2 * i + 1] * inverse * w[2 * i + 1];
+                y[2 * i] = a * c[i] - b * s[i];
+                y[2 * i + 1] = a * s[i] + b * c[i];
             }
-            if (!have) {
-                me.angles(p, row, s, c);
-                have = true;
-            }
-#pragma unroll
-            for (int u = 0; u < kInFlight; ++u) {
-                const int h = first + (at + u) * me.per_warp;
-                const bool live = at + u < p.passes && h < total;
-                if (!__any_sync(0xffffffffu, live)) break;
-                float x[8], y[8], square = 0.f;
-                unpack8<T>(raw[u], x);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) square = fmaf(x[i], x[i], square);
-                const float inverse = rsqrtf(head_sum(square, p.lane_bits) / (float)p.dim + p.eps);
-                const bool query = h < p.heads;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float a = x[2 * i] * inverse * (query ? me.wq[2 * i] : me.wk[2 * i]);
-                    const float b = x[2 * i + 1] * inverse * (query ? me.wq[2 * i + 1] : me.wk[2 * i + 1]);
-                    y[2 * i] = a * c[i] - b * s[i];
-                    y[2 * i + 1] = a * s[i] + b * c[i];
-                }
-                if (live && me.active)
-                    store8((query ? (T*)p.q_out + (long long)row * p.heads * p.dim + h * p.dim
-                                  : (T*)p.k_out + (long long)row * p.kv_heads * p.dim + (h - p.heads) * p.dim) + 8 * me.sub, y);
-            }
+            if (h >= 0) store8((T*)(at + u < me.query_passes ? p.q_out : p.k_out) + me.dense(at + u, row, h), y);
         }
     }
 }
 
 // dq, dk, and this block's share of the weights' gradients: partials[block][q | k][dim]
 template <typename T>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, 2)
 norm_rope_backward_kernel(const __grid_constant__ NormRopeParams p) {
     chain_begin();
-    const Lane<T> me(p);
-    const int total = p.heads + p.kv_heads, first = blockIdx.y * p.passes * me.per_warp + me.slot;
+    constexpr int TOGETHER = kInFlight / 2;
+    __shared__ __align__(16) float2 s_angles[kWarps][kMaxDim / 2];
+    __shared__ __align__(16) float s_weights[2 * kMaxDim];
+    __shared__ float s_sum[kWarps][2][kMaxDim];
+    const Warp<T> me(p, s_angles, s_weights);
+    const int first = blockIdx.y * p.passes, last = min(p.all_passes, first + p.passes);
     float dwq[8] = {}, dwk[8] = {};
     for (int row = blockIdx.x * kWarps + (threadIdx.x >> 5); row < p.rows; row += gridDim.x * kWarps) {
         float s[4], c[4];
-        bool have = false;
-        for (int at = 0; at < p.passes; at += kInFlight / 2) {
-            uint4 raw[kInFlight / 2][2], raw_g[kInFlight / 2][2];
+        bool turned = false;
+        for (int at = first; at < last; at += TOGETHER) {
+            uint4 raw[TOGETHER][2], raw_g[TOGETHER][2];
 #pragma unroll
-            for (int u = 0; u < kInFlight / 2; ++u) {
-                const int h = first + (at + u) * me.per_warp;
-                if (me.active && at + u < p.passes && h < total) {
-                    const bool query = h < p.heads;
-                    load8((query ? (const T*)p.q + row * p.q_pitch + h * p.dim : (const T*)p.k + row * p.k_pitch + (h - p.heads) * p.dim) + 8 * me.sub, raw[u]);
-                    load8((query ? (const T*)p.grad_q + (long long)row * p.heads * p.dim + h * p.dim
-                                 : (const T*)p.grad_k + (long long)row * p.kv_heads * p.dim + (h - p.heads) * p.dim) + 8 * me.sub, raw_g[u]);
+            for (int u = 0; u < TOGETHER; ++u) {
+                const int h = at + u < last ? me.head(at + u) : -1;
+                if (h >= 0) {
+                    load8(me.in(at + u, row, h), raw[u]);
+                    load8((const T*)(at + u < me.query_passes ? p.grad_q : p.grad_k) + me.dense(at + u, row, h), raw_g[u]);
                 } else {
                     raw[u][0] = raw[u][1] = raw_g[u][0] = raw_g[u][1] = make_uint4(0, 0, 0, 0);
                 }
             }
-            if (!have) {
-                me.angles(p, row, s, c);
-                have = true;
+            if (!turned) {
+                me.turn(row);
+                me.angle(c, s);
+                turned = true;
             }
 #pragma unroll
-            for (int u = 0; u < kInFlight / 2; ++u) {
-                const int h = first + (at + u) * me.per_warp;
-                const bool live = at + u < p.passes && h < total;
-                if (!__any_sync(0xffffffffu, live)) break;
-                float x[8], g[8], square = 0.f, dot = 0.f;
+            for (int u = 0; u < TOGETHER; ++u) {
+                if (at + u >= last) break;
+                const int h = me.head(at + u);
+                float x[8], g[8], w[8], square = 0.f, dot = 0.f;
                 unpack8<T>(raw[u], x);
                 unpack8<T>(raw_g[u], g);
 #pragma unroll
                 for (int i = 0; i < 8; ++i) square = fmaf(x[i], x[i], square);
-                const float inverse = rsqrtf(head_sum(square, p.lane_bits) / (float)p.dim + p.eps);
-                const bool query = h < p.heads;
+                const float inverse = rsqrtf(head_sum(square, p.lane_bits) * p.one_over_dim + p.eps);
+                me.weight(at + u, w);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {          // turned back
                     const float a = g[2 * i], b = g[2 * i + 1];
@@ -189,23 +214,27 @@ norm_rope_backward_kernel(const __grid_constant__ NormRopeParams p) {
                     g[2 * i + 1] = b * c[i] - a * s[i];
                 }
 #pragma unroll
+                for (int i = 0; i < 8; ++i) x[i] *= inverse;
+                // zero where there is no head
+                if (at + u < me.query_passes) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) dwq[i] = fmaf(g[i], x[i], dwq[i]);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) dwk[i] = fmaf(g[i], x[i], dwk[i]);
+                }
+#pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    x[i] *= inverse;
-                    const float gx = g[i] * x[i];
-                    if (query) dwq[i] += gx; else dwk[i] += gx;      // zero where there is no head
-                    g[i] *= query ? me.wq[i] : me.wk[i];
+                    g[i] *= w[i];
                     dot = fmaf(g[i], x[i], dot);
                 }
-                dot = head_sum(dot, p.lane_bits) / (float)p.dim;
+                dot = head_sum(dot, p.lane_bits) * p.one_over_dim;
 #pragma unroll
                 for (int i = 0; i < 8; ++i) g[i] = inverse * (g[i] - x[i] * dot);
-                if (live && me.active)
-                    store8((query ? (T*)p.q_out + (long long)row * p.heads * p.dim + h * p.dim
-                                  : (T*)p.k_out + (long long)row * p.kv_heads * p.dim + (h - p.heads) * p.dim) + 8 * me.sub, g);
+                if (h >= 0) store8((T*)(at + u < me.query_passes ? p.q_out : p.k_out) + me.dense(at + u, row, h), g);
             }
         }
     }
-    __shared__ float s_sum[kWarps][2][kMaxDim];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
@@ -241,22 +270,25 @@ norm_rope_weights_kernel(const float* __restrict__ partials, float* __restrict__
     if (lane == 0) (column < dim ? dq_weight : dk_weight - dim)[column] = sum;
 }
 
-struct Shape { int lane_bits, passes, chunks, blocks; };
+struct Shape { int lane_bits, all_passes, passes, chunks, blocks; };
 
-// Lanes per head, and how a row's heads are cut into chunks: whole rows to a warp (angles formed once) while the rows alone make
-// eight warps per SM, else shorter chunks down to one head per lane.
-Shape shape_of(long long rows, int heads, int kv_heads, int dim, int warps_per_sm) {
+// Lanes per head, and how a row's passes are cut into chunks: whole rows to a warp (angles formed once) while the rows alone make
+// eight warps per SM, else shorter chunks down to one pass.  `blocks`: of eight rows; for the backward at most two to an SM, which walk the rows
+// and leave one share of the weights' gradients each.
+Shape shape_of(long long rows, int heads, int kv_heads, int dim, bool backward) {
     Shape s = {};
     while ((8 << s.lane_bits) < dim) ++s.lane_bits;
-    const int per_warp = 32 >> s.lane_bits, all = ceil_div(heads + kv_heads, per_warp);
-    s.passes = all;
-    while (s.passes > 1 && rows * ceil_div(all, s.passes) < (long long)sm_count() * 8) s.passes = (s.passes + 1) / 2;
-    s.chunks = ceil_div(all, s.passes);
-    const long long blocks = (rows + kWarps - 1) / kWarps, most = (long long)sm_count() * warps_per_sm / kWarps / s.chunks;
-    s.blocks = (int)(blocks < (most > 1 ? most : 1) ? blocks : (most > 1 ? most : 1));
+    const int per_warp = 32 >> s.lane_bits;
+    s.all_passes = s.passes = ceil_div(heads, per_warp) + ceil_div(kv_heads, per_warp);
+    while (s.passes > 1 && rows * ceil_div(s.all_passes, s.passes) < (long long)sm_count() * 8) s.passes = (s.passes + 1) / 2;
+    s.chunks = ceil_div(s.all_passes, s.passes);
+    s.blocks = ceil_div(rows, kWarps);
+    if (backward) {
+        const int most = 2 * sm_count() / s.chunks > 1 ? 2 * sm_count() / s.chunks : 1;
+        if (s.blocks > most) s.blocks = most;
+    }
     return s;
 }
-constexpr int kForwardWarps = 32, kBackwardWarps = 16;     // per SM
 
 int norm_rope_check(const qmoe_norm_rope_t* a, bool backward) {
     if (!a) return fail_arg("norm_rope: argument is null");
@@ -283,8 +315,8 @@ void norm_rope_params(const qmoe_norm_rope_t* a, const Shape& s, NormRopeParams&
     p.offset = a->offset; p.q_pitch = a->q_pitch; p.k_pitch = a->k_pitch;
     p.rows = (int)(a->batch * a->time); p.time = (int)a->time;
     p.heads = a->heads; p.kv_heads = a->kv_heads; p.dim = a->dim;
-    p.lane_bits = s.lane_bits; p.passes = s.passes;
-    p.eps = (float)a->eps;
+    p.lane_bits = s.lane_bits; p.all_passes = s.all_passes; p.passes = s.passes;
+    p.eps = (float)a->eps; p.one_over_dim = 1.f / a->dim;
     const long double ratio = powl((long double)a->theta, -2.0L / a->dim);
     long double turns = 1.0L / 6.283185307179586476925286766559L;
     for (int i = 0; i < a->dim / 2; ++i, turns *= ratio) {
@@ -303,7 +335,7 @@ extern "C" int qmoe_norm_rope_forward(const qmoe_norm_rope_t* a, uint64_t stream
     if (!a->batch || !a->time) return 0;
     cudaStream_t stream = (cudaStream_t)stream_;
     TimedScope timed(KC_ELEMENTWISE, stream);
-    const Shape s = shape_of(a->batch * a->time, a->heads, a->kv_heads, a->dim, kForwardWarps);
+    const Shape s = shape_of(a->batch * a->time, a->heads, a->kv_heads, a->dim, false);
     NormRopeParams p = {};
     norm_rope_params(a, s, p);
     p.q_out = (void*)a->q_out; p.k_out = (void*)a->k_out;
@@ -316,7 +348,7 @@ extern "C" int qmoe_norm_rope_forward(const qmoe_norm_rope_t* a, uint64_t stream
 
 extern "C" int64_t qmoe_norm_rope_partials(int64_t batch, int64_t time, int32_t heads, int32_t kv_heads, int32_t dim) {
     if (batch <= 0 || time <= 0 || heads <= 0 || kv_heads <= 0 || dim < 8 || dim > kMaxDim) return 1;
-    const Shape s = shape_of(batch * time, heads, kv_heads, dim, kBackwardWarps);
+    const Shape s = shape_of(batch * time, heads, kv_heads, dim, true);
     return (int64_t)s.blocks * s.chunks * 2 * dim;
 }
 
@@ -329,7 +361,7 @@ extern "C" int qmoe_norm_rope_backward(const qmoe_norm_rope_t* a, uint64_t strea
         QMOE_CUDA(cudaMemsetAsync((void*)a->d_k_weight, 0, a->dim * sizeof(float), stream));
         return 0;
     }
-    const Shape s = shape_of(a->batch * a->time, a->heads, a->kv_heads, a->dim, kBackwardWarps);
+    const Shape s = shape_of(a->batch * a->time, a->heads, a->kv_heads, a->dim, true);
     NormRopeParams p = {};
     norm_rope_params(a, s, p);
     p.q_out = (void*)a->dq; p.k_out = (void*)a->dk;
