@@ -97,6 +97,17 @@ inline void chained(void (*kernel)(Parameters...), dim3 grid, dim3 block, size_t
     (void)cudaLaunchKernelEx(&config, kernel, arguments...);
 }
 
+// Dynamic shared memory beyond 48 KB, asked for once per kernel and device (about a microsecond a call).
+template <auto Kernel> inline cudaError_t allow_shared(int bytes) {
+    static int allowed[64] = {};
+    int device = 0;
+    if (cudaError_t code = cudaGetDevice(&device)) return code;
+    if (device < 64 && allowed[device] >= bytes) return cudaSuccess;
+    const cudaError_t code = cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (code == cudaSuccess && device < 64) allowed[device] = bytes;
+    return code;
+}
+
 // ---- small device helpers -------------------------------------------------------------------
 template <typename T> struct Act;
 template <> struct Act<float> {

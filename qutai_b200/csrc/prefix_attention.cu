@@ -9,6 +9,8 @@
 #include "common.cuh"
 #include "attention_ptx.cuh"
 
+#include <type_traits>
+
 namespace qmoe {
 
 int cache_check(const qmoe_cache_t* c);
@@ -845,9 +847,8 @@ int launch_tensor(const PrefixParams& p, const Plan& plan, const qmoe_cache_t* p
     tc.p = p;
     tc.status = device_status_address();
     tc.sequences = (int)sequences;
-    const auto kernel = prefix_tensor_kernel<DIM, INT8, OWN_BY_KEYS>;
-    QMOE_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kShared));
-    chained(kernel, (unsigned)(plan.prefix_items + (plan.together ? plan.own_items : 0)), L::kThreads, L::kShared, stream, tc);
+    QMOE_CUDA((allow_shared<prefix_tensor_kernel<DIM, INT8, OWN_BY_KEYS>>(L::kShared)));
+    chained(prefix_tensor_kernel<DIM, INT8, OWN_BY_KEYS>, (unsigned)(plan.prefix_items + (plan.together ? plan.own_items : 0)), L::kThreads, L::kShared, stream, tc);
     count_tensor_core_launch();
     QMOE_LAUNCH_CHECK("prefix_tensor_kernel");
     return 0;
@@ -861,18 +862,19 @@ int launch(PrefixParams& p, const Plan& plan, const qmoe_cache_t* prefix, cudaSt
         items = plan.together ? 0 : plan.own_items;
         p.prefix_items = 0;
     }
-    auto go = [&](auto kernel) -> int {
+    auto go = [&](auto prefix_by_keys, auto own_by_keys) -> int {
         constexpr int SHARED = Tile<DIM, INT8>::kShared;
-        QMOE_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SHARED));
-        chained(kernel, (unsigned)items, kThreads, SHARED, stream, p);
+        constexpr bool A = decltype(prefix_by_keys)::value, B = decltype(own_by_keys)::value;
+        QMOE_CUDA((allow_shared<prefix_attention_kernel<DIM, INT8, A, B>>(SHARED)));
+        chained(prefix_attention_kernel<DIM, INT8, A, B>, (unsigned)items, kThreads, SHARED, stream, p);
         QMOE_LAUNCH_CHECK("prefix_attention_kernel");
         return 0;
     };
     int rc = 0;
     if (!items) {}
-    else if (plan.own_by_keys && (plan.tensor || plan.prefix_by_keys)) rc = go(prefix_attention_kernel<DIM, INT8, true, true>);
-    else if (plan.own_by_keys) rc = go(prefix_attention_kernel<DIM, INT8, false, true>);
-    else rc = go(prefix_attention_kernel<DIM, INT8, false, false>);
+    else if (plan.own_by_keys && (plan.tensor || plan.prefix_by_keys)) rc = go(std::true_type(), std::true_type());
+    else if (plan.own_by_keys) rc = go(std::false_type(), std::true_type());
+    else rc = go(std::false_type(), std::false_type());
     if (rc || plan.slots == 1) return rc;
     chained(prefix_join_kernel<DIM>, (unsigned)((p.rows + kWarps - 1) / kWarps), kThreads, 0, stream, p);
     QMOE_LAUNCH_CHECK("prefix_join_kernel");

@@ -14,6 +14,8 @@
 #include "common.cuh"
 
 #include <math.h>
+#include <stddef.h>
+#include <string.h>
 
 namespace qmoe {
 namespace {
@@ -317,12 +319,19 @@ void norm_rope_params(const qmoe_norm_rope_t* a, const Shape& s, NormRopeParams&
     p.heads = a->heads; p.kv_heads = a->kv_heads; p.dim = a->dim;
     p.lane_bits = s.lane_bits; p.all_passes = s.all_passes; p.passes = s.passes;
     p.eps = (float)a->eps; p.one_over_dim = 1.f / a->dim;
-    const long double ratio = powl((long double)a->theta, -2.0L / a->dim);
-    long double turns = 1.0L / 6.283185307179586476925286766559L;
-    for (int i = 0; i < a->dim / 2; ++i, turns *= ratio) {
-        const long double fraction = ldexpl(turns - floorl(turns), 64);
-        p.turns[i] = fraction >= 18446744073709551615.0L ? 0ull : (unsigned long long)fraction;
+    // the frequencies depend on theta and the width alone: a program has one of each (1.5 us a call where they are formed every time)
+    static thread_local struct { double theta; int dim; unsigned long long turns[kMaxDim / 2]; } made = {};
+    if (made.theta != a->theta || made.dim != a->dim) {
+        const long double ratio = powl((long double)a->theta, -2.0L / a->dim);
+        long double turns = 1.0L / 6.283185307179586476925286766559L;
+        for (int i = 0; i < a->dim / 2; ++i, turns *= ratio) {
+            const long double fraction = ldexpl(turns - floorl(turns), 64);
+            made.turns[i] = fraction >= 18446744073709551615.0L ? 0ull : (unsigned long long)fraction;
+        }
+        made.theta = a->theta;
+        made.dim = a->dim;
     }
+    memcpy(p.turns, made.turns, a->dim / 2 * sizeof(p.turns[0]));
 }
 
 }  // namespace
@@ -336,7 +345,8 @@ extern "C" int qmoe_norm_rope_forward(const qmoe_norm_rope_t* a, uint64_t stream
     cudaStream_t stream = (cudaStream_t)stream_;
     TimedScope timed(KC_ELEMENTWISE, stream);
     const Shape s = shape_of(a->batch * a->time, a->heads, a->kv_heads, a->dim, false);
-    NormRopeParams p = {};
+    NormRopeParams p;
+    memset(&p, 0, offsetof(NormRopeParams, turns));
     norm_rope_params(a, s, p);
     p.q_out = (void*)a->q_out; p.k_out = (void*)a->k_out;
     const dim3 grid((unsigned)s.blocks, (unsigned)s.chunks);
@@ -362,7 +372,8 @@ extern "C" int qmoe_norm_rope_backward(const qmoe_norm_rope_t* a, uint64_t strea
         return 0;
     }
     const Shape s = shape_of(a->batch * a->time, a->heads, a->kv_heads, a->dim, true);
-    NormRopeParams p = {};
+    NormRopeParams p;
+    memset(&p, 0, offsetof(NormRopeParams, turns));
     norm_rope_params(a, s, p);
     p.q_out = (void*)a->dq; p.k_out = (void*)a->dk;
     p.grad_q = (const void*)a->grad_q; p.grad_k = (const void*)a->grad_k;

@@ -724,7 +724,7 @@ sample_kernel(const __grid_constant__ SampleParams p) {
 template <typename T, bool HELD, int kThreads>
 int launch(const SampleParams& p, int ctas, long long rows, cudaStream_t stream) {
     const size_t shared = (sizeof(Shared<kThreads>) + 15) / 16 * 16 + (HELD ? (size_t)p.slice * sizeof(T) : 0);
-    QMOE_CUDA(cudaFuncSetAttribute(sample_kernel<T, HELD, kThreads>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)shared));
+    QMOE_CUDA((allow_shared<sample_kernel<T, HELD, kThreads>>((int)shared)));
     cudaLaunchAttribute attributes[2] = {chain_attribute(), {}};
     attributes[1].id = cudaLaunchAttributeClusterDimension;
     attributes[1].val.clusterDim.x = ctas;
