@@ -144,22 +144,26 @@ __device__ __forceinline__ void attend(const PrefixParams& p, const Keys& keys, 
 
     const uint32_t base = smem_u32(smem);
     const long long head = ((own ? (long long)b * p.kv_heads : 0) + g) * keys.capacity;
-    auto fetch = [&](int tile) {         // keys begin + 64 tile ..; behind `end` zeros, whatever lies there
-        const uint32_t stage = base + (tile % L::kStages) * L::kStage;
-        const int first = begin + tile * kKeys;
-        constexpr int PIECES = L::kRowBytes / 16;
+    // a thread copies piece `piece` of every TOGETHER-th key of a tile
+    constexpr int PIECES = L::kRowBytes / 16, TOGETHER = kThreads / PIECES;
+    const int mine = threadIdx.x / PIECES, piece = threadIdx.x % PIECES;
+    const long long from = (head + begin + mine) * L::kRowBytes + piece * 16;
+    const uint32_t to = base + mine * L::kPitch + piece * 16;
+    auto fetch = [&](int tile, int slot) {         // keys begin + 64 tile ..; behind `end` zeros, whatever lies there
+        const uint32_t stage = to + slot * L::kStage;
+        const long long at = from + (long long)tile * kKeys * L::kRowBytes;
+        const int left = end - begin - tile * kKeys - mine;
 #pragma unroll
-        for (int i = threadIdx.x; i < kKeys * PIECES; i += kThreads) {
-            const int key = i / PIECES, piece = i % PIECES;
-            const bool there = first + key < end;
-            const long long from = (head + (there ? first + key : 0)) * L::kRowBytes + piece * 16;
-            copy16(stage + key * L::kPitch + piece * 16, keys.k + from, there);
-            copy16(stage + L::kBytes + key * L::kPitch + piece * 16, keys.v + from, there);
+        for (int i = 0; i < kKeys / TOGETHER; ++i) {
+            const bool there = i * TOGETHER < left;
+            const long long src = there ? at + i * TOGETHER * L::kRowBytes : 0;
+            copy16(stage + i * TOGETHER * L::kPitch, keys.k + src, there);
+            copy16(stage + L::kBytes + i * TOGETHER * L::kPitch, keys.v + src, there);
         }
         if (INT8) {
             const int key = threadIdx.x & (kKeys - 1);
-            const bool there = first + key < end, value = threadIdx.x >= kKeys;
-            copy4(stage + 2 * L::kBytes + threadIdx.x * 4, (value ? keys.v_scale : keys.k_scale) + head + (there ? first + key : 0), there);
+            const bool there = begin + tile * kKeys + key < end, value = threadIdx.x >= kKeys;
+            copy4(base + slot * L::kStage + 2 * L::kBytes + threadIdx.x * 4, (value ? keys.v_scale : keys.k_scale) + (there ? head + begin + tile * kKeys + key : 0), there);
         }
     };
 
@@ -170,15 +174,18 @@ __device__ __forceinline__ void attend(const PrefixParams& p, const Keys& keys, 
     const float scale2 = p.scale * LOG2E;
 #pragma unroll
     for (int s = 0; s < L::kStages - 1; ++s) {
-        if (s < tiles) fetch(s);
+        if (s < tiles) fetch(s, s);
         copies_commit();
     }
+    int slot = 0, ahead = L::kStages - 1;          // of tile j, of the one that is fetched
+    // rows quad + 8 of a warp's 16, where there are so many
+    const bool upper = rows - row0 > 8;
     for (int j = 0; j < tiles; ++j) {
         copies_wait<L::kStages - 2>();
         attend_sync();                 // tile j is here, and nobody reads the stage that is filled next
-        if (j + L::kStages - 1 < tiles) fetch(j + L::kStages - 1);
+        if (j + L::kStages - 1 < tiles) fetch(j + L::kStages - 1, ahead);
         copies_commit();
-        const uint32_t k_tile = base + (j % L::kStages) * L::kStage, v_tile = k_tile + L::kBytes, scales = k_tile + 2 * L::kBytes;
+        const uint32_t k_tile = base + slot * L::kStage, v_tile = k_tile + L::kBytes, scales = k_tile + 2 * L::kBytes;
         const int key0 = BY_KEYS ? warp * 16 : 0, first = begin + j * kKeys + key0;
         float s[NT][4];
 #pragma unroll
@@ -211,35 +218,46 @@ __device__ __forceinline__ void attend(const PrefixParams& p, const Keys& keys, 
                 for (int i = 0; i < 4; ++i)
                     if (first + 8 * n + 2 * t4 + (i & 1) >= limit[i >> 1]) s[n][i] = -INFINITY;
         }
-        float alpha[2], base2[2];
+        if (++slot == L::kStages) slot = 0;
+        if (++ahead == L::kStages) ahead = 0;
+        float alpha[2] = {1.f, 1.f}, from2[2];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
+            if (i && !upper) break;
             float peak = -INFINITY;
 #pragma unroll
             for (int n = 0; n < NT; ++n) peak = fmaxf(peak, fmaxf(s[n][2 * i], s[n][2 * i + 1]));
             peak = fmaxf(peak, __shfl_xor_sync(0xffffffffu, peak, 1));
             peak = fmaxf(peak, __shfl_xor_sync(0xffffffffu, peak, 2));
-            const float next = fmaxf(m[i], peak);
-            base2[i] = next == -INFINITY ? 0.f : next;        // a row that has seen nothing yet
-            alpha[i] = exp2_fast((m[i] - base2[i]) * scale2);
-            m[i] = next;
-            l[i] *= alpha[i];
+            // the base of the exponentials follows the maximum only when it is 2^8 behind (see prefix_tensor_kernel)
+            if (peak * scale2 > m[i] + 8.f) {
+                alpha[i] = exp2_fast(m[i] - peak * scale2);
+                m[i] = peak * scale2;
+                l[i] *= alpha[i];
+            }
+            from2[i] = m[i] == -INFINITY ? 0.f : m[i];       // a row that has seen nothing yet
         }
+        if (__any_sync(0xffffffffu, alpha[0] != 1.f || alpha[1] != 1.f)) {
 #pragma unroll
-        for (int c = 0; c < COLS; ++c) {
-            o[c][0] *= alpha[0]; o[c][1] *= alpha[0];
-            o[c][2] *= alpha[1]; o[c][3] *= alpha[1];
+            for (int c = 0; c < COLS; ++c) {
+                o[c][0] *= alpha[0]; o[c][1] *= alpha[0];
+                o[c][2] *= alpha[1]; o[c][3] *= alpha[1];
+            }
         }
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
+            float2 vs = make_float2(1.f, 1.f);
+            if constexpr (INT8) vs = load_shared_f2(scales + (kKeys + key0 + 8 * n + 2 * t4) * 4);      // the value's scale goes with its probability
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                s[n][i] = exp2_fast((s[n][i] - base2[i >> 1]) * scale2);
-                l[i >> 1] += s[n][i];
-            }
-            if constexpr (INT8) {        // the value's scale goes with its probability
-                const float2 vs = load_shared_f2(scales + (kKeys + key0 + 8 * n + 2 * t4) * 4);
-                s[n][0] *= vs.x; s[n][1] *= vs.y; s[n][2] *= vs.x; s[n][3] *= vs.y;
+            for (int i = 0; i < 2; ++i) {
+                if (i && !upper) {
+                    s[n][2] = s[n][3] = 0.f;
+                    break;
+                }
+                const float p0 = exp2_fast(fmaf(s[n][2 * i], scale2, -from2[i])), p1 = exp2_fast(fmaf(s[n][2 * i + 1], scale2, -from2[i]));
+                l[i] += p0 + p1;
+                s[n][2 * i] = INT8 ? p0 * vs.x : p0;
+                s[n][2 * i + 1] = INT8 ? p1 * vs.y : p1;
             }
         }
 #pragma unroll
@@ -312,15 +330,15 @@ __device__ __forceinline__ void attend(const PrefixParams& p, const Keys& keys, 
         const float from = top == -INFINITY ? 0.f : top;
 #pragma unroll
         for (int w = 0; w < kWarps; ++w) {
-            factor[w] = exp2_fast((part[(w * 16 + r) * (DIM + 4) + DIM] - from) * scale2);
+            factor[w] = exp2_fast(part[(w * 16 + r) * (DIM + 4) + DIM] - from);
             total += factor[w] * part[(w * 16 + r) * (DIM + 4) + DIM + 1];
         }
         const bool whole = p.slots == 1;
         const long long slot = (long long)(keys.first_slot + split) * p.rows + to;
         const float inverse = total > 0.f ? 1.f / total : 0.f;
         if (piece == 0) {
-            if (whole) p.lse[to] = total > 0.f ? top * p.scale + logf(total) : -INFINITY;
-            else p.part_ml[slot] = make_float2(top * scale2, total);
+            if (whole) p.lse[to] = total > 0.f ? (top + log2f(total)) * LN2 : -INFINITY;
+            else p.part_ml[slot] = make_float2(top, total);
         }
         for (int d = piece * 4; d < DIM; d += 32) {
             float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -339,8 +357,8 @@ __device__ __forceinline__ void attend(const PrefixParams& p, const Keys& keys, 
             const long long slot = (long long)(keys.first_slot + split) * p.rows + at[i];
             const float inverse = l[i] > 0.f ? 1.f / l[i] : 0.f;
             if (t4 == 0) {
-                if (p.slots == 1) p.lse[at[i]] = l[i] > 0.f ? m[i] * p.scale + logf(l[i]) : -INFINITY;
-                else p.part_ml[slot] = make_float2(m[i] * scale2, l[i]);
+                if (p.slots == 1) p.lse[at[i]] = l[i] > 0.f ? (m[i] + log2f(l[i])) * LN2 : -INFINITY;
+                else p.part_ml[slot] = make_float2(m[i], l[i]);
             }
 #pragma unroll
             for (int c = 0; c < COLS; ++c)
@@ -777,7 +795,7 @@ prefix_join_kernel(const __grid_constant__ PrefixParams p) {
 
 struct Plan { Keys prefix, own; int slots; long long prefix_items, own_items; bool tensor, together, prefix_by_keys, own_by_keys; };
 
-// Chunks of keys: as long as they leave three items to an SM, but not below two tiles.
+// Chunks of keys: as long as they leave six items to an SM, but not below two tiles.
 Plan plan_of(const qmoe_prefix_attention_t* a, const qmoe_cache_t* c) {
     Plan plan = {};
     const long long group = a->heads / c->kv_heads, own_rows = a->time * group, all_rows = c->batch * own_rows;
@@ -786,7 +804,7 @@ Plan plan_of(const qmoe_prefix_attention_t* a, const qmoe_cache_t* c) {
     plan.own_by_keys = own_rows <= 16;
     plan.prefix.row_tiles = plan.tensor ? ceil_div(c->batch * a->time, 128 / group) : ceil_div(all_rows, plan.prefix_by_keys ? 16 : 64);
     plan.own.row_tiles = ceil_div(own_rows, plan.own_by_keys ? 16 : 64);
-    const long long prefix_tiles = ceil_div(a->prefix_longest, kKeys), own_tiles = ceil_div(a->longest, kKeys), wanted = (long long)sm_count() * 3;
+    const long long prefix_tiles = ceil_div(a->prefix_longest, kKeys), own_tiles = ceil_div(a->longest, kKeys), wanted = (long long)sm_count() * 6;
     const long long prefix_heads = (long long)plan.prefix.row_tiles * c->kv_heads, own_heads = (long long)plan.own.row_tiles * c->kv_heads * c->batch;
     const long long prefix_mma = plan.tensor ? 0 : prefix_tiles;
     long long chunk = prefix_mma > own_tiles ? prefix_mma : own_tiles;
