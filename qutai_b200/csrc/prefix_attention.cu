@@ -391,16 +391,16 @@ prefix_attention_kernel(const __grid_constant__ PrefixParams p) {
 // The prefix on the tcgen05 tensor cores, for rows that fill their tiles: 128 rows (whole groups of heads of 128 / group sequences) against
 // blocks of 64 keys.  Warp 0 asks TMA for the tiles, warp 1 issues the MMAs, four row warps own a TMEM lane (a row) per thread:
 //     S = Q K^T -> rows: max, exp2, sum, P as two bf16 numbers, put back over the scores -> O += P V, twice, accumulated in tensor memory.
-// The scores of the next blocks go to other buffers meanwhile.  Keys and values of 8 bits come through two more warps, which load them
+// The scores of the next blocks go to other buffers meanwhile.  Keys and values of 8 bits come through warp 0 and two more, which load them
 // and put them into shared memory as bf16, exactly, in the order in which TMA would have; their scales go to the rows, the key's into
 // the score, the value's into the probability.
 // What bounds it: the exponential unit, 512 cycles for a block and SM (the products take 384, 256 of them the two of P V), which two CTAs to
 // an SM share: one's exponentials run beside the other's waits.
 // ------------------------------------------------------------------------------------------------
-constexpr int kTcKeys = 64, kTcColumns = 256, kTcConverters = 2;
+constexpr int kTcKeys = 64, kTcColumns = 256, kTcConverters = 3;
 
 template <int DIM, bool INT8> struct TcTile {
-    static constexpr int kThreads = 192 + (INT8 ? 32 * kTcConverters : 0);
+    static constexpr int kThreads = 192 + (INT8 ? 32 * (kTcConverters - 1) : 0);       // warp 0 is one of them
     static constexpr int kHalves = DIM / 64;                       // a row of 64 elements is the 128 bytes of a swizzle
     static constexpr int kQHalf = 128 * 128, kKeyHalf = kTcKeys * 128;
     static constexpr int kQ = kHalves * kQHalf, kKey = kHalves * kKeyHalf;
@@ -482,13 +482,67 @@ prefix_tensor_kernel(const __grid_constant__ PrefixTcParams tc) {
     const int n = end > begin ? (end - begin + kTcKeys - 1) / kTcKeys : 0;
     const Wait wait{&s_abort, tc.status};
 
-    if (warp == 0) {
-        if (lane == 0 && n) {
-            mbar_expect_tx(bar(Q_FULL), p.group * tc.sequences * DIM * 2);
-            for (int half = 0; half < L::kHalves; ++half) tma_load_3d(&tc.map_q, q_tile + half * L::kQHalf, bar(Q_FULL), half * 64, g * p.group, first_sequence);
+    if (warp == 0 && lane == 0 && n) {
+        mbar_expect_tx(bar(Q_FULL), p.group * tc.sequences * DIM * 2);
+        for (int half = 0; half < L::kHalves; ++half) tma_load_3d(&tc.map_q, q_tile + half * L::kQHalf, bar(Q_FULL), half * 64, g * p.group, first_sequence);
+    }
+    __syncwarp();
+    if (INT8 && (warp == 0 || warp >= 6)) {
+        // pieces of 16 values, a thread's EACH of a tile: piece i of the tile is piece i % PIECES of key i / PIECES
+        constexpr int PIECES = DIM / 16, ALL = kTcKeys * PIECES, EACH = (ALL + 32 * kTcConverters - 1) / (32 * kTcConverters);
+        const int mine = warp ? threadIdx.x - 160 : lane;
+        const long long head = (long long)g * p.prefix.capacity + begin;
+        uint4 k[EACH], v[EACH];
+        float k_scale = 0.f, v_scale = 0.f;
+        auto fetch = [&](int j) {        // behind `end` zeros, whatever lies there
+#pragma unroll
+            for (int i = 0; i < EACH; ++i) {
+                const int at = i * 32 * kTcConverters + mine, key = j * kTcKeys + at / PIECES;
+                const bool there = at < ALL && begin + key < end;
+                const long long from = (head + key) * DIM + at % PIECES * 16;
+                k[i] = there ? *reinterpret_cast<const uint4*>(p.prefix.k + from) : make_uint4(0, 0, 0, 0);
+                v[i] = there ? *reinterpret_cast<const uint4*>(p.prefix.v + from) : make_uint4(0, 0, 0, 0);
+            }
+            const bool there = mine < kTcKeys && begin + j * kTcKeys + mine < end;
+            k_scale = there ? p.prefix.k_scale[head + j * kTcKeys + mine] : 0.f;
+            v_scale = there ? p.prefix.v_scale[head + j * kTcKeys + mine] : 0.f;
+        };
+        if (n) fetch(0);
+        int st = 0;
+        uint32_t parity = 1;
+        bool ok = true;
+        for (int j = 0; ok && j < n; ++j) {
+            auto put = [&](uint32_t to, const uint4* values) {
+#pragma unroll
+                for (int i = 0; i < EACH; ++i) {
+                    const int at = i * 32 * kTcConverters + mine, key = at / PIECES, piece = at % PIECES;
+                    if (at < ALL) store_bytes(to + piece / 4 * L::kKeyHalf + key * 128, piece % 4, key, values[i]);
+                }
+            };
+            ok = wait.all(bar(K_EMPTY + st), parity);
+            if (!ok) break;
+            put(k_tile + st * L::kKey, k);
+            fence_async_shared();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar(K_FULL + st));
+            ok = wait.all(bar(V_EMPTY + st), parity);
+            if (!ok) break;
+            put(v_tile + st * L::kKey, v);
+            if (mine < kTcKeys) {
+                scales[st * 2 * kTcKeys + mine] = k_scale;
+                scales[st * 2 * kTcKeys + kTcKeys + mine] = v_scale;
+            }
+            if (j + 1 < n) fetch(j + 1);
+            fence_async_shared();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar(V_FULL + st));
+            if (++st == L::kStages) { st = 0; parity ^= 1u; }
+        }
+    } else if (warp == 0) {
+        if (lane == 0) {
             int st = 0;
             uint32_t parity = 1;
-            for (int j = 0; !INT8 && j < n && !s_abort; ++j) {
+            for (int j = 0; j < n && !s_abort; ++j) {
                 if (!wait(bar(K_EMPTY + st), parity)) break;
                 mbar_expect_tx(bar(K_FULL + st), L::kKey);
                 for (int half = 0; half < L::kHalves; ++half)
@@ -550,54 +604,6 @@ prefix_tensor_kernel(const __grid_constant__ PrefixTcParams tc) {
         }
         // the last commit has arrived before this CTA's shared memory can go to another one
         if (ok) wait.all(bar(V_EMPTY + (n - 1) % L::kStages), (uint32_t)((n - 1) / L::kStages) & 1u);
-    } else if (INT8 && warp >= 6) {
-        // pieces of 16 values, a thread's EACH of a tile: piece i of the tile is piece i % PIECES of key i / PIECES
-        constexpr int PIECES = DIM / 16, EACH = kTcKeys * PIECES / (32 * kTcConverters);
-        const int mine = threadIdx.x - 192;
-        const long long head = (long long)g * p.prefix.capacity + begin;
-        uint4 k[EACH], v[EACH];
-        float k_scale = 0.f, v_scale = 0.f;
-        auto fetch = [&](int j) {        // behind `end` zeros, whatever lies there
-#pragma unroll
-            for (int i = 0; i < EACH; ++i) {
-                const int at = i * 32 * kTcConverters + mine, key = j * kTcKeys + at / PIECES;
-                const bool there = begin + key < end;
-                const long long from = (head + key) * DIM + at % PIECES * 16;
-                k[i] = there ? *reinterpret_cast<const uint4*>(p.prefix.k + from) : make_uint4(0, 0, 0, 0);
-                v[i] = there ? *reinterpret_cast<const uint4*>(p.prefix.v + from) : make_uint4(0, 0, 0, 0);
-            }
-            const bool there = begin + j * kTcKeys + mine < end;
-            k_scale = there ? p.prefix.k_scale[head + j * kTcKeys + mine] : 0.f;
-            v_scale = there ? p.prefix.v_scale[head + j * kTcKeys + mine] : 0.f;
-        };
-        if (n) fetch(0);
-        bool ok = true;
-        for (int j = 0; ok && j < n; ++j) {
-            const int st = j % L::kStages;
-            const uint32_t parity = (uint32_t)(j / L::kStages) & 1u ^ 1u;
-            auto put = [&](uint32_t to, const uint4* values) {
-#pragma unroll
-                for (int i = 0; i < EACH; ++i) {
-                    const int at = i * 32 * kTcConverters + mine, key = at / PIECES, piece = at % PIECES;
-                    store_bytes(to + piece / 4 * L::kKeyHalf + key * 128, piece % 4, key, values[i]);
-                }
-            };
-            ok = wait.all(bar(K_EMPTY + st), parity);
-            if (!ok) break;
-            put(k_tile + st * L::kKey, k);
-            fence_async_shared();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(bar(K_FULL + st));
-            ok = wait.all(bar(V_EMPTY + st), parity);
-            if (!ok) break;
-            put(v_tile + st * L::kKey, v);
-            scales[st * 2 * kTcKeys + mine] = k_scale;
-            scales[st * 2 * kTcKeys + kTcKeys + mine] = v_scale;
-            if (j + 1 < n) fetch(j + 1);
-            fence_async_shared();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(bar(V_FULL + st));
-        }
     } else {
         const int quad = warp & 3, row = quad * 32 + lane;
         const int sequence = first_sequence + row / p.group;
@@ -720,20 +726,31 @@ prefix_tensor_kernel(const __grid_constant__ PrefixTcParams tc) {
             }
             if (n || whole) {
                 tc_fence_after();
+                // 32 columns at a time through shared memory (the tiles are done with), so that the rows are written in pieces of 128 bytes (64
+                // sequences, 4096 keys: 3300 of a block's 14000 cycles with a row to a thread)
+                constexpr int PITCH = 36;
+                float* const stage = reinterpret_cast<float*>(smem_raw + (k_tile - base)) + quad * 32 * PITCH;
+                const float factor = n ? whole ? inverse : 1.f : 0.f;
 #pragma unroll 1
                 for (int e = 0; e < DIM; e += 32) {
                     uint32_t o[32];
                     tmem_ld32(tmem_o + lane_base + e, o);
                     tmem_ld_wait();
-                    if (!live) continue;
-                    auto value = [&](int c) { return n ? __uint_as_float(o[c]) : 0.f; };
-                    if (whole) {
-                        auto two = [&](int c) { return pack2(value(c) * inverse, value(c + 1) * inverse); };
+                    __syncwarp();
 #pragma unroll
-                        for (int c = 0; c < 32; c += 8) *reinterpret_cast<uint4*>(p.out + at * DIM + e + c) = make_uint4(two(c), two(c + 2), two(c + 4), two(c + 6));
-                    } else {
+                    for (int c = 0; c < 32; c += 4) {
+                        auto value = [&](int i) { return n ? __uint_as_float(o[c + i]) * factor : 0.f; };
+                        *reinterpret_cast<float4*>(stage + lane * PITCH + c) = make_float4(value(0), value(1), value(2), value(3));
+                    }
+                    __syncwarp();
 #pragma unroll
-                        for (int c = 0; c < 32; c += 4) *reinterpret_cast<float4*>(p.part_o + slot * DIM + e + c) = make_float4(value(c), value(c + 1), value(c + 2), value(c + 3));
+                    for (int i = 0; i < 8; ++i) {
+                        const int r = i * 4 + lane / 8;
+                        const float4 v = *reinterpret_cast<const float4*>(stage + r * PITCH + lane % 8 * 4);
+                        const long long to = __shfl_sync(0xffffffffu, live ? at : -1, r);
+                        if (to < 0) continue;
+                        if (whole) *reinterpret_cast<uint2*>(p.out + to * DIM + e + lane % 8 * 4) = make_uint2(pack2(v.x, v.y), pack2(v.z, v.w));
+                        else *reinterpret_cast<float4*>(p.part_o + ((long long)(p.prefix.first_slot + split) * p.rows + to) * DIM + e + lane % 8 * 4) = v;
                     }
                 }
             }
