@@ -550,7 +550,7 @@ int64_t qmoe_norm_rope_partials(int64_t batch, int64_t time, int32_t heads, int3
 int qmoe_norm_rope_backward(const qmoe_norm_rope_t* norm_rope, uint64_t stream);
 
 /* ---------------------------------------------------------------------------------------------
- * A key/value cache for decoding, and attention over it (upstream decodes without one: every token runs the whole sequence again).
+ * A key/value cache for decoding, and attention over it (no upstream counterpart).
  * Keys and values lie [batch, kv_heads, capacity, dim], so that a head's positions are contiguous; sequence b holds lengths[b] of them.  In a
  * QMOE_INT8 cache the `dim` values of a head and position are whole multiples, -127 .. 127, of a scale of their own,
  * max |x| / 127 in f32; a value is the whole number times the scale.
@@ -592,7 +592,7 @@ int64_t qmoe_prefix_attention_scratch(const qmoe_prefix_attention_t* attention, 
 int qmoe_prefix_attention(const qmoe_prefix_attention_t* attention, const qmoe_cache_t* cache, const qmoe_cache_t* prefix, uint64_t stream);
 
 /* ---------------------------------------------------------------------------------------------
- * One token a row from given uniform numbers (no upstream counterpart on the device).  The weight of a token is
+ * One token a row from given uniform numbers (no upstream counterpart).  The weight of a token is
  * exp((logit - largest) / temperature), held as a whole number of 2^-31 (a weight below 2^-32 of the largest is none), so that sums
  * do not depend on their order.  Kept are the top_k largest logits (0 or at least vocab: all; of equal ones those of lower
  * index), of these the shortest run from the largest that holds top_p of their weight, of these the ones of at least

@@ -26,6 +26,7 @@ from .attention import attention_backward, attention_forward
 from .expert_parallel import ExpertParallelMoE
 from .head import LMHead
 from .layers import MoEFeedForward, RMSNorm, SparseMoE, Tensor
+from .rotary import norm_rope_backward, norm_rope_forward
 from .storage import DeviceStorage
 
 
@@ -44,6 +45,7 @@ class Config:
     rope_theta: float = 10000.0
     aux_loss_coef: float = 0.01
     ffn_type: str = "moe"
+    qk_norm: bool = False       # not upstream's: every query and key head normalised (``qutai_b200.rotary``) before its rotation
 
 
 def _accumulate(parameter, storage, stream):
@@ -134,7 +136,8 @@ def _add(a, b, stream):
 
 
 class GQA:
-    """Grouped-query attention with rotary embedding (src/qutai/lm/layers.py:316-349)."""
+    """Grouped-query attention with rotary embedding (src/qutai/lm/layers.py:316-349); with ``config.qk_norm`` the heads of q and k are
+    normalised, each with a weight of its own, in the pass that rotates them."""
 
     def __init__(self, config, *, seed, stream=0):
         width = config.d_model
@@ -146,35 +149,61 @@ class GQA:
         self.k = Linear(width, kv_width, std=0.02, seed=s(1), stream=stream)
         self.v = Linear(width, kv_width, std=0.02, seed=s(2), stream=stream)
         self.out = Linear(width, width, std=0.02 / sqrt(2 * config.n_layers), seed=s(3), stream=stream)
+        self.q_norm = self.k_norm = None
+        if getattr(config, "qk_norm", False):
+            self.q_norm, self.k_norm = (RMSNorm(self.dim, config.norm_eps, stream=stream) for _ in range(2))
         self.width, self.kv_width, self.stream = width, kv_width, stream
 
     def parameters(self):
-        return tuple(p for layer in (self.q, self.k, self.v, self.out) for p in layer.parameters())
+        return tuple(parameter for _, parameter in self.named_weights())
 
-    def _rope(self, values, batch, time, heads, inverse):
+    def named_weights(self):
+        """``(name, weight)`` in the order of ``Decoder.named_parameters``."""
+        names = ("q", "k", "v", "out") + (("q_norm", "k_norm") if self.q_norm is not None else ())
+        return [(name, getattr(self, name).weight) for name in names]
+
+    def _rope(self, values, batch, time, heads, inverse, offset=0):
         out = DeviceStorage(values.size, "bfloat16")
-        lib.call("qmoe_rope", values.ptr, out.ptr, lib.QMOE_BF16, batch, time, heads, self.dim, float(self.theta), 0, 1 if inverse else 0,
+        lib.call("qmoe_rope", values.ptr, out.ptr, lib.QMOE_BF16, batch, time, heads, self.dim, float(self.theta), offset, 1 if inverse else 0,
                  self.stream)
         return out
 
-    def forward(self, x, batch, time):
+    def _view(self, storage, batch, time, width):
+        return Tensor(storage, (batch, time, width))
+
+    def project(self, x, batch, time, offset=0):
+        """Queries, keys and values of ``batch`` sequences' rows ``x`` at positions ``offset + t``, rotated and, with ``qk_norm``, normalised, as tensors
+        [batch, time, width]; and the projections that came before (``None`` without ``qk_norm``: the rotation's backward needs none)."""
         rows = batch * time
-        view = lambda storage, width: Tensor(storage, (batch, time, width))
-        q = self._rope(self.q.forward(x, rows), batch, time, self.heads, False)
-        k = self._rope(self.k.forward(x, rows), batch, time, self.kv_heads, False)
+        q, k = self.q.forward(x, rows), self.k.forward(x, rows)
+        plain = None
+        if self.q_norm is None:
+            q, k = self._rope(q, batch, time, self.heads, False, offset), self._rope(k, batch, time, self.kv_heads, False, offset)
+        else:
+            plain = self._view(q, batch, time, self.width), self._view(k, batch, time, self.kv_width)
+            q, k = norm_rope_forward(*plain, self.q_norm.weight, self.k_norm.weight, self.heads, self.kv_heads, eps=self.q_norm.eps, theta=self.theta,
+                                     offset=offset, stream=self.stream)
         v = self.v.forward(x, rows)
-        qt, kt, vt = view(q, self.width), view(k, self.kv_width), view(v, self.kv_width)
+        return (self._view(q, batch, time, self.width), self._view(k, batch, time, self.kv_width), self._view(v, batch, time, self.kv_width)), plain
+
+    def forward(self, x, batch, time):
+        (qt, kt, vt), plain = self.project(x, batch, time)
         attended, lse = attention_forward(qt, kt, vt, self.heads, self.kv_heads, self.stream)
-        saved = (x, qt, kt, vt, attended, lse)
-        return self.out.forward(attended, rows), saved
+        return self.out.forward(attended, batch * time), (x, qt, kt, vt, attended, lse, plain)
 
     def backward(self, dy, saved, batch, time):
         rows = batch * time
-        x, qt, kt, vt, attended, lse = saved
+        x, qt, kt, vt, attended, lse, plain = saved
         d_attended = self.out.backward(dy, attended, rows)
         dq, dk, dv = attention_backward(d_attended, qt, kt, vt, attended, lse, self.heads, self.kv_heads, self.stream)
-        dq = self._rope(dq, batch, time, self.heads, True)
-        dk = self._rope(dk, batch, time, self.kv_heads, True)
+        if plain is None:
+            dq = self._rope(dq, batch, time, self.heads, True)
+            dk = self._rope(dk, batch, time, self.kv_heads, True)
+        else:
+            dq, dk, dwq, dwk = norm_rope_backward(dq, dk, *plain, self.q_norm.weight, self.k_norm.weight, self.heads, self.kv_heads,
+                                                  eps=self.q_norm.eps, theta=self.theta, stream=self.stream)
+            _accumulate(self.q_norm.weight, dwq, self.stream)
+            _accumulate(self.k_norm.weight, dwk, self.stream)
         dx = self.q.backward(dq, x, rows)
         dx = _add(dx, self.k.backward(dk, x, rows), self.stream)
         return _add(dx, self.v.backward(dv, x, rows), self.stream)
@@ -273,7 +302,7 @@ class Decoder:
         for i, block in enumerate(self.blocks):
             prefix = f"blocks.{i}."
             result.extend((prefix + name + ".weight", getattr(block, name).weight) for name in ("attn_norm", "ffn_norm"))
-            result.extend((prefix + "attn." + name + ".weight", getattr(block.attn, name).weight) for name in ("q", "k", "v", "out"))
+            result.extend((prefix + "attn." + name + ".weight", weight) for name, weight in block.attn.named_weights())
             result.append((prefix + "ffn.router.weight", block.ffn.router.weight))
             if self.world > 1:
                 result.extend(block.ffn.named_expert_parameters(prefix=prefix + "ffn.experts"))

@@ -2,8 +2,8 @@
 
 ``KVCache`` holds the keys and values of a batch of sequences, in bfloat16 or quantised to 8 bits with a scale for each head and
 position, and each sequence's length on the device.  ``prefix_attention`` lets new queries see a prefix that all
-sequences share (a cache of batch 1, read once for all of them) and what their own sequence holds.  Upstream has no cache: it runs
-the whole sequence again for every token.  Dependency-free: ctypes and the standard library only.
+sequences share (a cache of batch 1, read once for all of them) and what their own sequence holds.  No upstream counterpart.
+Dependency-free: ctypes and the standard library only.
 """
 from __future__ import annotations
 

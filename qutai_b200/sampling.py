@@ -1,8 +1,8 @@
 """Drawing one token a row by temperature, top-k, top-p and min-p from given uniform numbers, over ``qmoe_sample``.
 
 The random numbers are an input, so a run can be repeated, and sums of weights are formed in whole numbers, so the same logits,
-settings and numbers give the same tokens whatever the batch around them.  Upstream samples on the host.  Dependency-free:
-ctypes and the standard library only.
+settings and numbers give the same tokens whatever the batch around them.  No upstream counterpart.  Dependency-free: ctypes and
+the standard library only.
 """
 from __future__ import annotations
 
