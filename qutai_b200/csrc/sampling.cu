@@ -62,7 +62,7 @@ template <int kThreads> struct Shared {
     int ask, ask_bucket;
     int bound;                           // the last bucket that counts
     unsigned members[kMaxCtas];          // of the list, from every CTA, in every CTA
-    u64 least, selected;
+    u64 least, selected, all;
     union {
         struct {
             // this CTA's.  Masses in two halves of 16 bits, for which shared memory has an addition of its own, while 65536 of them
@@ -79,6 +79,9 @@ template <int kThreads> struct Shared {
         };
         u64 table[kTable];               // step 5: sums of warps
     };
+    u64 picked[kThreads];                // first CTA: the members of one bucket of a long list
+    unsigned pickings;
+    int bucket;
     uint32_t count[kBuckets];            // first CTA: the cluster's, of the buckets before
     union {
         u64 mass[kBuckets];
@@ -250,7 +253,7 @@ sample_kernel(const __grid_constant__ SampleParams p) {
     auto exponent = [&](float f) { return exponent_of(f, largest, inverse, odd); };
     // 2
     u64 total = 0, passing = 0;
-    auto weigh = [&](auto any_odd, auto any_min) {
+    auto weigh = [&](auto any_odd, auto any_min) __attribute__((always_inline)) {
         for (int v = threadIdx.x; v < pieces; v += kThreads) {
             float f[N];
             piece(v, f);
@@ -264,7 +267,7 @@ sample_kernel(const __grid_constant__ SampleParams p) {
         }
     };
     // 3: the first CTA; top-k's bound needs no masses' sum and comes along with it
-    auto find_bound = [&]() {
+    auto find_bound = [&]() __attribute__((always_inline)) {
         for (int i = threadIdx.x; i < ctas * kThreads; i += kThreads) {
             const float e = exponent(s.maxima[i]);
             if (!(e > -kLastZ)) continue;
@@ -338,7 +341,7 @@ sample_kernel(const __grid_constant__ SampleParams p) {
         const int bound = s.bound;
         // The members of bucket `only`, or of all up to the bound, to the first CTA's list, if it holds them: counted first, so that everyone
         // knows their place.  Their number.
-        auto enlist = [&](int only) -> unsigned {
+        auto enlist = [&](int only) __attribute__((always_inline)) -> unsigned {
             auto member = [&](float e) {
                 if (!(e > -kLastZ)) return false;
                 const int b = bucket_of(e);
@@ -378,11 +381,92 @@ sample_kernel(const __grid_constant__ SampleParams p) {
             cluster.sync();
             return n;
         };
+        // sums of the buckets before, in place
+        auto accumulate = [&]() __attribute__((always_inline)) {
+            __syncthreads();
+            u64 counts = 0, masses = 0, mass[kPerThread];
+            uint32_t count[kPerThread];
+#pragma unroll
+            for (int i = 0; i < kPerThread; ++i) {
+                counts += count[i] = s.count[threadIdx.x * kPerThread + i];
+                masses += mass[i] = s.mass[threadIdx.x * kPerThread + i];
+            }
+            counts = block_before(counts, s.scratch);
+            masses = block_before(masses, s.scratch);
+#pragma unroll
+            for (int i = 0; i < kPerThread; ++i) {
+                const int b = threadIdx.x * kPerThread + i;
+                s.count[b] = (uint32_t)counts;
+                s.mass[b] = masses;
+                counts += count[i];
+                masses += mass[i];
+            }
+            if (threadIdx.x == kThreads - 1) s.all = masses;
+            __syncthreads();
+        };
         auto weight_at = [&](u64 at) { return expf(exponent(logit_at(at))); };
+        // Of n <= kThreads places in shared memory: kept by count, the number before (and `base` of them ahead of all) below `limit`; by mass, the mass
+        // before 0 or below `threshold`.  s.least: the least place that is kept, all ones for none; s.selected: the kept ones' mass.
+        // Every one is compared with all others, by as many lanes as there are for each.
+        auto compare = [&](const u64* places, unsigned n, bool counts, u64 base, u64 limit, double threshold) __attribute__((always_inline)) {
+            int bits = 0;
+            while (bits < 5 && n << (bits + 1) <= kThreads) ++bits;
+            const unsigned me = threadIdx.x >> bits, of = 1u << bits;
+            const u64 at = me < n ? places[me] : 0;
+            if (threadIdx.x == 0) { s.least = ~0ull; s.selected = 0; }
+            u64 before = 0;
+            for (unsigned j = threadIdx.x & (of - 1); j < n; j += of)
+                if (places[j] > at) before += counts ? 1u : mass_of(weight_at(places[j]));
+            for (unsigned o = 1; o < of; o <<= 1) before += __shfl_xor_sync(0xffffffffu, before, o);
+            before += base;
+            __syncthreads();
+            if (me < n && (threadIdx.x & (of - 1)) == 0 && (counts ? before < limit : before == 0 || (double)before < threshold)) {
+                atomicMin(&s.least, at);
+                atomicAdd(&s.selected, (u64)mass_of(weight_at(at)));
+            }
+            __syncthreads();
+        };
+        // the places of the list that `in` takes, to s.picked; their number, which may be more than fit there
+        auto pick = [&](unsigned n, auto in) __attribute__((always_inline)) -> unsigned {
+            if (threadIdx.x == 0) s.pickings = 0;
+            __syncthreads();
+            for (unsigned i = threadIdx.x; i < n; i += kThreads) {
+                const u64 at = s.list[i];
+                if (!in(at)) continue;
+                const unsigned to = atomicAdd(&s.pickings, 1u);
+                if (to < kThreads) s.picked[to] = at;
+            }
+            __syncthreads();
+            return s.pickings;
+        };
+        // a histogram of the list over `bucket`, then sums of the buckets before
+        auto spread = [&](unsigned n, auto bucket) __attribute__((always_inline)) {
+            for (int b = threadIdx.x; b < kBuckets; b += kThreads) { s.count[b] = 0; s.mass[b] = 0; }
+            __syncthreads();
+            for (unsigned i = threadIdx.x; i < n; i += kThreads) {
+                const u64 at = s.list[i];
+                const int b = bucket(at);
+                if (b < 0) continue;
+                atomicAdd(&s.count[b], 1u);
+                atomicAdd(&s.mass[b], (u64)mass_of(weight_at(at)));
+            }
+            accumulate();
+        };
+        // the last bucket that holds anything and whose sum before `keeps`
+        auto crossing = [&](auto keeps) __attribute__((always_inline)) {
+            if (threadIdx.x == 0) s.bucket = 0;
+            __syncthreads();
+            for (int b = threadIdx.x; b < kBuckets; b += kThreads)
+                if ((b + 1 == kBuckets || s.count[b + 1] != s.count[b]) && keeps(b)) atomicMax(&s.bucket, b);
+            __syncthreads();
+            const int found = s.bucket;
+            __syncthreads();
+            return found;
+        };
         // Of the first CTA's sorted list: kept by count, the number before (and `base` of them ahead of the list) below `limit`; by mass, the mass
         // before 0 or below `threshold`.  The least place that is kept, all ones for none; `selected` becomes the kept members' mass.
         constexpr int EACH = kList / kThreads;
-        auto least_kept = [&](unsigned n, bool counts, u64 base, u64 limit, double threshold) {
+        auto least_kept = [&](unsigned n, bool counts, u64 base, u64 limit, double threshold) __attribute__((always_inline)) {
             if (threadIdx.x == 0) { s.least = ~0ull; s.selected = 0; }
             u64 mass[EACH], sum = 0;
             const unsigned begin = threadIdx.x * EACH;
@@ -447,71 +531,58 @@ sample_kernel(const __grid_constant__ SampleParams p) {
                     if (kept && target >= behind && target < behind + kept) finish((int)(0xffffffffu - (uint32_t)at), logit_at(at));
                     return;
                 }
-                sort_falling<kThreads>(s.list, n);
+                // A longer one: a finer histogram of it, whose crossing bucket's members are compared; or, should even those be many, sorted
+                const float finer = kBuckets * (kBuckets / kLastZ) / (bound + 1);
+                auto fine = [&](u64 at) { return min(kBuckets - 1, (int)(exponent(logit_at(at)) * -finer)); };
                 u64 whole = total;
-                if (by_count) {
-                    least_kept(n, true, 0, (u64)top_k, 0.0);
-                    first = s.least;
-                    whole = s.selected;
-                    __syncthreads();
-                }
-                if (by_mass) {
-                    least_kept(n, false, 0, 0, (double)top_p * (double)whole);
-                    first = max(first, s.least);
-                    __syncthreads();
-                }
-                // the kept ones by index: their places' lower halves fall with it.  A place turned about, upper half for lower
-                for (unsigned i = threadIdx.x; i < n; i += kThreads) {
-                    const u64 at = s.list[i];
-                    s.list[i] = at >= first && !(weight_at(at) < min_p) ? at << 32 | at >> 32 : 0;
-                }
-                sort_falling<kThreads>(s.list, n);
-                u64 sum = 0;
-                uint32_t mass[EACH];
-                const unsigned begin = threadIdx.x * EACH;
-#pragma unroll
-                for (int i = 0; i < EACH; ++i) {
-                    const u64 turned = begin + i < n ? s.list[begin + i] : 0;
-                    sum += mass[i] = turned ? mass_of(weight_at(turned << 32)) : 0u;
-                }
-                u64 before = block_before(sum, s.scratch);
-                if (threadIdx.x == kThreads - 1) s.selected = before + sum;
-                __syncthreads();
-                const u64 target = target_of(s.selected);
-#pragma unroll
-                for (int i = 0; i < EACH; ++i) {
-                    if (target >= before && target < before + mass[i]) {
-                        const u64 turned = s.list[begin + i];
-                        finish((int)(0xffffffffu - (uint32_t)(turned >> 32)), logit_at(turned << 32));
+                bool spread_out = false;
+                auto cut_at = [&](bool counts, u64 limit, double threshold) __attribute__((always_inline)) {
+                    if (!spread_out) spread(n, fine);
+                    spread_out = true;
+                    const int b = crossing([&](int i) {
+                        const u64 before = counts ? (u64)s.count[i] : s.mass[i];
+                        return counts ? before < limit : before == 0 || (double)before < threshold;
+                    });
+                    const unsigned members = pick(n, [&](u64 at) { return fine(at) == b; });
+                    if (members <= kThreads) {
+                        compare(s.picked, members, counts, counts ? (u64)s.count[b] : s.mass[b], limit, threshold);
+                        if (counts) whole = s.mass[b] + s.selected;
+                    } else {
+                        sort_falling<kThreads>(s.list, n);
+                        least_kept(n, counts, 0, limit, threshold);
+                        if (counts) whole = s.selected;
                     }
-                    before += mass[i];
+                    first = max(first, members ? s.least : 0);          // an empty last bucket: all of them
+                    if (counts && !members) whole = total;
+                    __syncthreads();
+                };
+                if (by_count) cut_at(true, (u64)top_k, 0.0);
+                if (by_mass) cut_at(false, 0, (double)top_p * (double)whole);
+                // the kept ones by index: the bucket of indices in which the drawn number lies, and in it the token
+                const unsigned each = (p.vocab + kBuckets - 1) / kBuckets;
+                auto index_of = [&](u64 at) { return 0xffffffffu - (uint32_t)at; };
+                auto kept_at = [&](u64 at) { return at >= first && !(weight_at(at) < min_p); };
+                spread(n, [&](u64 at) { return kept_at(at) ? (int)(index_of(at) / each) : -1; });
+                const u64 target = target_of(s.all);
+                const int b = crossing([&](int i) { return s.mass[i] <= target; });
+                const unsigned members = pick(n, [&](u64 at) { return kept_at(at) && (int)(index_of(at) / each) == b; });
+                // (no more than `each` of them: vocabularies beyond 512 * kBuckets tokens may have to look through the list)
+                const u64* const among = members <= kThreads ? s.picked : s.list;
+                const unsigned many = members <= kThreads ? members : n;
+                for (unsigned i = threadIdx.x; i < many; i += kThreads) {
+                    const u64 at = among[i];
+                    if (!kept_at(at) || (int)(index_of(at) / each) != b) continue;
+                    u64 before = s.mass[b];
+                    for (unsigned j = 0; j < many; ++j) {
+                        const u64 other = among[j];
+                        if (index_of(other) < index_of(at) && kept_at(other) && (int)(index_of(other) / each) == b) before += mass_of(weight_at(other));
+                    }
+                    if (target >= before && target < before + mass_of(weight_at(at))) finish((int)index_of(at), logit_at(at));
                 }
                 return;
             }
         }
         // 4
-        // sums of the buckets before, in place
-        auto accumulate = [&]() {
-            __syncthreads();
-            u64 counts = 0, masses = 0, mass[kPerThread];
-            uint32_t count[kPerThread];
-#pragma unroll
-            for (int i = 0; i < kPerThread; ++i) {
-                counts += count[i] = s.count[threadIdx.x * kPerThread + i];
-                masses += mass[i] = s.mass[threadIdx.x * kPerThread + i];
-            }
-            counts = block_before(counts, s.scratch);
-            masses = block_before(masses, s.scratch);
-#pragma unroll
-            for (int i = 0; i < kPerThread; ++i) {
-                const int b = threadIdx.x * kPerThread + i;
-                s.count[b] = (uint32_t)counts;
-                s.mass[b] = masses;
-                counts += count[i];
-                masses += mass[i];
-            }
-            __syncthreads();
-        };
         __syncthreads();
         for (int b = threadIdx.x; b < kBuckets; b += kThreads) s.own.count[b] = s.own.low[b] = s.own.high[b] = 0;
         __syncthreads();
@@ -545,7 +616,7 @@ sample_kernel(const __grid_constant__ SampleParams p) {
         }
         cluster.sync();
         // The first CTA leads: it asks for a bucket's members, or what lies above a place, until it knows the threshold.
-        auto ask = [&](int what, int bucket, u64 at) {          // by the first CTA; every CTA then answers in `answer`
+        auto ask = [&](int what, int bucket, u64 at) __attribute__((always_inline)) {          // by the first CTA; every CTA then answers in `answer`
             if (threadIdx.x < ctas) {
                 Shared* other = cluster.map_shared_rank(&s, threadIdx.x);
                 other->ask = what;
@@ -554,7 +625,7 @@ sample_kernel(const __grid_constant__ SampleParams p) {
             }
         };
         unsigned listed = 0;
-        auto answer = [&]() {
+        auto answer = [&]() __attribute__((always_inline)) {
             cluster.sync();
             const int what = s.ask;
             if (what == ASK_DONE) return false;
@@ -586,19 +657,9 @@ sample_kernel(const __grid_constant__ SampleParams p) {
             accumulate();
             u64 whole = total;           // of what top-k keeps
             int listed_bucket = -1;
-            auto threshold_of = [&](bool counts, u64 limit, double threshold) -> u64 {
+            auto threshold_of = [&](bool counts, u64 limit, double threshold) __attribute__((always_inline)) -> u64 {
                 auto keeps = [&](u64 before) { return counts ? before < limit : before == 0 || (double)before < threshold; };
-                // the last bucket whose first member is kept
-                if (threadIdx.x == 0) s.bound = 0;
-                __syncthreads();
-                for (int b = threadIdx.x; b < kBuckets; b += kThreads) {
-                    const u64 before = counts ? (u64)s.count[b] : s.mass[b];
-                    const bool empty = b + 1 < kBuckets ? s.count[b + 1] == s.count[b] : false;
-                    if (!empty && keeps(before)) atomicMax(&s.bound, b);
-                }
-                __syncthreads();
-                const int bucket = s.bound;
-                __syncthreads();
+                const int bucket = crossing([&](int b) { return keeps(counts ? (u64)s.count[b] : s.mass[b]); });      // the last whose first member is kept
                 if (bucket != listed_bucket) {
                     ask(ASK_LIST, bucket, 0);
                     answer();
@@ -623,8 +684,13 @@ sample_kernel(const __grid_constant__ SampleParams p) {
                     }
                     return c;
                 }
-                sort_falling<kThreads>(s.list, n);
-                least_kept(n, counts, counts ? (u64)s.count[bucket] : s.mass[bucket], limit, threshold);
+                const u64 base = counts ? (u64)s.count[bucket] : s.mass[bucket];
+                if (n <= kThreads) {
+                    compare(s.list, n, counts, base, limit, threshold);
+                } else {
+                    sort_falling<kThreads>(s.list, n);
+                    least_kept(n, counts, base, limit, threshold);
+                }
                 if (counts) whole = s.mass[bucket] + s.selected;
                 const u64 c = n ? s.least : 0;      // an empty last bucket: everything is kept
                 __syncthreads();
