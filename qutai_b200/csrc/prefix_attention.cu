@@ -18,7 +18,7 @@ int cache_check(const qmoe_cache_t* c);
 namespace {
 
 constexpr int kWarps = 4, kThreads = 32 * kWarps;
-constexpr int kKeys = 64;                // keys of a tile
+constexpr int kKeys = 64;                // what chunks of keys are counted in
 constexpr float LN2 = 0.6931471805599453f;
 
 struct Keys {                            // the prefix, or the sequences' caches
@@ -94,15 +94,21 @@ __device__ __forceinline__ uint32_t bytes_to_bf16(uint32_t w) {
     return r;
 }
 
-template <int DIM, bool INT8> struct Tile {
+// Keys of a tile: 128 where a warp has a quarter of them, so that its steps have some work to overlap (64 sequences, 512 positions: 1450 cycles a
+// tile of 64, in which nothing was waited for but one step for the next)
+template <int DIM, bool INT8, bool BY_KEYS> struct Tile {
+    static constexpr int kKeys = BY_KEYS && DIM == 64 ? 128 : 64;
     static constexpr int kRowBytes = INT8 ? DIM : 2 * DIM;
     static constexpr int kPitch = kRowBytes + 16;                  // 16 more: no two of the rows read together share a bank
     static constexpr int kBytes = kKeys * kPitch;
-    static constexpr int kStages = DIM == 128 && !INT8 ? 2 : 3;    // the wide ones as many as leave room for two blocks on an SM
+    static constexpr int kStages = !INT8 && kKeys * DIM > 64 * 64 ? 2 : 3;         // the large ones as many as leave room for two blocks on an SM
     static constexpr int kStage = 2 * kBytes + (INT8 ? 2 * kKeys * 4 : 0);
     static constexpr int kJoin = kWarps * 16 * (DIM + 4) * 4;      // the warps' parts, where they share the keys
     static constexpr int kShared = kStages * kStage > kJoin ? kStages * kStage : kJoin;
 };
+template <int DIM, bool INT8, bool A, bool B> constexpr int shared_of() {
+    return Tile<DIM, INT8, A>::kShared > Tile<DIM, INT8, B>::kShared ? Tile<DIM, INT8, A>::kShared : Tile<DIM, INT8, B>::kShared;
+}
 
 // Rows of a tile: 16 to a warp (BY_KEYS false: 64 rows, every warp walks all keys) or the same 16 for all warps (BY_KEYS: a
 // quarter of every tile of keys each, joined at the end), for the few rows of one sequence.
@@ -111,21 +117,20 @@ __device__ __forceinline__ void attend_sync() { asm volatile("bar.sync 1, %0;" :
 
 template <int DIM, bool INT8, bool BY_KEYS>
 __device__ __forceinline__ void attend(const PrefixParams& p, const Keys& keys, uint8_t* smem, int b, int g, int row_tile, int split, bool own) {
-    using L = Tile<DIM, INT8>;
-    constexpr int ROWS = BY_KEYS ? 16 : 16 * kWarps, NT = BY_KEYS ? kKeys / 8 / kWarps : kKeys / 8, COLS = DIM / 8;
+    using L = Tile<DIM, INT8, BY_KEYS>;
+    constexpr int KEYS = L::kKeys, ROWS = BY_KEYS ? 16 : 16 * kWarps, NT = BY_KEYS ? KEYS / 8 / kWarps : KEYS / 8, COLS = DIM / 8;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, quad = lane >> 2, t4 = lane & 3;
     const int rows = own ? p.time * p.group : p.batch * p.time * p.group, row0 = row_tile * ROWS + (BY_KEYS ? 0 : 16 * warp);
-    const int length = min(max(keys.lengths[b], 0), keys.longest);
-    const int begin = split * keys.chunk, end = min(length, begin + keys.chunk);
-    // this lane's two rows: where they lie among all rows, and how many keys they see
+    // This lane's two rows: where they lie among all rows, and their queries.  All that can be asked for at once is: the length and the queries, and behind
+    // the length the first tiles, ahead of the queries' first use (under load each takes 1500 cycles; one after the other an item began at 6000).
+    const int held = keys.lengths[b];
     long long at[2];
-    int limit[2];
+    int step[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-        const int m = row0 + quad + 8 * i, step = m / p.group;
-        const bool in = m < rows;
-        at[i] = in ? (((own ? (long long)b * p.time : 0) + step) * p.kv_heads + g) * p.group + (m - step * p.group) : -1;
-        limit[i] = !in ? 0 : own ? min(end, length - p.time + step + 1) : end;
+        const int m = row0 + quad + 8 * i;
+        step[i] = (int)((unsigned)m / (unsigned)p.group);
+        at[i] = m < rows ? (((own ? (long long)b * p.time : 0) + step[i]) * p.kv_heads + g) * p.group + (m - step[i] * p.group) : -1;
     }
     uint32_t qf[DIM / 16][4];
 #pragma unroll
@@ -135,12 +140,19 @@ __device__ __forceinline__ void attend(const PrefixParams& p, const Keys& keys, 
             // a lane's four elements of 16: two and two eight apart as the instruction numbers them; for 8-bit keys they are four
             // neighbours instead (one word of the key), the same permutation of the contraction on both sides
             const __nv_bfloat16* src = p.q + (at[i] < 0 ? 0 : at[i]) * DIM + kk * 16;
-            uint2 v;
-            if (INT8) v = *reinterpret_cast<const uint2*>(src + 4 * t4);
-            else v = make_uint2(*reinterpret_cast<const uint32_t*>(src + 2 * t4), *reinterpret_cast<const uint32_t*>(src + 2 * t4 + 8));
-            qf[kk][i] = at[i] < 0 ? 0u : v.x;
-            qf[kk][2 + i] = at[i] < 0 ? 0u : v.y;
+            uint2 v = make_uint2(0u, 0u);
+            if (at[i] >= 0) {
+                if (INT8) v = *reinterpret_cast<const uint2*>(src + 4 * t4);
+                else v = make_uint2(*reinterpret_cast<const uint32_t*>(src + 2 * t4), *reinterpret_cast<const uint32_t*>(src + 2 * t4 + 8));
+            }
+            qf[kk][i] = v.x;
+            qf[kk][2 + i] = v.y;
         }
+    const int length = min(max(held, 0), keys.longest);
+    const int begin = split * keys.chunk, end = min(length, begin + keys.chunk);
+    int limit[2];                        // keys that the two rows see
+#pragma unroll
+    for (int i = 0; i < 2; ++i) limit[i] = at[i] < 0 ? 0 : own ? min(end, length - p.time + step[i] + 1) : end;
 
     const uint32_t base = smem_u32(smem);
     const long long head = ((own ? (long long)b * p.kv_heads : 0) + g) * keys.capacity;
@@ -149,28 +161,31 @@ __device__ __forceinline__ void attend(const PrefixParams& p, const Keys& keys, 
     const int mine = threadIdx.x / PIECES, piece = threadIdx.x % PIECES;
     const long long from = (head + begin + mine) * L::kRowBytes + piece * 16;
     const uint32_t to = base + mine * L::kPitch + piece * 16;
-    auto fetch = [&](int tile, int slot) {         // keys begin + 64 tile ..; behind `end` zeros, whatever lies there
+    auto fetch = [&](int tile, int slot) {         // keys begin + KEYS tile ..; behind `end` zeros, whatever lies there
         const uint32_t stage = to + slot * L::kStage;
-        const long long at = from + (long long)tile * kKeys * L::kRowBytes;
-        const int left = end - begin - tile * kKeys - mine;
+        const long long at = from + (long long)tile * KEYS * L::kRowBytes;
+        const int left = end - begin - tile * KEYS - mine;
 #pragma unroll
-        for (int i = 0; i < kKeys / TOGETHER; ++i) {
+        for (int i = 0; i < KEYS / TOGETHER; ++i) {
             const bool there = i * TOGETHER < left;
             const long long src = there ? at + i * TOGETHER * L::kRowBytes : 0;
             copy16(stage + i * TOGETHER * L::kPitch, keys.k + src, there);
             copy16(stage + L::kBytes + i * TOGETHER * L::kPitch, keys.v + src, there);
         }
         if (INT8) {
-            const int key = threadIdx.x & (kKeys - 1);
-            const bool there = begin + tile * kKeys + key < end, value = threadIdx.x >= kKeys;
-            copy4(base + slot * L::kStage + 2 * L::kBytes + threadIdx.x * 4, (value ? keys.v_scale : keys.k_scale) + (there ? head + begin + tile * kKeys + key : 0), there);
+#pragma unroll
+            for (int i = threadIdx.x; i < 2 * KEYS; i += kThreads) {
+                const int key = i & (KEYS - 1);
+                const bool there = begin + tile * KEYS + key < end;
+                copy4(base + slot * L::kStage + 2 * L::kBytes + i * 4, (i >= KEYS ? keys.v_scale : keys.k_scale) + (there ? head + begin + tile * KEYS + key : 0), there);
+            }
         }
     };
 
     float o[COLS][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
 #pragma unroll
     for (int c = 0; c < COLS; ++c) o[c][0] = o[c][1] = o[c][2] = o[c][3] = 0.f;
-    const int tiles = end > begin ? (end - begin + kKeys - 1) / kKeys : 0;
+    const int tiles = end > begin ? (end - begin + KEYS - 1) / KEYS : 0;
     const float scale2 = p.scale * LOG2E;
 #pragma unroll
     for (int s = 0; s < L::kStages - 1; ++s) {
@@ -186,7 +201,7 @@ __device__ __forceinline__ void attend(const PrefixParams& p, const Keys& keys, 
         if (j + L::kStages - 1 < tiles) fetch(j + L::kStages - 1, ahead);
         copies_commit();
         const uint32_t k_tile = base + slot * L::kStage, v_tile = k_tile + L::kBytes, scales = k_tile + 2 * L::kBytes;
-        const int key0 = BY_KEYS ? warp * 16 : 0, first = begin + j * kKeys + key0;
+        const int key0 = BY_KEYS ? warp * (KEYS / kWarps) : 0, first = begin + j * KEYS + key0;
         float s[NT][4];
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
@@ -247,7 +262,7 @@ __device__ __forceinline__ void attend(const PrefixParams& p, const Keys& keys, 
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
             float2 vs = make_float2(1.f, 1.f);
-            if constexpr (INT8) vs = load_shared_f2(scales + (kKeys + key0 + 8 * n + 2 * t4) * 4);      // the value's scale goes with its probability
+            if constexpr (INT8) vs = load_shared_f2(scales + (KEYS + key0 + 8 * n + 2 * t4) * 4);      // the value's scale goes with its probability
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
                 if (i && !upper) {
@@ -408,7 +423,7 @@ template <int DIM, bool INT8> struct TcTile {
     static constexpr int kBuffers = DIM == 64 ? 3 : 2;             // of scores: with O all of a CTA's 256 columns
     static constexpr int kTiles = kQ + 2 * kStages * kKey;
     static constexpr int kScales = INT8 ? kStages * 2 * kTcKeys * 4 : 0;
-    static constexpr int kNeeded = kTiles + 256 + kScales, kShared = kNeeded > Tile<DIM, INT8>::kShared ? kNeeded : Tile<DIM, INT8>::kShared;
+    static constexpr int kNeeded = kTiles + 256 + kScales, kShared = kNeeded > shared_of<DIM, INT8, true, false>() ? kNeeded : shared_of<DIM, INT8, true, false>();
 };
 
 struct alignas(64) PrefixTcParams {
@@ -812,7 +827,7 @@ prefix_join_kernel(const __grid_constant__ PrefixParams p) {
 
 struct Plan { Keys prefix, own; int slots; long long prefix_items, own_items; bool tensor, together, prefix_by_keys, own_by_keys; };
 
-// Chunks of keys: as long as they leave six items to an SM, but not below two tiles.
+// Chunks of keys: as long as they leave four items to an SM, but not below two tiles.
 Plan plan_of(const qmoe_prefix_attention_t* a, const qmoe_cache_t* c) {
     Plan plan = {};
     const long long group = a->heads / c->kv_heads, own_rows = a->time * group, all_rows = c->batch * own_rows;
@@ -821,7 +836,7 @@ Plan plan_of(const qmoe_prefix_attention_t* a, const qmoe_cache_t* c) {
     plan.own_by_keys = own_rows <= 16;
     plan.prefix.row_tiles = plan.tensor ? ceil_div(c->batch * a->time, 128 / group) : ceil_div(all_rows, plan.prefix_by_keys ? 16 : 64);
     plan.own.row_tiles = ceil_div(own_rows, plan.own_by_keys ? 16 : 64);
-    const long long prefix_tiles = ceil_div(a->prefix_longest, kKeys), own_tiles = ceil_div(a->longest, kKeys), wanted = (long long)sm_count() * 6;
+    const long long prefix_tiles = ceil_div(a->prefix_longest, kKeys), own_tiles = ceil_div(a->longest, kKeys), wanted = (long long)sm_count() * 4;
     const long long prefix_heads = (long long)plan.prefix.row_tiles * c->kv_heads, own_heads = (long long)plan.own.row_tiles * c->kv_heads * c->batch;
     const long long prefix_mma = plan.tensor ? 0 : prefix_tiles;
     long long chunk = prefix_mma > own_tiles ? prefix_mma : own_tiles;
@@ -898,8 +913,8 @@ int launch(PrefixParams& p, const Plan& plan, const qmoe_cache_t* prefix, cudaSt
         p.prefix_items = 0;
     }
     auto go = [&](auto prefix_by_keys, auto own_by_keys) -> int {
-        constexpr int SHARED = Tile<DIM, INT8>::kShared;
         constexpr bool A = decltype(prefix_by_keys)::value, B = decltype(own_by_keys)::value;
+        constexpr int SHARED = shared_of<DIM, INT8, A, B>();
         QMOE_CUDA((allow_shared<prefix_attention_kernel<DIM, INT8, A, B>>(SHARED)));
         chained(prefix_attention_kernel<DIM, INT8, A, B>, (unsigned)items, kThreads, SHARED, stream, p);
         QMOE_LAUNCH_CHECK("prefix_attention_kernel");
