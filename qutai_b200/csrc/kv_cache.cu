@@ -80,11 +80,12 @@ cache_append_kernel(const __grid_constant__ CacheParams p) {
     const bool in = unit < p.units;      // (the shuffles below need all of a warp's lanes)
     const unsigned row = in ? unit / (unsigned)p.kv_heads : 0, b = row / (unsigned)p.time;
     const int h = in ? (int)(unit - row * p.kv_heads) : 0, t = (int)(row - b * p.time);
-    const long long position = (long long)p.lengths[b] + t;
-    const bool live = in && t < (p.counts ? min(p.counts[b], p.time) : p.time) && position >= 0 && position < p.capacity;
-    const bool active = live && sub * V < p.dim;
+    // the values are read whether they are wanted or not: nothing waits for the lengths but what is written
+    const int held = p.lengths[b], wanted = p.counts ? min(p.counts[b], p.time) : p.time;
     float f[V] = {};
-    if (active) load_values<V>((key ? (const T*)p.k_in + row * p.k_pitch : (const T*)p.v_in + row * p.v_pitch) + h * p.dim + V * sub, f);
+    if (in && sub * V < p.dim) load_values<V>((key ? (const T*)p.k_in + row * p.k_pitch : (const T*)p.v_in + row * p.v_pitch) + h * p.dim + V * sub, f);
+    const long long position = (long long)held + t;
+    const bool active = in && t < wanted && position >= 0 && position < p.capacity && sub * V < p.dim;
     const long long at = ((long long)b * p.kv_heads + h) * p.capacity + position;
     if constexpr (INT8) {
         float most = 0.f;

@@ -286,16 +286,27 @@ norm_rope_backward_kernel(const __grid_constant__ NormRopeParams p) {
     }
 }
 
-// A warp per column of the weights' gradients: its lanes stride over the blocks' shares and meet in a fixed tree
-__global__ void __launch_bounds__(kThreads)
+// 32 columns of the weights' gradients to a block: its 32 warps stride over the blocks' shares, all of a warp's loads in flight together, and meet
+// in a fixed order
+constexpr int kWeightThreads = 1024, kShares = 16;
+__global__ void __launch_bounds__(kWeightThreads)
 norm_rope_weights_kernel(const float* __restrict__ partials, float* __restrict__ dq_weight, float* __restrict__ dk_weight, int blocks, int dim) {
     chain_begin();
-    const int column = blockIdx.x * kWarps + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-    if (column >= 2 * dim) return;
+    __shared__ float s_sum[32][33];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, column = blockIdx.x * 32 + lane;
     float sum = 0.f;
-    for (int b = lane; b < blocks; b += 32) sum += partials[(long long)b * 2 * dim + column];
-    sum = warp_sum(sum);
-    if (lane == 0) (column < dim ? dq_weight : dk_weight - dim)[column] = sum;
+    for (int b = warp; b < blocks; b += 32 * kShares) {
+        float v[kShares];
+#pragma unroll
+        for (int i = 0; i < kShares; ++i) v[i] = b + 32 * i < blocks && column < 2 * dim ? partials[(long long)(b + 32 * i) * 2 * dim + column] : 0.f;
+#pragma unroll
+        for (int i = 0; i < kShares; ++i) sum += v[i];
+    }
+    s_sum[warp][lane] = sum;
+    __syncthreads();
+    sum = warp_sum(s_sum[lane][warp]);               // warp: a column now
+    const int mine = blockIdx.x * 32 + warp;
+    if (lane == 0 && mine < 2 * dim) (mine < dim ? dq_weight : dk_weight - dim)[mine] = sum;
 }
 
 struct Shape { int lane_bits, all_passes, passes, chunks, blocks; };
@@ -417,7 +428,7 @@ extern "C" int qmoe_norm_rope_backward(const qmoe_norm_rope_t* a, uint64_t strea
     const dim3 grid((unsigned)s.blocks, (unsigned)s.chunks);
     launch_by_width(a, [&](auto value, auto bits) { chained(norm_rope_backward_kernel<decltype(value), decltype(bits)::value>, grid, kThreads, 0, stream, p); });
     QMOE_LAUNCH_CHECK("norm_rope_backward_kernel");
-    chained(norm_rope_weights_kernel, (unsigned)ceil_div(2 * a->dim, kWarps), kThreads, 0, stream, (const float*)a->partials, (float*)a->d_q_weight,
+    chained(norm_rope_weights_kernel, (unsigned)ceil_div(2 * a->dim, 32), kWeightThreads, 0, stream, (const float*)a->partials, (float*)a->d_q_weight,
             (float*)a->d_k_weight, s.blocks * s.chunks, a->dim);
     QMOE_LAUNCH_CHECK("norm_rope_weights_kernel");
     return 0;

@@ -110,17 +110,13 @@ def prefix_attention(q, heads, cache, prefix=None, *, out=None, stream=0):
         raise ValueError("q must be [batch, time, heads * dim] with the batch and head width of the cache")
     if q.storage.dtype != "bfloat16":
         raise ValueError("prefix_attention takes bfloat16 queries")
-    a = lib.PrefixAttention()
-    a.time, a.heads, a.longest = q.shape[1], heads, cache.longest
-    shared = None
-    if prefix is not None:
-        a.prefix_longest, shared = prefix.longest, ctypes.byref(prefix._struct)
     rows = cache.batch * q.shape[1] * heads
     result = outputs(out, ((rows * cache.dim, "bfloat16"), (rows, "float32")))
-    a.q, a.out, a.lse = q.storage.ptr, result[0].ptr, result[1].ptr
-    if (a.q | a.out) & 15:
+    q_ptr, out_ptr = q.storage.ptr, result[0].ptr
+    if (q_ptr | out_ptr) & 15:
         raise ValueError("q and the output must be 16-byte aligned")
-    own = ctypes.byref(cache._struct)
+    a = lib.PrefixAttention(q.shape[1], heads, 0, 0 if prefix is None else prefix.longest, cache.longest, q_ptr, out_ptr, result[1].ptr)
+    own, shared = ctypes.byref(cache._struct), None if prefix is None else ctypes.byref(prefix._struct)
     nbytes = lib.load().qmoe_prefix_attention_scratch(ctypes.byref(a), own, shared)
     scratch = DeviceStorage(nbytes // 4, "float32") if nbytes else None
     a.scratch = scratch.ptr if nbytes else 0

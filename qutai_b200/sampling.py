@@ -25,9 +25,7 @@ def sample(logits, uniforms, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, 
         raise ValueError("logits must be float32 or bfloat16")
     if uniforms.dtype != "float32" or uniforms.size != rows:
         raise ValueError("uniforms must hold one float32 number for each row")
-    a = lib.Sample()
-    a.rows, a.vocab, a.dtype, a.logits, a.uniforms = rows, vocab, lib.DTYPE_CODES[logits.storage.dtype], logits.storage.ptr, uniforms.ptr
-    a.temperature = a.top_p = 1.0
+    a = lib.Sample(rows, vocab, lib.DTYPE_CODES[logits.storage.dtype], 0, 1.0, 1.0, 0.0, 0.0, logits.storage.ptr, uniforms.ptr)
     for name, value, dtype in (("temperature", temperature, "float32"), ("top_k", top_k, "int32"), ("top_p", top_p, "float32"), ("min_p", min_p, "float32")):
         if not hasattr(value, "ptr"):
             setattr(a, name, value)

@@ -154,3 +154,86 @@ def test_offsets_beyond_32_bits(dtype):
         view.update({name: getattr(cache, name).view(places, 70) for name in ("k_scale", "v_scale")})
     tail = KVCache(1, 70, kv_heads, dim, dtype, lengths=to_device(np.array([70]), "int32"), longest=70, **view)
     assert np.array_equal(to_host(prefix_attention(Tensor(q, (1, 1, dim)), 1, tail)[0]), want)
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "int8"])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("batch,time,heads,kv_heads,prefix", [(50, 1, 6, 2, 129), (33, 3, 5, 1, 640), (70, 1, 7, 7, 2000), (2, 40, 9, 3, 333), (1, 300, 2, 1, 128), (9, 1, 64, 1, 191),
+                                                              (3, 1, 200, 1, 500), (300, 1, 4, 2, 1024)])
+def test_rows_that_fill_tiles_over_a_prefix(batch, time, heads, kv_heads, prefix, dim, dtype):
+    """Groups of heads that do not divide a tile of rows, new positions in several tiles, prefixes that end in and at blocks of keys."""
+    rng = np.random.default_rng(prefix)
+    check(batch, time, heads, kv_heads, dim, prefix=prefix, lengths=[int(n) for n in rng.integers(0, time + 70, batch)], dtype=dtype, prefix_room=40)
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "int8"])
+@pytest.mark.parametrize("prefix,room", [(200, 0), (150, 800), (0, 700)])
+def test_a_prefix_and_nothing_of_their_own(prefix, room, dtype):
+    """A new cache: the prefix alone, in one part or several, and a prefix that holds nothing where there could be much."""
+    from gpu_util import to_device, to_host
+    from qutai_b200.kv_cache import KVCache, prefix_attention
+    from qutai_b200.layers import Tensor
+
+    rng = np.random.default_rng(prefix)
+    batch, heads, kv_heads, dim = 40, 4, 2, 64
+    shared, held = make(rng, 1, kv_heads, prefix + room, dim, dtype, [prefix], np.nan)
+    q = to_host(to_device(rng.standard_normal((batch, heads, dim)), "bfloat16"), (batch, heads, dim))
+    out, lse = prefix_attention(Tensor(to_device(q, "bfloat16"), (batch, 1, heads * dim)), heads, KVCache(batch, 5, kv_heads, dim, dtype), shared)
+    out, lse = to_host(out, q.shape), to_host(lse, (batch, heads))
+    if not prefix:
+        assert not out.any() and np.all(np.isneginf(lse))
+        return
+    for h in range(heads):
+        k, v = (held[name][0, h // 2, :prefix] for name in "kv")
+        s = q[:, h] @ k.T / 8
+        p = np.exp(s - s.max(-1, keepdims=True))
+        want, size = p @ v / p.sum(-1, keepdims=True), p @ np.abs(v) / p.sum(-1, keepdims=True)
+        assert np.all(np.abs(out[:, h] - want) <= 2.0 ** -9 * 1.05 * (size + np.abs(want)) + 1e-6)
+        assert np.all(np.abs(lse[:, h] - s.max(-1) - np.log(p.sum(-1))) <= 1e-5 * (1 + np.abs(s).max()))
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "int8"])
+def test_scores_that_grow_along_the_prefix(dtype):
+    """The maximum of a row rises by more than 2^8 from block to block: everything summed so far is rescaled each time."""
+    from gpu_util import to_device, to_host
+    from qutai_b200.kv_cache import KVCache, prefix_attention
+    from qutai_b200.layers import Tensor
+
+    rng = np.random.default_rng(3)
+    batch, heads, dim, prefix = 24, 4, 64, 700
+    k = rng.standard_normal((1, prefix, dim)) * 0.3
+    k[..., 0] = np.arange(prefix) * 2.0                 # scores up to 175 apart over the prefix, 16 from block to block
+    v = rng.standard_normal((1, prefix, dim))
+    shared, cache = KVCache(1, prefix, 1, dim, dtype), KVCache(batch, 4, 1, dim, dtype)
+    shared.append(Tensor(to_device(k, "bfloat16"), k.shape), Tensor(to_device(v, "bfloat16"), v.shape))
+    k, v = (to_host(x.storage, (prefix, dim)) for x in shared.read(0, prefix, dtype="float32"))
+    q = rng.standard_normal((batch, heads, dim))
+    q[..., 0] = 1.0
+    q = to_host(to_device(q, "bfloat16"), q.shape)
+    out, lse = prefix_attention(Tensor(to_device(q, "bfloat16"), (batch, 1, heads * dim)), heads, cache, shared)
+    s = q @ k.T / 8
+    p = np.exp(s - s.max(-1, keepdims=True))
+    want, size = p @ v / p.sum(-1, keepdims=True), p @ np.abs(v) / p.sum(-1, keepdims=True)
+    assert np.all(np.abs(to_host(out, q.shape) - want) <= 2.0 ** -9 * 1.05 * (size + np.abs(want)) + 1e-6)
+    assert np.all(np.abs(to_host(lse, (batch, heads)) - s.max(-1) - np.log(p.sum(-1))) <= 1e-5 * (1 + np.abs(s).max()))
+
+
+def test_another_stream_than_the_default_one():
+    import ctypes
+
+    from gpu_util import to_device
+    from qutai_b200 import lib
+    from qutai_b200.kv_cache import prefix_attention
+    from qutai_b200.layers import Tensor
+
+    rng = np.random.default_rng(8)
+    cache, _ = make(rng, 80, 2, 30, 64, "bfloat16", [int(n) for n in rng.integers(0, 31, 80)], np.nan)
+    shared, _ = make(rng, 1, 2, 300, 64, "bfloat16", [300], np.nan)
+    q = Tensor(to_device(rng.standard_normal((80, 1, 256)), "bfloat16"), (80, 1, 256))
+    want = [s.tobytes() for s in prefix_attention(q, 4, cache, shared)]
+    stream = ctypes.c_uint64()
+    lib.call("qmoe_stream_create", ctypes.byref(stream))
+    got = prefix_attention(q, 4, cache, shared, stream=stream.value)
+    lib.call("qmoe_stream_sync", stream.value)
+    assert [s.tobytes() for s in got] == want
+    lib.call("qmoe_stream_destroy", stream.value)

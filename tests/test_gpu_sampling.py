@@ -155,3 +155,14 @@ def test_more_tokens_than_there_are_with_any_weight():
     logits[2:, 1::4] = -200.0
     check(logits, rng.random(4), top_k=2000, top_p=0.9)
     check(logits, rng.random(4), top_k=2000)
+
+
+@pytest.mark.parametrize("top_k", [300, 600, 1500, 2040, 2060, 6000])
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_lists_of_every_length(top_k, dtype):
+    """The candidates in one comparison, in a histogram of their own, in the row's: the same tokens by the same rule."""
+    rng = np.random.default_rng(top_k)
+    logits = rng.standard_normal((6, 20011)) * 2.0
+    logits[3:] = np.round(logits[3:] * 2) / 2           # few levels, every one many times
+    check(logits, rng.random(6), dtype, top_k=top_k)
+    check(logits, rng.random(6), dtype, top_k=top_k, top_p=0.7, temperature=0.9, min_p=0.01)
