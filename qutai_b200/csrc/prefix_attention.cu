@@ -780,34 +780,37 @@ prefix_tensor_kernel(const __grid_constant__ PrefixTcParams tc) {
     }
 }
 
-// A warp per row: the parts' weights, a lane each, then their weighted sum, eight parts' values on their way together
-template <int DIM>
-__global__ void __launch_bounds__(kThreads)
+// The parts of a row: WARPS warps to a row, which take every WARPS-th part, their weights a lane each, eight parts' values on their way together, and
+// meet in shared memory.  One warp to a row, four rows to a block, where that leaves enough warps or there is little to each; else eight: 16 rows in 97
+// parts of 128 values take 26 us with one and 5 with eight, 4096 rows in 10 parts 5 and 12.
+template <int DIM, int WARPS>
+__global__ void __launch_bounds__(WARPS == 1 ? kThreads : 32 * WARPS)
 prefix_join_kernel(const __grid_constant__ PrefixParams p) {
     chain_begin();
-    const long long row = (long long)blockIdx.x * kWarps + (threadIdx.x >> 5);
-    const int lane = threadIdx.x & 31;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, mine = WARPS == 1 ? 0 : warp;
+    const long long row = WARPS == 1 ? (long long)blockIdx.x * kWarps + warp : blockIdx.x;
     if (row >= p.rows) return;
     constexpr int LANES = DIM / 4, TOGETHER = 32 / LANES, DEEP = 8 / TOGETHER;        // lanes of a part's row, parts at a time, such loads in flight
     float top = -INFINITY, total = 0.f;
     float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int first = 0; first < p.slots; first += 32) {
-        const float2 ml = first + lane < p.slots ? p.part_ml[(first + lane) * p.rows + row] : make_float2(-INFINITY, 0.f);
+    for (int first = mine; first < p.slots; first += 32 * WARPS) {
+        const int slot = first + lane * WARPS;
+        const float2 ml = slot < p.slots ? p.part_ml[slot * p.rows + row] : make_float2(-INFINITY, 0.f);
         const float next = fmaxf(top, warp_max(ml.x)), from = next == -INFINITY ? 0.f : next, alpha = exp2_fast(top - from);
         const float factor = ml.y == 0.f ? 0.f : exp2_fast(ml.x - from);             // 0: saw no key, its values were not written
         top = next;
         total = total * alpha + warp_sum(factor * ml.y);
         sum.x *= alpha; sum.y *= alpha; sum.z *= alpha; sum.w *= alpha;
-        const int many = min(32, p.slots - first);
+        const int many = min(32, (p.slots - first + WARPS - 1) / WARPS);
         for (int s = 0; s < many; s += TOGETHER * DEEP) {
             float4 v[DEEP];
             float f[DEEP];
 #pragma unroll
             for (int i = 0; i < DEEP; ++i) {
-                const int slot = s + i * TOGETHER + lane / LANES;
-                f[i] = __shfl_sync(0xffffffffu, factor, slot & 31);
-                if (slot >= many) f[i] = 0.f;
-                v[i] = f[i] != 0.f ? *reinterpret_cast<const float4*>(p.part_o + ((first + slot) * p.rows + row) * DIM + lane % LANES * 4) : make_float4(0.f, 0.f, 0.f, 0.f);
+                const int part = s + i * TOGETHER + lane / LANES;
+                f[i] = __shfl_sync(0xffffffffu, factor, part & 31);
+                if (part >= many) f[i] = 0.f;
+                v[i] = f[i] != 0.f ? *reinterpret_cast<const float4*>(p.part_o + ((first + part * WARPS) * p.rows + row) * DIM + lane % LANES * 4) : make_float4(0.f, 0.f, 0.f, 0.f);
             }
 #pragma unroll
             for (int i = 0; i < DEEP; ++i) { sum.x += f[i] * v[i].x; sum.y += f[i] * v[i].y; sum.z += f[i] * v[i].z; sum.w += f[i] * v[i].w; }
@@ -820,6 +823,25 @@ prefix_join_kernel(const __grid_constant__ PrefixParams p) {
         sum.z += __shfl_xor_sync(0xffffffffu, sum.z, o);
         sum.w += __shfl_xor_sync(0xffffffffu, sum.w, o);
     }
+    if constexpr (WARPS > 1) {
+        __shared__ float2 s_ml[WARPS];
+        __shared__ float4 s_sum[WARPS][LANES];
+        if (lane == 0) s_ml[warp] = make_float2(top, total);
+        if (lane < LANES) s_sum[warp][lane] = sum;
+        __syncthreads();
+        if (warp) return;
+        const float2 ml = lane < WARPS ? s_ml[lane] : make_float2(-INFINITY, 0.f);
+        top = warp_max(ml.x);
+        const float factor = exp2_fast(ml.x - (top == -INFINITY ? 0.f : top));
+        total = warp_sum(factor * ml.y);
+        sum = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) {
+            const float f = __shfl_sync(0xffffffffu, factor, w);
+            const float4 v = s_sum[w][lane % LANES];
+            sum.x += f * v.x; sum.y += f * v.y; sum.z += f * v.z; sum.w += f * v.w;
+        }
+    }
     const float inverse = total > 0.f ? 1.f / total : 0.f;
     if (lane < LANES) *reinterpret_cast<uint2*>(p.out + row * DIM + lane * 4) = make_uint2(pack2(sum.x * inverse, sum.y * inverse), pack2(sum.z * inverse, sum.w * inverse));
     if (lane == 0) p.lse[row] = total > 0.f ? (top + log2f(total)) * LN2 : -INFINITY;
@@ -831,7 +853,11 @@ struct Plan { Keys prefix, own; int slots; long long prefix_items, own_items; bo
 Plan plan_of(const qmoe_prefix_attention_t* a, const qmoe_cache_t* c) {
     Plan plan = {};
     const long long group = a->heads / c->kv_heads, own_rows = a->time * group, all_rows = c->batch * own_rows;
-    plan.tensor = group <= 128 && all_rows > 64 && a->prefix_longest >= 2 * kTcKeys;
+    // Tensor memory's kernel begins 3 us later and takes 128 rows for the price of one: it is ahead from some 8e5 pairs of a query row and a key on with
+    // 64 values to a head, from 4e5 on with 128 (4 heads, without it and with it: 64 rows by 2048 keys 8.4 and 9.9 us, with 128 values 13.6 and 12.4;
+    // 32 by 32768: 25 and 18, 41 and 22; 256 by 8192: 25 and 19, 39 and 24).  Up to 16 rows the other form has every warp at work on keys of its own and
+    // stays ahead (8 heads of int8, 16 rows, 16384 keys: 22 us and 30), as it does for short prefixes (1024 rows of 8 heads by 256 keys: 34 and 40).
+    plan.tensor = group <= 128 && all_rows > 16 && a->prefix_longest >= 512 && all_rows * c->kv_heads * c->dim * a->prefix_longest >= 50000000;
     plan.prefix_by_keys = all_rows <= 16;
     plan.own_by_keys = own_rows <= 16;
     plan.prefix.row_tiles = plan.tensor ? ceil_div(c->batch * a->time, 128 / group) : ceil_div(all_rows, plan.prefix_by_keys ? 16 : 64);
@@ -926,7 +952,8 @@ int launch(PrefixParams& p, const Plan& plan, const qmoe_cache_t* prefix, cudaSt
     else if (plan.own_by_keys) rc = go(std::false_type(), std::true_type());
     else rc = go(std::false_type(), std::false_type());
     if (rc || plan.slots == 1) return rc;
-    chained(prefix_join_kernel<DIM>, (unsigned)((p.rows + kWarps - 1) / kWarps), kThreads, 0, stream, p);
+    if (plan.slots <= 8 || plan.slots * 32 <= p.rows) chained(prefix_join_kernel<DIM, 1>, (unsigned)((p.rows + kWarps - 1) / kWarps), kThreads, 0, stream, p);
+    else chained(prefix_join_kernel<DIM, 8>, (unsigned)p.rows, 256, 0, stream, p);
     QMOE_LAUNCH_CHECK("prefix_join_kernel");
     return 0;
 }

@@ -167,7 +167,25 @@ def test_rows_that_fill_tiles_over_a_prefix(batch, time, heads, kv_heads, prefix
 
 
 @pytest.mark.parametrize("dtype", ["bfloat16", "int8"])
-@pytest.mark.parametrize("prefix,room", [(200, 0), (150, 800), (0, 700)])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("batch,time,heads,kv_heads,prefix,room", [
+    (17, 1, 1, 1, 61700, 0), (4, 1, 32, 4, 8193, 0), (50, 1, 6, 2, 129, 3500), (33, 3, 5, 1, 2200, 0), (70, 1, 7, 7, 2171, 0), (2, 40, 9, 3, 333, 1300), (1, 300, 2, 1, 1800, 0),
+    (9, 1, 64, 1, 128, 1800), (9, 1, 64, 1, 1951, 1), (3, 1, 128, 1, 2816, 0), (3, 1, 200, 1, 500, 2000), (600, 1, 4, 2, 511, 1), (40, 1, 8, 2, 0, 4000), (40, 1, 8, 2, 1, 4000)])
+def test_long_prefixes(batch, time, heads, kv_heads, prefix, room, dim, dtype):
+    """The same where the prefix is long for the number of rows, or could be, by what the host knows of it."""
+    rng = np.random.default_rng(prefix)
+    check(batch, time, heads, kv_heads, dim, prefix=prefix, lengths=[int(n) for n in rng.integers(0, time + 70, batch)], dtype=dtype, prefix_room=room)
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "int8"])
+@pytest.mark.parametrize("garbage", [np.nan, np.inf, 3.0e38])
+def test_what_lies_behind_a_long_prefix_is_not_seen(garbage, dtype):
+    check(40, 1, 8, 2, 128, prefix=700, prefix_room=3300, lengths=[3, 70, 0, 64] * 10, room=70, garbage=garbage, dtype=dtype)
+    check(70, 1, 8, 1, 64, prefix=2300, prefix_room=50, lengths=[30] * 70, room=1, garbage=garbage, dtype=dtype, sharp=60.0)
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "int8"])
+@pytest.mark.parametrize("prefix,room", [(200, 0), (150, 800), (0, 700), (150, 7000), (0, 7000)])
 def test_a_prefix_and_nothing_of_their_own(prefix, room, dtype):
     """A new cache: the prefix alone, in one part or several, and a prefix that holds nothing where there could be much."""
     from gpu_util import to_device, to_host
@@ -193,14 +211,15 @@ def test_a_prefix_and_nothing_of_their_own(prefix, room, dtype):
 
 
 @pytest.mark.parametrize("dtype", ["bfloat16", "int8"])
-def test_scores_that_grow_along_the_prefix(dtype):
+@pytest.mark.parametrize("batch", [24, 400])
+def test_scores_that_grow_along_the_prefix(batch, dtype):
     """The maximum of a row rises by more than 2^8 from block to block: everything summed so far is rescaled each time."""
     from gpu_util import to_device, to_host
     from qutai_b200.kv_cache import KVCache, prefix_attention
     from qutai_b200.layers import Tensor
 
     rng = np.random.default_rng(3)
-    batch, heads, dim, prefix = 24, 4, 64, 700
+    heads, dim, prefix = 4, 64, 700
     k = rng.standard_normal((1, prefix, dim)) * 0.3
     k[..., 0] = np.arange(prefix) * 2.0                 # scores up to 175 apart over the prefix, 16 from block to block
     v = rng.standard_normal((1, prefix, dim))
