@@ -31,10 +31,10 @@ typedef unsigned long long u64;
 constexpr int kMaxCtas = 8;
 constexpr int kBuckets = 1024;
 constexpr int kList = 2048;
-constexpr int kTable = 2048;
+constexpr int kTable = 256;
 constexpr float kOne = 2147483648.f;     // 2^31: the mass of the largest logit's token
 constexpr float kLastZ = 22.25f;         // exp(-z) 2^31 < 1/2 from z = 22.2 on: no mass
-constexpr long long kMaxVocab = 2000000;         // eight slices of at most kTable sums of warps
+constexpr long long kMaxVocab = 2000000;         // eight slices, of which a warp's share has at most kTable sums
 constexpr int kMaxSlice = 160 * 1024;    // bytes of a row's slice in shared memory
 constexpr int kMaxHeld = 65536;          // its elements
 
@@ -61,6 +61,7 @@ template <int kThreads> struct Shared {
     u64 ask_place;                       // what the first CTA asks, in every CTA
     int ask, ask_bucket;
     int bound;                           // the last bucket that counts
+    unsigned staged;                     // members found in this CTA
     unsigned members[kMaxCtas];          // of the list, from every CTA, in every CTA
     u64 least, selected, all;
     union {
@@ -73,11 +74,11 @@ template <int kThreads> struct Shared {
                 u64 mass[kBuckets];
             };
         } own;
-        struct {                         // first CTA, while no histogram is being made: places, and of a short list masses
+        struct {                         // while no histogram is being made: this CTA's members; in the first CTA all of them, and masses of up to kThreads
             u64 list[kList];
             uint32_t list_mass[kThreads];
         };
-        u64 table[kTable];               // step 5: sums of warps
+        u64 table[kTable];               // step 5: sums of warps over one warp's share
     };
     u64 picked[kThreads];                // first CTA: the members of one bucket of a long list
     unsigned pickings;
@@ -188,10 +189,11 @@ sample_kernel(const __grid_constant__ SampleParams p) {
     const long long row = blockIdx.x / ctas;
     cluster.barrier_arrive();            // waited for ahead of the first store to another CTA: by then all of them run
     // the row in pieces of 16 bytes from the 16-byte boundary at or before its start: element i of piece v is token N v + i - lead.  A
-    // thread has the same pieces throughout.
+    // thread has the same pieces throughout, a warp a run of them, so that its sums say where in the row they lie
     const T* const x = (const T*)p.logits + row * p.vocab;
     const int lead = (int)(((uintptr_t)x & 15u) / sizeof(T));
-    const int first_piece = rank * (p.slice / N), pieces = p.slice / N;
+    const int first_piece = rank * (p.slice / N), pieces = p.slice / N, share = (pieces + kWarps - 1) / kWarps;
+    const int begin = warp * share + lane, end = min(pieces, (warp + 1) * share);
     auto token_of = [&](int v, int i) { return (first_piece + v) * N + i - lead; };
     auto inside = [&](int v) { return token_of(v, 0) >= 0 && token_of(v, N) <= p.vocab; };
     auto gather = [&](int v) {           // a piece at the row's ends, or beyond: -infinity where there is no token
@@ -204,9 +206,32 @@ sample_kernel(const __grid_constant__ SampleParams p) {
         if constexpr (HELD) return held[v];
         else return inside(v) ? *reinterpret_cast<const uint4*>(x + token_of(v, 0)) : gather(v);
     };
-    auto piece = [&](int v, float* f) { Vec16<T>::unpack(raw(v), f); };
-    auto add = [&](int b, uint32_t mass) {
-        atomicAdd(&s.own.count[b], 1u);
+    // this thread's pieces in order; of those that come from memory the next two are asked for meanwhile
+    auto each_piece = [&](auto use) __attribute__((always_inline)) {
+        if constexpr (HELD) {
+            for (int v = begin; v < end; v += 32) use(v, held[v]);
+        } else {
+            uint4 next = {}, after = {};
+            if (begin < end) next = raw(begin);
+            if (begin + 32 < end) after = raw(begin + 32);
+            for (int v = begin; v < end; v += 32) {
+                const uint4 now = next;
+                next = after;
+                if (v + 64 < end) after = raw(v + 64);
+                use(v, now);
+            }
+        }
+    };
+    auto each = [&](auto use) __attribute__((always_inline)) {      // the same by element
+        each_piece([&](int v, const uint4& d) __attribute__((always_inline)) {
+            float f[N];
+            Vec16<T>::unpack(d, f);
+#pragma unroll
+            for (int i = 0; i < N; ++i) use(f[i], v, i);
+        });
+    };
+    auto add = [&](int b, uint32_t mass, bool counts) {
+        if (counts) atomicAdd(&s.own.count[b], 1u);
         if constexpr (HELD) {
             atomicAdd(&s.own.low[b], mass & 0xffffu);
             atomicAdd(&s.own.high[b], mass >> 16);
@@ -219,7 +244,7 @@ sample_kernel(const __grid_constant__ SampleParams p) {
         else return of->own.mass[b];
     };
     if constexpr (HELD) {
-        for (int v = threadIdx.x; v < pieces; v += kThreads) {
+        for (int v = begin; v < end; v += 32) {
             if (inside(v)) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(held + v)), "l"(x + token_of(v, 0)) : "memory");
             else held[v] = gather(v);
         }
@@ -238,7 +263,7 @@ sample_kernel(const __grid_constant__ SampleParams p) {
     // 1
     Shared* const first_cta = cluster.map_shared_rank(&s, 0);
     float largest = -INFINITY;
-    for (int v = threadIdx.x; v < pieces; v += kThreads) largest = max_of(raw(v), largest, T());
+    each_piece([&](int, const uint4& d) __attribute__((always_inline)) { largest = max_of(d, largest, T()); });
     cluster.barrier_wait();
     if (by_count || by_mass) first_cta->maxima[rank * kThreads + threadIdx.x] = largest;
     largest = block_max<kThreads>(largest, s.scratch);
@@ -254,17 +279,12 @@ sample_kernel(const __grid_constant__ SampleParams p) {
     // 2
     u64 total = 0, passing = 0;
     auto weigh = [&](auto any_odd, auto any_min) __attribute__((always_inline)) {
-        for (int v = threadIdx.x; v < pieces; v += kThreads) {
-            float f[N];
-            piece(v, f);
-#pragma unroll
-            for (int i = 0; i < N; ++i) {
-                const float weight = expf(exponent_of(f[i], largest, inverse, any_odd.value));
-                const uint32_t mass = mass_of(weight);
-                total += mass;
-                if (any_min.value && !(weight < min_p)) passing += mass;
-            }
-        }
+        each([&](float f, int, int) __attribute__((always_inline)) {
+            const float weight = expf(exponent_of(f, largest, inverse, any_odd.value));
+            const uint32_t mass = mass_of(weight);
+            total += mass;
+            if (any_min.value && !(weight < min_p)) passing += mass;
+        });
     };
     // 3: the first CTA; top-k's bound needs no masses' sum and comes along with it
     auto find_bound = [&]() __attribute__((always_inline)) {
@@ -274,7 +294,7 @@ sample_kernel(const __grid_constant__ SampleParams p) {
             const uint32_t mass = mass_of(expf(e));
             if (!mass) continue;
             if (by_count) atomicAdd(&s.own.count[bucket_of(e)], 1u);
-            else add(bucket_of(e), mass);
+            else add(bucket_of(e), mass, true);
         }
         __syncthreads();
         // a thread's buckets: the first that reaches what is wanted, together with all before
@@ -309,9 +329,8 @@ sample_kernel(const __grid_constant__ SampleParams p) {
     if (odd) weigh(Yes(), Yes());
     else if (min_p > 0.f) weigh(No(), Yes());
     else weigh(No(), No());
-    if (odd || min_p > 0.f) passing = block_sum<kThreads>(passing, s.scratch);
     total = block_sum<kThreads>(total, s.scratch);
-    if (!odd && !(min_p > 0.f)) passing = total;
+    passing = odd || min_p > 0.f ? block_sum<kThreads>(passing, s.scratch) : total;        // its warps' sums stay for step 5
     if (threadIdx.x < ctas) {
         Shared* other = cluster.map_shared_rank(&s, threadIdx.x);
         other->totals[rank] = total;
@@ -339,45 +358,46 @@ sample_kernel(const __grid_constant__ SampleParams p) {
             cluster.sync();
         }
         const int bound = s.bound;
-        // The members of bucket `only`, or of all up to the bound, to the first CTA's list, if it holds them: counted first, so that everyone
-        // knows their place.  Their number.
+        // The members of bucket `only`, or of all up to the bound, to the first CTA's list, if it holds them: to the own one first, from where they
+        // follow those of the CTAs before.  Their number, or one beyond the list's size.
         auto enlist = [&](int only) __attribute__((always_inline)) -> unsigned {
-            auto member = [&](float e) {
-                if (!(e > -kLastZ)) return false;
-                const int b = bucket_of(e);
-                return (only < 0 ? b <= bound : b == only) && mass_of(expf(e)) != 0;
-            };
-            unsigned mine = 0;
-            for (int v = threadIdx.x; v < pieces; v += kThreads) {
+            constexpr float kScale = -kBuckets / kLastZ;
+            const int last = only < 0 ? bound : only;
+            const float from = (float)max(only, 0), to = last + 1 < kBuckets ? (float)(last + 1) : INFINITY;      // bucket_of without its conversion
+            __syncthreads();
+            if (threadIdx.x == 0) s.staged = 0;
+            __syncthreads();
+            bool full = false;
+            each_piece([&](int v, const uint4& d) __attribute__((always_inline)) {
+                if (full) return;
                 float f[N];
-                piece(v, f);
+                Vec16<T>::unpack(d, f);
+                unsigned members = 0;
 #pragma unroll
-                for (int i = 0; i < N; ++i) mine += member(exponent(f[i]));
-            }
-            unsigned to = block_before(mine, s.scratch);
-            if (threadIdx.x == kThreads - 1)
+                for (int i = 0; i < N; ++i) {
+                    const float e = exponent(f[i]), at = e * kScale;
+                    if (e > -kLastZ && at >= from && at < to && (e > -20.f || mass_of(expf(e)) != 0)) members |= 1u << i;
+                }
+                if (!members) return;
+                unsigned where = atomicAdd(&s.staged, (unsigned)__popc(members));
+                full = where + __popc(members) > kList;
+                if (full) return;
 #pragma unroll
-                for (int c = 0; c < kMaxCtas; ++c)
-                    if (c < ctas) cluster.map_shared_rank(&s, c)->members[rank] = to + mine;
+                for (int i = 0; i < N; ++i)
+                    if (members >> i & 1) s.list[where++] = place_of(f[i], token_of(v, i));
+            });
+            __syncthreads();
+            const unsigned mine = s.staged;
+            if (threadIdx.x < ctas) cluster.map_shared_rank(&s, threadIdx.x)->members[rank] = mine;
             cluster.sync();
-            unsigned n = 0;
+            unsigned n = 0, ahead = 0;
 #pragma unroll
             for (int c = 0; c < kMaxCtas; ++c) {
-                if (c == rank) to += n;
+                if (c == rank) ahead = n;
                 if (c < ctas) n += s.members[c];
             }
-            if (n <= kList && mine) {
-                for (int v = threadIdx.x; v < pieces; v += kThreads) {
-                    float f[N];
-                    piece(v, f);
-#pragma unroll
-                    for (int i = 0; i < N; ++i) {
-                        const float e = exponent(f[i]);
-                        if (!member(e)) continue;
-                        first_cta->list[to++] = place_of(f[i], token_of(v, i));
-                    }
-                }
-            }
+            if (n <= kList && rank)
+                for (unsigned i = threadIdx.x; i < mine; i += kThreads) first_cta->list[ahead + i] = s.list[i];
             cluster.sync();
             return n;
         };
@@ -413,16 +433,19 @@ sample_kernel(const __grid_constant__ SampleParams p) {
             while (bits < 5 && n << (bits + 1) <= kThreads) ++bits;
             const unsigned me = threadIdx.x >> bits, of = 1u << bits;
             const u64 at = me < n ? places[me] : 0;
+            const uint32_t mass = me < n ? mass_of(weight_at(at)) : 0u;
+            const bool leads = me < n && (threadIdx.x & (of - 1)) == 0;
             if (threadIdx.x == 0) { s.least = ~0ull; s.selected = 0; }
+            if (leads) s.list_mass[me] = mass;
+            __syncthreads();
             u64 before = 0;
             for (unsigned j = threadIdx.x & (of - 1); j < n; j += of)
-                if (places[j] > at) before += counts ? 1u : mass_of(weight_at(places[j]));
+                if (places[j] > at) before += counts ? 1u : s.list_mass[j];
             for (unsigned o = 1; o < of; o <<= 1) before += __shfl_xor_sync(0xffffffffu, before, o);
             before += base;
-            __syncthreads();
-            if (me < n && (threadIdx.x & (of - 1)) == 0 && (counts ? before < limit : before == 0 || (double)before < threshold)) {
+            if (leads && (counts ? before < limit : before == 0 || (double)before < threshold)) {
                 atomicMin(&s.least, at);
-                atomicAdd(&s.selected, (u64)mass_of(weight_at(at)));
+                atomicAdd(&s.selected, (u64)mass);
             }
             __syncthreads();
         };
@@ -457,7 +480,7 @@ sample_kernel(const __grid_constant__ SampleParams p) {
             if (threadIdx.x == 0) s.bucket = 0;
             __syncthreads();
             for (int b = threadIdx.x; b < kBuckets; b += kThreads)
-                if ((b + 1 == kBuckets || s.count[b + 1] != s.count[b]) && keeps(b)) atomicMax(&s.bucket, b);
+                if ((b + 1 == kBuckets || s.mass[b + 1] != s.mass[b]) && keeps(b)) atomicMax(&s.bucket, b);
             __syncthreads();
             const int found = s.bucket;
             __syncthreads();
@@ -586,19 +609,14 @@ sample_kernel(const __grid_constant__ SampleParams p) {
         __syncthreads();
         for (int b = threadIdx.x; b < kBuckets; b += kThreads) s.own.count[b] = s.own.low[b] = s.own.high[b] = 0;
         __syncthreads();
-        for (int v = threadIdx.x; v < pieces; v += kThreads) {
-            float f[N];
-            piece(v, f);
-#pragma unroll
-            for (int i = 0; i < N; ++i) {
-                const float e = exponent(f[i]);
-                if (!(e > -kLastZ)) continue;
-                const int b = bucket_of(e);
-                if (b > bound) continue;
-                const uint32_t mass = mass_of(expf(e));
-                if (mass) add(b, mass);
-            }
-        }
+        each([&](float f, int, int) __attribute__((always_inline)) {
+            const float e = exponent(f);
+            if (!(e > -kLastZ)) return;
+            const int b = bucket_of(e);
+            if (b > bound) return;
+            const uint32_t mass = mass_of(expf(e));
+            if (mass) add(b, mass, by_count);         // a bucket with members has mass: only top-k needs their number
+        });
         cluster.sync();
         // the cluster's, an equal share of the buckets by every CTA
         for (int b = rank * (kBuckets / ctas) + threadIdx.x; b < (rank + 1) * (kBuckets / ctas); b += kThreads) {
@@ -634,18 +652,13 @@ sample_kernel(const __grid_constant__ SampleParams p) {
             } else {
                 const u64 at = s.ask_place;
                 u64 count = 0, mass = 0;
-                for (int v = threadIdx.x; v < pieces; v += kThreads) {
-                    float f[N];
-                    piece(v, f);
-#pragma unroll
-                    for (int i = 0; i < N; ++i) {
-                        const float e = exponent(f[i]);
-                        if (!(e > -kLastZ) || place_of(f[i], token_of(v, i)) <= at) continue;
-                        const uint32_t m = mass_of(expf(e));
-                        count += m != 0;
-                        mass += m;
-                    }
-                }
+                each([&](float f, int v, int i) __attribute__((always_inline)) {
+                    const float e = exponent(f);
+                    if (!(e > -kLastZ) || place_of(f, token_of(v, i)) <= at) return;
+                    const uint32_t m = mass_of(expf(e));
+                    count += m != 0;
+                    mass += m;
+                });
                 count = block_sum<kThreads>(count, s.scratch);
                 mass = block_sum<kThreads>(mass, s.scratch);
                 if (threadIdx.x == 0) { first_cta->answer_count[rank] = count; first_cta->answer_mass[rank] = mass; }
@@ -706,38 +719,49 @@ sample_kernel(const __grid_constant__ SampleParams p) {
         }
     }
     // 5
-    auto kept_of = [&](float f, int v, int i) -> uint32_t {
+    const float edge = first ? logit_at(first) : -INFINITY;
+    const unsigned edge_token = 0xffffffffu - (uint32_t)first;
+    auto kept_of = [&](float f, int v, int i) __attribute__((always_inline)) -> uint32_t {
         const float e = exponent(f);
-        if (!(e > -kLastZ) || place_of(f, token_of(v, i)) < first) return 0u;
+        if (!(f >= edge) || !(e > -kLastZ) || (f == edge && (unsigned)token_of(v, i) > edge_token)) return 0u;
         const float weight = expf(e);
         return weight < min_p ? 0u : mass_of(weight);
     };
     u64 sum = 0, before = 0, all = 0;
-    if (first) {
-        for (int v = threadIdx.x; v < pieces; v += kThreads) {
-            float f[N];
-            piece(v, f);
-#pragma unroll
-            for (int i = 0; i < N; ++i) sum += kept_of(f[i], v, i);
-        }
+    if (cut || one) {
+        each([&](float f, int v, int i) __attribute__((always_inline)) { sum += kept_of(f, v, i); });
         sum = block_sum<kThreads>(sum, s.scratch);
         if (threadIdx.x < ctas) cluster.map_shared_rank(&s, threadIdx.x)->kept[rank] = sum;
         cluster.sync();
     }
     for (int c = 0; c < ctas; ++c) {
-        const u64 share = first ? s.kept[c] : s.passing[c];
-        if (c == rank) { before = all; sum = share; }
-        all += share;
+        const u64 of_cta = cut || one ? s.kept[c] : s.passing[c];
+        if (c == rank) { before = all; sum = of_cta; }
+        all += of_cta;
     }
     const u64 target = target_of(all);
     if (target < before || target >= before + sum) return;          // another CTA's
-    const int rounds = (pieces + kThreads - 1) / kThreads;
+    // the warp in whose share it lies, by the warps' sums; all warps look through that share
+    int from, until;
+    {
+        u64 of_warp = lane < kWarps ? s.scratch[lane] : 0, upto = of_warp;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const u64 other = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += other;
+        }
+        const int which = __ffs(__ballot_sync(0xffffffffu, before + upto > target)) - 1;
+        before += __shfl_sync(0xffffffffu, upto - of_warp, which);
+        from = which * share;
+        until = min(pieces, from + share);
+    }
+    const int rounds = (until - from + kThreads - 1) / kThreads;
     for (int r = 0; r < rounds; ++r) {
-        const int v = r * kThreads + threadIdx.x;
+        const int v = from + r * kThreads + threadIdx.x;
         u64 mine = 0;
-        if (v < pieces) {
+        if (v < until) {
             float f[N];
-            piece(v, f);
+            Vec16<T>::unpack(raw(v), f);
 #pragma unroll
             for (int i = 0; i < N; ++i) mine += kept_of(f[i], v, i);
         }
@@ -746,7 +770,7 @@ sample_kernel(const __grid_constant__ SampleParams p) {
     }
     __syncthreads();
     if (warp) return;
-    // the warp's share of the table: 32 sums at a time
+    // 32 sums of the table at a time
     for (int at = 0; at < rounds * kWarps; at += 32) {
         const u64 mine = at + lane < rounds * kWarps ? s.table[at + lane] : 0;
         u64 upto = mine;
@@ -762,13 +786,13 @@ sample_kernel(const __grid_constant__ SampleParams p) {
         }
         const int which = __ffs(hit) - 1;
         before += __shfl_sync(0xffffffffu, upto - mine, which);
-        const int entry = at + which, v = entry / kWarps * kThreads + entry % kWarps * 32 + lane;
+        const int entry = at + which, v = from + entry / kWarps * kThreads + entry % kWarps * 32 + lane;
         float f[N];
         uint32_t masses[N];
         u64 lane_sum = 0;
-        if (v < pieces) piece(v, f);
+        if (v < until) Vec16<T>::unpack(raw(v), f);
 #pragma unroll
-        for (int i = 0; i < N; ++i) lane_sum += masses[i] = v < pieces ? kept_of(f[i], v, i) : 0u;
+        for (int i = 0; i < N; ++i) lane_sum += masses[i] = v < until ? kept_of(f[i], v, i) : 0u;
         u64 running = lane_sum;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
