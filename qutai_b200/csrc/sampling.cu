@@ -86,6 +86,7 @@ template <int kThreads> struct Shared {
     uint32_t count[kBuckets];            // first CTA: the cluster's, of the buckets before
     union {
         u64 mass[kBuckets];
+        struct { uint32_t low[kBuckets], high[kBuckets]; };      // the masses' halves while they are added up
         float maxima[kMaxCtas * kThreads];       // first CTA: of every thread
     };
 };
@@ -367,6 +368,7 @@ sample_kernel(const __grid_constant__ SampleParams p) {
             __syncthreads();
             if (threadIdx.x == 0) s.staged = 0;
             __syncthreads();
+            const bool thin = to > kScale * -20.f;       // weights that may have no mass
             bool full = false;
             each_piece([&](int v, const uint4& d) __attribute__((always_inline)) {
                 if (full) return;
@@ -376,8 +378,12 @@ sample_kernel(const __grid_constant__ SampleParams p) {
 #pragma unroll
                 for (int i = 0; i < N; ++i) {
                     const float e = exponent(f[i]), at = e * kScale;
-                    if (e > -kLastZ && at >= from && at < to && (e > -20.f || mass_of(expf(e)) != 0)) members |= 1u << i;
+                    if (e > -kLastZ && at >= from && at < to) members |= 1u << i;
                 }
+                if (thin)
+#pragma unroll
+                    for (int i = 0; i < N; ++i)
+                        if (members >> i & 1 && mass_of(expf(exponent(f[i]))) == 0) members ^= 1u << i;
                 if (!members) return;
                 unsigned where = atomicAdd(&s.staged, (unsigned)__popc(members));
                 full = where + __popc(members) > kList;
@@ -427,25 +433,47 @@ sample_kernel(const __grid_constant__ SampleParams p) {
         auto weight_at = [&](u64 at) { return expf(exponent(logit_at(at))); };
         // Of n <= kThreads places in shared memory: kept by count, the number before (and `base` of them ahead of all) below `limit`; by mass, the mass
         // before 0 or below `threshold`.  s.least: the least place that is kept, all ones for none; s.selected: the kept ones' mass.
-        // Every one is compared with all others, by as many lanes as there are for each.
-        auto compare = [&](const u64* places, unsigned n, bool counts, u64 base, u64 limit, double threshold) __attribute__((always_inline)) {
-            int bits = 0;
-            while (bits < 5 && n << (bits + 1) <= kThreads) ++bits;
-            const unsigned me = threadIdx.x >> bits, of = 1u << bits;
-            const u64 at = me < n ? places[me] : 0;
-            const uint32_t mass = me < n ? mass_of(weight_at(at)) : 0u;
-            const bool leads = me < n && (threadIdx.x & (of - 1)) == 0;
+        // Few are compared with all others, by as many lanes as there are for each, more are sorted (512 rows of 131071 bfloat16 logits, some 200 of them equal ones: 671 and 549 us).
+        auto compare = [&](u64* places, unsigned n, bool counts, u64 base, u64 limit, double threshold) __attribute__((always_inline)) {
+            u64 at, mass_ahead = 0;
+            uint32_t mass;
+            unsigned ahead = 0;
+            bool leads;
             if (threadIdx.x == 0) { s.least = ~0ull; s.selected = 0; }
-            if (leads) s.list_mass[me] = mass;
-            __syncthreads();
-            u64 before = 0;
-            for (unsigned j = threadIdx.x & (of - 1); j < n; j += of)
-                if (places[j] > at) before += counts ? 1u : s.list_mass[j];
-            for (unsigned o = 1; o < of; o <<= 1) before += __shfl_xor_sync(0xffffffffu, before, o);
-            before += base;
-            if (leads && (counts ? before < limit : before == 0 || (double)before < threshold)) {
-                atomicMin(&s.least, at);
-                atomicAdd(&s.selected, (u64)mass);
+            if (n > kThreads / 4) {
+                sort_falling<kThreads>(places, n);
+                ahead = threadIdx.x;
+                leads = ahead < n;
+                at = leads ? places[ahead] : 0;
+                mass = leads ? mass_of(weight_at(at)) : 0u;
+                mass_ahead = block_before((u64)mass, s.scratch);
+            } else {
+                int bits = 0;
+                while (bits < 5 && n << (bits + 1) <= kThreads) ++bits;
+                const unsigned me = threadIdx.x >> bits, of = 1u << bits;
+                at = me < n ? places[me] : 0;
+                mass = me < n ? mass_of(weight_at(at)) : 0u;
+                leads = me < n && (threadIdx.x & (of - 1)) == 0;
+                if (leads) s.list_mass[me] = mass;
+                __syncthreads();
+                for (unsigned j = threadIdx.x & (of - 1); j < n; j += of)
+                    if (places[j] > at) {
+                        ++ahead;
+                        mass_ahead += s.list_mass[j];
+                    }
+                for (unsigned o = 1; o < of; o <<= 1) {
+                    ahead += __shfl_xor_sync(0xffffffffu, ahead, o);
+                    mass_ahead += __shfl_xor_sync(0xffffffffu, mass_ahead, o);
+                }
+            }
+            // the kept ones are a run from the highest: the last of them, by which no other follows that is kept, is the one to know
+            auto keeps = [&](u64 number, u64 mass_before) {
+                const u64 before = base + (counts ? number : mass_before);
+                return counts ? before < limit : before == 0 || (double)before < threshold;
+            };
+            if (leads && keeps(ahead, mass_ahead) && (ahead + 1 == n || !keeps(ahead + 1, mass_ahead + mass))) {
+                s.least = at;
+                s.selected = mass_ahead + mass;
             }
             __syncthreads();
         };
@@ -464,15 +492,24 @@ sample_kernel(const __grid_constant__ SampleParams p) {
         };
         // a histogram of the list over `bucket`, then sums of the buckets before
         auto spread = [&](unsigned n, auto bucket) __attribute__((always_inline)) {
-            for (int b = threadIdx.x; b < kBuckets; b += kThreads) { s.count[b] = 0; s.mass[b] = 0; }
+            for (int b = threadIdx.x; b < kBuckets; b += kThreads) s.count[b] = s.low[b] = s.high[b] = 0;
             __syncthreads();
             for (unsigned i = threadIdx.x; i < n; i += kThreads) {
                 const u64 at = s.list[i];
                 const int b = bucket(at);
                 if (b < 0) continue;
+                const uint32_t mass = mass_of(weight_at(at));
                 atomicAdd(&s.count[b], 1u);
-                atomicAdd(&s.mass[b], (u64)mass_of(weight_at(at)));
+                atomicAdd(&s.low[b], mass & 0xffffu);
+                atomicAdd(&s.high[b], mass >> 16);
             }
+            __syncthreads();
+            u64 mass[kPerThread];
+#pragma unroll
+            for (int i = 0; i < kPerThread; ++i) mass[i] = (u64)s.low[threadIdx.x * kPerThread + i] + ((u64)s.high[threadIdx.x * kPerThread + i] << 16);
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < kPerThread; ++i) s.mass[threadIdx.x * kPerThread + i] = mass[i];
             accumulate();
         };
         // the last bucket that holds anything and whose sum before `keeps`
@@ -697,14 +734,34 @@ sample_kernel(const __grid_constant__ SampleParams p) {
                     }
                     return c;
                 }
-                const u64 base = counts ? (u64)s.count[bucket] : s.mass[bucket];
-                if (n <= kThreads) {
-                    compare(s.list, n, counts, base, limit, threshold);
+                u64 base = counts ? (u64)s.count[bucket] : s.mass[bucket], mass_base = s.mass[bucket];
+                unsigned some = n;
+                u64* among = s.list;
+                // more than can be compared with one another cheaply: a histogram within the bucket, unless the one at hand is still needed
+                if (n > 64 && !(counts && by_mass)) {
+                    spread(n, [&](u64 at) {
+                        const float within = exponent(logit_at(at)) * (-kBuckets / kLastZ) - bucket;
+                        return max(0, min(kBuckets - 1, (int)(within * kBuckets)));
+                    });
+                    const int b = crossing([&](int i) { return keeps(base + (counts ? (u64)s.count[i] : s.mass[i])); });
+                    const unsigned found = pick(n, [&](u64 at) {
+                        const float within = exponent(logit_at(at)) * (-kBuckets / kLastZ) - bucket;
+                        return max(0, min(kBuckets - 1, (int)(within * kBuckets))) == b;
+                    });
+                    if (found && found <= kThreads) {
+                        base += counts ? (u64)s.count[b] : s.mass[b];
+                        mass_base += s.mass[b];
+                        among = s.picked;
+                        some = found;
+                    }
+                }
+                if (some <= kThreads) {
+                    compare(among, some, counts, base, limit, threshold);
                 } else {
                     sort_falling<kThreads>(s.list, n);
                     least_kept(n, counts, base, limit, threshold);
                 }
-                if (counts) whole = s.mass[bucket] + s.selected;
+                if (counts) whole = mass_base + s.selected;
                 const u64 c = n ? s.least : 0;      // an empty last bucket: everything is kept
                 __syncthreads();
                 return c;
