@@ -29,8 +29,6 @@ namespace cg = cooperative_groups;
 typedef unsigned long long u64;
 
 constexpr int kMaxCtas = 8;
-constexpr int kBuckets = 1024;
-constexpr int kList = 2048;
 constexpr int kTable = 256;
 constexpr float kOne = 2147483648.f;     // 2^31: the mass of the largest logit's token
 constexpr float kLastZ = 22.25f;         // exp(-z) 2^31 < 1/2 from z = 22.2 on: no mass
@@ -54,6 +52,9 @@ struct SampleParams {
 enum { ASK_DONE = 0, ASK_LIST = 1, ASK_ABOVE = 2 };
 
 template <int kThreads> struct Shared {
+    // 256 threads: four such CTAs with slices of 33 KB on an SM instead of the three that twice the sizes leave (512 rows of 131071 by top-p 549 -> 445 us,
+    // by min-p 121 -> 108; by top-k 1000, of which the longer list held all, 229 -> 409)
+    static constexpr int kBuckets = 2 * kThreads, kList = 4 * kThreads;
     float tops[kMaxCtas];                // of every CTA, in every CTA
     u64 totals[kMaxCtas], passing[kMaxCtas], kept[kMaxCtas];
     u64 scratch[kThreads / 32];
@@ -108,7 +109,7 @@ __device__ __forceinline__ float exponent_of(float x, float largest, float inver
     return apart * inverse;
 }
 __device__ __forceinline__ uint32_t mass_of(float weight) { return __float2uint_rn(weight * kOne); }      // of NaN: 0
-__device__ __forceinline__ int bucket_of(float exponent) { return min(kBuckets - 1, (int)(exponent * (-kBuckets / kLastZ))); }
+template <int kBuckets> __device__ __forceinline__ int bucket_of(float exponent) { return min(kBuckets - 1, (int)(exponent * (-kBuckets / kLastZ))); }
 __device__ __forceinline__ float max_of(const uint4& v, float so_far, __nv_bfloat16) {
     const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&v);
     const __nv_bfloat162 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
@@ -180,8 +181,9 @@ template <typename T, bool HELD, int kThreads>
 __global__ void __launch_bounds__(kThreads, 1024 / kThreads)
 sample_kernel(const __grid_constant__ SampleParams p) {
     chain_begin();
-    constexpr int N = Vec16<T>::N, kWarps = kThreads / 32, kPerThread = kBuckets / kThreads;
+    constexpr int N = Vec16<T>::N, kWarps = kThreads / 32;
     using Shared = Shared<kThreads>;
+    constexpr int kBuckets = Shared::kBuckets, kList = Shared::kList, kPerThread = kBuckets / kThreads;
     extern __shared__ __align__(16) uint8_t smem[];
     Shared& s = *reinterpret_cast<Shared*>(smem);
     uint4* held = reinterpret_cast<uint4*>(smem + (sizeof(Shared) + 15) / 16 * 16);
@@ -294,8 +296,8 @@ sample_kernel(const __grid_constant__ SampleParams p) {
             if (!(e > -kLastZ)) continue;
             const uint32_t mass = mass_of(expf(e));
             if (!mass) continue;
-            if (by_count) atomicAdd(&s.own.count[bucket_of(e)], 1u);
-            else add(bucket_of(e), mass, true);
+            if (by_count) atomicAdd(&s.own.count[bucket_of<kBuckets>(e)], 1u);
+            else add(bucket_of<kBuckets>(e), mass, true);
         }
         __syncthreads();
         // a thread's buckets: the first that reaches what is wanted, together with all before
@@ -649,7 +651,7 @@ sample_kernel(const __grid_constant__ SampleParams p) {
         each([&](float f, int, int) __attribute__((always_inline)) {
             const float e = exponent(f);
             if (!(e > -kLastZ)) return;
-            const int b = bucket_of(e);
+            const int b = bucket_of<kBuckets>(e);
             if (b > bound) return;
             const uint32_t mass = mass_of(expf(e));
             if (mass) add(b, mass, by_count);         // a bucket with members has mass: only top-k needs their number
