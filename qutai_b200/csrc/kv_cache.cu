@@ -2,11 +2,14 @@
 // cache is an 8-bit one, and positions read back.  Both are streams: what bounds them is HBM, or the launch for a handful of rows.
 //
 // 8 bits are whole multiples of a scale of each head and position, max |x| / 127.  Against an 8-bit floating type under the same scale
-// the error is a quarter (dim 64, normal values: 0.7 % of the root mean square instead of 2.6 %), and the whole numbers are exact in
+// the error is a quarter (dim 64, normal values, by calculation: 0.7 % of the root mean square instead of 2.6 %), and the whole numbers are exact in
 // bf16, so the attention that reads them can hand them to the tensor cores as they are.  The division is the rounded one
 // of IEEE, not a product with the reciprocal: x / s then lies on the same side of a tie everywhere.
 //
 // dim / 16 lanes (rounded up to a power of two) hold a head of one position, 16 values each.
+//
+// Measured, 8 bits, 4 heads of 64: one position each of 64 sequences written and up to 301 of each read into bfloat16 9.7 us, 25 MB; 8192 positions written
+// and read 9.6 us, 17 MB.  Two launches of which the second waits for the first are most of either; the division takes the append 60 % of the issue slots.
 #include "common.cuh"
 
 #include <type_traits>

@@ -94,8 +94,8 @@ __device__ __forceinline__ uint32_t bytes_to_bf16(uint32_t w) {
     return r;
 }
 
-// Keys of a tile: 128 where a warp has a quarter of them, so that its steps have some work to overlap (64 sequences, 512 positions: 1450 cycles a
-// tile of 64, in which nothing was waited for but one step for the next)
+// Keys of a tile: 128 where a warp has a quarter of them, so that its steps have some work to overlap: a tile of 64 took 1450 cycles (128 sequences, 8
+// heads, up to 1025 positions), in which nothing was waited for but one step for the next
 template <int DIM, bool INT8, bool BY_KEYS> struct Tile {
     static constexpr int kKeys = BY_KEYS && DIM == 64 ? 128 : 64;
     static constexpr int kRowBytes = INT8 ? DIM : 2 * DIM;
@@ -110,11 +110,13 @@ template <int DIM, bool INT8, bool A, bool B> constexpr int shared_of() {
     return Tile<DIM, INT8, A>::kShared > Tile<DIM, INT8, B>::kShared ? Tile<DIM, INT8, A>::kShared : Tile<DIM, INT8, B>::kShared;
 }
 
-// Rows of a tile: 16 to a warp (BY_KEYS false: 64 rows, every warp walks all keys) or the same 16 for all warps (BY_KEYS: a
-// quarter of every tile of keys each, joined at the end), for the few rows of one sequence.
 // of the threads that attend, in whatever block
 __device__ __forceinline__ void attend_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kThreads) : "memory"); }
 
+// Rows of a tile: 16 to a warp (BY_KEYS false: 64 rows, every warp walks all keys) or the same 16 for all warps (BY_KEYS: a
+// quarter of every tile of keys each, joined at the end), for the few rows of one sequence.
+// What bounds it: one step's wait for the next (loads, products, exponentials) of three to four blocks on an SM.  128 sequences of up to 1025
+// positions, 8 heads of 64: 134 MB in 30 us, 4.5 TB/s, two thirds of what HBM copies at.
 template <int DIM, bool INT8, bool BY_KEYS>
 __device__ __forceinline__ void attend(const PrefixParams& p, const Keys& keys, uint8_t* smem, int b, int g, int row_tile, int split, bool own) {
     using L = Tile<DIM, INT8, BY_KEYS>;
@@ -409,8 +411,9 @@ prefix_attention_kernel(const __grid_constant__ PrefixParams p) {
 // The scores of the next blocks go to other buffers meanwhile.  Keys and values of 8 bits come through warp 0 and two more, which load them
 // and put them into shared memory as bf16, exactly, in the order in which TMA would have; their scales go to the rows, the key's into
 // the score, the value's into the probability.
-// What bounds it: the exponential unit, 512 cycles for a block and SM (the products take 384, 256 of them the two of P V), which two CTAs to
-// an SM share: one's exponentials run beside the other's waits.
+// What bounds it: the exponential unit, 512 cycles for a block (the products take 384, 256 of them the two of P V), beside the rows' other
+// instructions; two CTAs to an SM, so that one's run beside the other's waits.  512 rows of 8 heads by 32768 keys of 64: 68 us, 1550 cycles for a block of each
+// of the two CTAs, the exponential unit busy for 52 % of the time, the tensor cores for 39 %.  Three CTAs to an SM and more tiles ahead were no faster.
 // ------------------------------------------------------------------------------------------------
 constexpr int kTcKeys = 64, kTcColumns = 256, kTcConverters = 3;
 
@@ -741,8 +744,8 @@ prefix_tensor_kernel(const __grid_constant__ PrefixTcParams tc) {
             }
             if (n || whole) {
                 tc_fence_after();
-                // 32 columns at a time through shared memory (the tiles are done with), so that the rows are written in pieces of 128 bytes (64
-                // sequences, 4096 keys: 3300 of a block's 14000 cycles with a row to a thread)
+                // 32 columns at a time through shared memory (the tiles are done with), so that the rows are written in pieces of 128 bytes and not by
+                // a thread each.  (A short item spends a quarter of its time here either way: 3400 of 14000 cycles, 64 sequences, 4096 keys.)
                 constexpr int PITCH = 36;
                 float* const stage = reinterpret_cast<float*>(smem_raw + (k_tile - base)) + quad * 32 * PITCH;
                 const float factor = n ? whole ? inverse : 1.f : 0.f;
@@ -782,7 +785,7 @@ prefix_tensor_kernel(const __grid_constant__ PrefixTcParams tc) {
 
 // The parts of a row: WARPS warps to a row, which take every WARPS-th part, their weights a lane each, eight parts' values on their way together, and
 // meet in shared memory.  One warp to a row, four rows to a block, where that leaves enough warps or there is little to each; else eight: 16 rows in 97
-// parts of 128 values take 26 us with one and 5 with eight, 4096 rows in 10 parts 5 and 12.
+// parts of 128 values take 26 us with one and 5 with eight, 4096 rows in 10 parts 5 and 12.  What bounds it is the wait for the parts, from L2.
 template <int DIM, int WARPS>
 __global__ void __launch_bounds__(WARPS == 1 ? kThreads : 32 * WARPS)
 prefix_join_kernel(const __grid_constant__ PrefixParams p) {

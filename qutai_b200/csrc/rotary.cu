@@ -11,6 +11,9 @@
 // turns is held as a 64-bit fraction F (2^64 = one turn), so position * F modulo 2^64, an integer product, IS that fraction, exact to
 // 2^-64 * position at any position, and its upper half goes to sincospi.  (In 32 bits the angle of position 100000 is off by 4e-3.)
 // Sums over rows run in a fixed order (no atomics).
+//
+// What bounds it: the instructions, issued in 68 % of the cycles forward and 63 % backward.  8192 rows of 16 and 4 heads of 64 in bfloat16: forward
+// 11.5 us, 42 MB at 3.6 TB/s; backward 18 us, 63 MB at 3.5 TB/s, and 5 us for the joined sum of its blocks' shares of the weights' gradients.
 #include "common.cuh"
 
 #include <math.h>
@@ -329,7 +332,7 @@ Shape shape_of(long long rows, int heads, int kv_heads, int dim, bool backward) 
     return s;
 }
 
-// the usual widths with their lanes known to the compiler (64: 12.6 -> 11 us for 8192 rows of 16 and 4 heads), others with a loop
+// the usual widths with their lanes known to the compiler, others with a loop (8192 rows of 16 and 4 heads of 64, both directions: 34.8 us and 36.8)
 template <typename Launch> void launch_by_width(const qmoe_norm_rope_t* a, Launch launch) {
     auto by_type = [&](auto value) {
         if (a->dim == 64) launch(value, std::integral_constant<int, 3>());

@@ -15,7 +15,13 @@
 //   4  else a histogram, counts and masses, of what lies above the bound; its crossing bucket is the only one whose members have to be
 //      told apart, and goes to the list instead.  A bucket too full for that (thousands of equal logits): the threshold by bisection over
 //      the places, every step a question to all CTAs
-//   5  every CTA's kept mass; the CTA that holds the drawn number's place walks to it by sums over warps, lanes and elements
+//   5  every CTA's kept mass; the warp's share that holds the drawn number's place, by the warps' sums, is looked through by sums over warps, lanes and
+//      elements
+//
+// What bounds it: instructions and the exponential unit (an exponential and a conversion for every token), and for few rows the cluster's barriers.  256 rows
+// of 131071 bfloat16 logits by top-p and min-p: 58 us, 67 MB at 1.2 TB/s, 64 % of the issue slots of the SMs that have work; one row of 32000 by top-k and
+// top-p: 9.8 us, some 40 % of it the barriers and the launch.  Where thousands of tokens are kept, the histogram's atomics and the passes after it:
+// 512 rows of 131071 by top-p 0.95 445 us, 98 without any cut.
 #include "common.cuh"
 
 #include <cooperative_groups.h>
