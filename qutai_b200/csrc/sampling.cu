@@ -500,6 +500,7 @@ sample_kernel(const __grid_constant__ SampleParams p) {
         };
         // a histogram of the list over `bucket`, then sums of the buckets before
         auto spread = [&](unsigned n, auto bucket) __attribute__((always_inline)) {
+            __syncthreads();             // the one before has been read
             for (int b = threadIdx.x; b < kBuckets; b += kThreads) s.count[b] = s.low[b] = s.high[b] = 0;
             __syncthreads();
             for (unsigned i = threadIdx.x; i < n; i += kThreads) {

@@ -166,3 +166,21 @@ def test_lists_of_every_length(top_k, dtype):
     logits[3:] = np.round(logits[3:] * 2) / 2           # few levels, every one many times
     check(logits, rng.random(6), dtype, top_k=top_k)
     check(logits, rng.random(6), dtype, top_k=top_k, top_p=0.7, temperature=0.9, min_p=0.01)
+
+
+@pytest.mark.parametrize("settings", [{"top_k": 600}, {"top_k": 2040, "top_p": 0.7}, {"top_p": 0.9}, {"top_k": 6000, "top_p": 0.8, "min_p": 0.01}, {"min_p": 0.01}])
+@pytest.mark.parametrize("rows", [5, 300])
+def test_every_call_gives_the_same(rows, settings):
+    """The same bits from the same arguments, twenty calls in a row, on rows of few and of many different logits."""
+    from gpu_util import to_device
+    from qutai_b200.layers import Tensor
+    from qutai_b200.sampling import sample
+
+    rng = np.random.default_rng(rows)
+    logits = rng.standard_normal((rows, 20011)) * 2.0
+    logits[::2] = np.round(logits[::2] * 2) / 2
+    logits = Tensor(to_device(logits, "bfloat16"), logits.shape)
+    uniforms = to_device(rng.random(rows), "float32")
+    first = [x.tobytes() for x in sample(logits, uniforms, **settings)]
+    for _ in range(20):
+        assert [x.tobytes() for x in sample(logits, uniforms, **settings)] == first
