@@ -575,8 +575,8 @@ int qmoe_cache_read(const qmoe_cache_t* cache, int64_t start, int64_t count, uin
 /* New queries of a batch over a prefix that all its sequences share and over each sequence's own cache, which holds the keys
  * of the new positions already:
  *     out[b, t, h, :] = softmax([q . Kp^T, q . Kb^T] / sqrt(dim)) [Vp; Vb],   query t seeing the whole prefix and the first
- * lengths[b] - time + t + 1 positions of sequence b.  A row that sees nothing gives zeros and lse = -infinity.  The prefix (a cache of batch 1) is
- * read once for all sequences.  bf16 queries, dim 64 or 128. */
+ * lengths[b] - time + t + 1 positions of sequence b.  A row that sees nothing gives zeros and lse = -infinity; one with a score that is NaN or
+ * +infinity gives NaN in both.  The prefix (a cache of batch 1) is read once for all sequences.  bf16 queries, dim 64 or 128. */
 typedef struct qmoe_prefix_attention {
     int64_t time;                        /* new positions of every sequence */
     int32_t heads;

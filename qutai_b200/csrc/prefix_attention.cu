@@ -2,6 +2,7 @@
 //     out = softmax([q Kp^T, q Kb^T] / sqrt(dim)) [Vp; Vb],
 // the prefix read once for the whole batch.  A softmax over a set of keys is joined from its parts: a part that has seen the keys S leaves
 // m = max s, l = sum exp(s - m), o = sum exp(s - m) v, and parts meet as M = max m, sum exp(m - M) o / sum exp(m - M) l.
+// l = 0 says that a part has seen nothing; a score that is no number leaves m as it is and l NaN, and with it the row.
 //
 // Work items.  All queries that meet the same keys are rows of one product: for the prefix the batch * time * group queries of a
 // key/value head, for a sequence's own cache its time * group.  An item is one key/value head, a tile of rows, and a chunk of the
@@ -352,9 +353,9 @@ __device__ __forceinline__ void attend(const PrefixParams& p, const Keys& keys, 
         }
         const bool whole = p.slots == 1;
         const long long slot = (long long)(keys.first_slot + split) * p.rows + to;
-        const float inverse = total > 0.f ? 1.f / total : 0.f;
+        const float inverse = total != 0.f ? 1.f / total : 0.f;         // (NaN stays)
         if (piece == 0) {
-            if (whole) p.lse[to] = total > 0.f ? (top + log2f(total)) * LN2 : -INFINITY;
+            if (whole) p.lse[to] = total != 0.f ? (top + log2f(total)) * LN2 : -INFINITY;
             else p.part_ml[slot] = make_float2(top, total);
         }
         for (int d = piece * 4; d < DIM; d += 32) {
@@ -372,9 +373,9 @@ __device__ __forceinline__ void attend(const PrefixParams& p, const Keys& keys, 
         for (int i = 0; i < 2; ++i) {
             if (at[i] < 0) continue;
             const long long slot = (long long)(keys.first_slot + split) * p.rows + at[i];
-            const float inverse = l[i] > 0.f ? 1.f / l[i] : 0.f;
+            const float inverse = l[i] != 0.f ? 1.f / l[i] : 0.f;
             if (t4 == 0) {
-                if (p.slots == 1) p.lse[at[i]] = l[i] > 0.f ? (m[i] + log2f(l[i])) * LN2 : -INFINITY;
+                if (p.slots == 1) p.lse[at[i]] = l[i] != 0.f ? (m[i] + log2f(l[i])) * LN2 : -INFINITY;
                 else p.part_ml[slot] = make_float2(m[i], l[i]);
             }
 #pragma unroll
@@ -737,9 +738,9 @@ prefix_tensor_kernel(const __grid_constant__ PrefixTcParams tc) {
         if (ok) {
             const bool whole = p.slots == 1;
             const long long slot = (long long)(p.prefix.first_slot + split) * p.rows + at;
-            const float inverse = l > 0.f ? 1.f / l : 0.f;
+            const float inverse = l != 0.f ? 1.f / l : 0.f;
             if (live) {
-                if (whole) p.lse[at] = l > 0.f ? (m + log2f(l)) * LN2 : -INFINITY;
+                if (whole) p.lse[at] = l != 0.f ? (m + log2f(l)) * LN2 : -INFINITY;
                 else p.part_ml[slot] = make_float2(m, l);
             }
             if (n || whole) {
@@ -800,7 +801,9 @@ prefix_join_kernel(const __grid_constant__ PrefixParams p) {
         const int slot = first + lane * WARPS;
         const float2 ml = slot < p.slots ? p.part_ml[slot * p.rows + row] : make_float2(-INFINITY, 0.f);
         const float next = fmaxf(top, warp_max(ml.x)), from = next == -INFINITY ? 0.f : next, alpha = exp2_fast(top - from);
-        const float factor = ml.y == 0.f ? 0.f : exp2_fast(ml.x - from);             // 0: saw no key, its values were not written
+        const bool saw = ml.y != 0.f;    // else no key: its values were not written
+        const unsigned seen = __ballot_sync(0xffffffffu, saw);
+        const float factor = saw ? ml.y == ml.y ? exp2_fast(ml.x - from) : ml.y : 0.f;         // NaN where the part is
         top = next;
         total = total * alpha + warp_sum(factor * ml.y);
         sum.x *= alpha; sum.y *= alpha; sum.z *= alpha; sum.w *= alpha;
@@ -811,9 +814,8 @@ prefix_join_kernel(const __grid_constant__ PrefixParams p) {
 #pragma unroll
             for (int i = 0; i < DEEP; ++i) {
                 const int part = s + i * TOGETHER + lane / LANES;
-                f[i] = __shfl_sync(0xffffffffu, factor, part & 31);
-                if (part >= many) f[i] = 0.f;
-                v[i] = f[i] != 0.f ? *reinterpret_cast<const float4*>(p.part_o + ((first + part * WARPS) * p.rows + row) * DIM + lane % LANES * 4) : make_float4(0.f, 0.f, 0.f, 0.f);
+                f[i] = __shfl_sync(0xffffffffu, factor, part);                    // 0 from `many` on
+                v[i] = seen >> part & 1 ? *reinterpret_cast<const float4*>(p.part_o + ((first + part * WARPS) * p.rows + row) * DIM + lane % LANES * 4) : make_float4(0.f, 0.f, 0.f, 0.f);
             }
 #pragma unroll
             for (int i = 0; i < DEEP; ++i) { sum.x += f[i] * v[i].x; sum.y += f[i] * v[i].y; sum.z += f[i] * v[i].z; sum.w += f[i] * v[i].w; }
@@ -845,9 +847,9 @@ prefix_join_kernel(const __grid_constant__ PrefixParams p) {
             sum.x += f * v.x; sum.y += f * v.y; sum.z += f * v.z; sum.w += f * v.w;
         }
     }
-    const float inverse = total > 0.f ? 1.f / total : 0.f;
+    const float inverse = total != 0.f ? 1.f / total : 0.f;
     if (lane < LANES) *reinterpret_cast<uint2*>(p.out + row * DIM + lane * 4) = make_uint2(pack2(sum.x * inverse, sum.y * inverse), pack2(sum.z * inverse, sum.w * inverse));
-    if (lane == 0) p.lse[row] = total > 0.f ? (top + log2f(total)) * LN2 : -INFINITY;
+    if (lane == 0) p.lse[row] = total != 0.f ? (top + log2f(total)) * LN2 : -INFINITY;
 }
 
 struct Plan { Keys prefix, own; int slots; long long prefix_items, own_items; bool tensor, together, prefix_by_keys, own_by_keys; };
