@@ -37,8 +37,8 @@ def _describe(q, k, v, heads, kv_heads):
 def attention_forward(q, k, v, heads, kv_heads, stream=0):
     """Returns ``(out, lse)`` as device storages (bfloat16 [batch * time * heads * dim], float32 [batch * time * heads])."""
     a = _describe(q, k, v, heads, kv_heads)
-    out = DeviceStorage(q.storage.size, "bfloat16")
-    lse = DeviceStorage(a.batch * a.time * a.heads, "float32")
+    out = DeviceStorage(q.storage.size, "bfloat16", stream=stream)
+    lse = DeviceStorage(a.batch * a.time * a.heads, "float32", stream=stream)
     a.out, a.lse = out.ptr, lse.ptr
     lib.call("qmoe_attention_forward", ctypes.byref(a), stream)
     return out, lse
@@ -50,10 +50,10 @@ def attention_backward(gradient, q, k, v, out, lse, heads, kv_heads, stream=0):
     gradient = getattr(gradient, "storage", gradient)
     if gradient.dtype != "bfloat16" or gradient.size != q.storage.size:
         raise ValueError("the gradient must be bfloat16 and shaped like the output")
-    dq = DeviceStorage(q.storage.size, "bfloat16")
-    dk = DeviceStorage(k.storage.size, "bfloat16")
-    dv = DeviceStorage(v.storage.size, "bfloat16")
-    delta = DeviceStorage(lse.size, "float32")
+    dq = DeviceStorage(q.storage.size, "bfloat16", stream=stream)
+    dk = DeviceStorage(k.storage.size, "bfloat16", stream=stream)
+    dv = DeviceStorage(v.storage.size, "bfloat16", stream=stream)
+    delta = DeviceStorage(lse.size, "float32", stream=stream)
     a.out, a.lse, a.grad_out, a.delta = out.ptr, lse.ptr, gradient.ptr, delta.ptr
     a.dq, a.dk, a.dv = dq.ptr, dk.ptr, dv.ptr
     lib.call("qmoe_attention_backward", ctypes.byref(a), stream)

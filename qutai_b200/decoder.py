@@ -62,11 +62,11 @@ class Linear:
     (tensor cores from 128 rows on, whatever their number)."""
 
     def __init__(self, width_in, width_out, *, std, seed, stream=0):
-        storage = DeviceStorage(width_out * width_in, "float32")
+        storage = DeviceStorage(width_out * width_in, "float32", stream=stream)
         storage.fill_normal(0.0, std, 0x5EED if seed is None else seed, stream)
         self.weight = Tensor(storage, (width_out, width_in), requires_grad=True)
         self.width_in, self.width_out, self.stream = width_in, width_out, stream
-        self._operand = DeviceStorage(storage.size, "bfloat16")
+        self._operand = DeviceStorage(storage.size, "bfloat16", stream=stream)
 
     def parameters(self):
         return (self.weight,)
@@ -81,18 +81,18 @@ class Linear:
         lib.call("qmoe_gemm", a.ptr, lib.QMOE_BF16, b.ptr, lib.QMOE_BF16, c.ptr, c_dtype, m, k, n, ta, tb, 0, self.stream)
 
     def forward(self, x, rows):
-        y = DeviceStorage(rows * self.width_out, "bfloat16")
+        y = DeviceStorage(rows * self.width_out, "bfloat16", stream=self.stream)
         self._gemm(x, self.operand(), y, rows, self.width_in, self.width_out, 0, 1, lib.QMOE_BF16)
         return y
 
     def backward(self, dy, x, rows):
         """Input gradient [rows, in] (bf16); the weight gradient [out, in] (float32) is accumulated into ``weight.grad``."""
-        dx = DeviceStorage(rows * self.width_in, "bfloat16")
+        dx = DeviceStorage(rows * self.width_in, "bfloat16", stream=self.stream)
         self._gemm(dy, self.operand(), dx, rows, self.width_out, self.width_in, 0, 0, lib.QMOE_BF16)
-        dw = DeviceStorage(self.weight.storage.size, "float32")
+        dw = DeviceStorage(self.weight.storage.size, "float32", stream=self.stream)
         partials = lib.load().qmoe_gemm_wgrad_partials(self.width_out, rows, self.width_in)
         if partials:    # few output tiles, many rows: the rows are cut into ranges that run side by side
-            scratch = DeviceStorage(partials, "float32")
+            scratch = DeviceStorage(partials, "float32", stream=self.stream)
             lib.call("qmoe_gemm_wgrad_split", dy.ptr, x.ptr, dw.ptr, scratch.ptr, self.width_out, rows, self.width_in, self.stream)
         else:
             self._gemm(dy, x, dw, self.width_out, rows, self.width_in, 1, 0, lib.QMOE_F32)
@@ -114,15 +114,15 @@ def _integers(rows, room):
 
 
 def _rms_norm(x, norm, rows, width, stream):
-    out, inverse = DeviceStorage(rows * width, "bfloat16"), DeviceStorage(rows, "float32")
+    out, inverse = DeviceStorage(rows * width, "bfloat16", stream=stream), DeviceStorage(rows, "float32", stream=stream)
     lib.call("qmoe_rms_norm", x.ptr, lib.QMOE_BF16, norm.weight.storage.ptr, out.ptr, lib.QMOE_BF16, inverse.ptr, rows, width,
              norm.eps, stream)
     return out, inverse
 
 
 def _rms_norm_backward(gradient, x, norm, inverse, rows, width, stream):
-    dx, dw = DeviceStorage(rows * width, "bfloat16"), DeviceStorage(width, "float32")
-    partials = DeviceStorage(lib.load().qmoe_rms_norm_partials(rows, width), "float32")
+    dx, dw = DeviceStorage(rows * width, "bfloat16", stream=stream), DeviceStorage(width, "float32", stream=stream)
+    partials = DeviceStorage(lib.load().qmoe_rms_norm_partials(rows, width), "float32", stream=stream)
     lib.call("qmoe_rms_norm_backward", gradient.ptr, lib.QMOE_BF16, x.ptr, lib.QMOE_BF16, norm.weight.storage.ptr, inverse.ptr,
              dx.ptr, dw.ptr, partials.ptr, rows, width, stream)
     _accumulate(norm.weight, dw, stream)
@@ -130,7 +130,7 @@ def _rms_norm_backward(gradient, x, norm, inverse, rows, width, stream):
 
 
 def _add(a, b, stream):
-    out = DeviceStorage(a.size, a.dtype)
+    out = DeviceStorage(a.size, a.dtype, stream=stream)
     lib.call("qmoe_add", a.ptr, b.ptr, out.ptr, lib.DTYPE_CODES[a.dtype], a.size, stream)
     return out
 
@@ -163,7 +163,7 @@ class GQA:
         return [(name, getattr(self, name).weight) for name in names]
 
     def _rope(self, values, batch, time, heads, inverse, offset=0):
-        out = DeviceStorage(values.size, "bfloat16")
+        out = DeviceStorage(values.size, "bfloat16", stream=self.stream)
         lib.call("qmoe_rope", values.ptr, out.ptr, lib.QMOE_BF16, batch, time, heads, self.dim, float(self.theta), offset, 1 if inverse else 0,
                  self.stream)
         return out
@@ -279,7 +279,7 @@ class Decoder:
         if config.d_model % config.n_heads or config.d_model // config.n_heads != 64:
             raise ValueError("the head width d_model / n_heads must be 64")
         self.config, self.stream = config, stream
-        table = DeviceStorage(config.vocab_size * config.d_model, "float32")
+        table = DeviceStorage(config.vocab_size * config.d_model, "float32", stream=stream)
         table.fill_normal(0.0, 0.02, 0x5EED if seed is None else seed, stream)
         self.embedding = type("Projection", (), {})()
         self.embedding.weight = Tensor(table, (config.vocab_size, config.d_model), requires_grad=True)
@@ -381,7 +381,7 @@ class Decoder:
         ids = uploaded.view(0, rows)
         tables = (uploaded.view(2 * rows, distinct), uploaded.view(3 * rows, distinct + 1), uploaded.view(rows, rows))
         label_ids = ids if labels is None else DeviceStorage.from_bytes(array("q", targets).tobytes(), "int64", stream)
-        x = DeviceStorage(rows * width, "bfloat16")
+        x = DeviceStorage(rows * width, "bfloat16", stream=stream)
         lib.call("qmoe_embedding", self.embedding.weight.storage.ptr, ids.ptr, x.ptr, lib.QMOE_BF16, rows, width, c.vocab_size, stream)
         auxiliary = []
         for block in self.blocks:
@@ -397,7 +397,7 @@ class Decoder:
             if self._share[0] != value:
                 self._share = (value, DeviceStorage.from_values([value], "float32", stream))
             share = self._share[1]
-            weighted = DeviceStorage(1, "float32")
+            weighted = DeviceStorage(1, "float32", stream=stream)
             lib.call("qmoe_scale_f32", lm.storage.ptr, weighted.ptr, 0, share.ptr, 1, 1, stream)
             lib.call("qmoe_ep_all_reduce_f32", weighted.ptr, 1, stream)
             lm = Tensor(weighted, ())
@@ -407,7 +407,7 @@ class Decoder:
         for aux in auxiliary:
             lib.call("qmoe_add", mean_aux.ptr, aux.storage.ptr, mean_aux.ptr, lib.QMOE_F32, 1, stream)
         lib.call("qmoe_scale_f32", mean_aux.ptr, mean_aux.ptr, 0, self._one_over_layers.ptr, 1, 1, stream)
-        scaled = DeviceStorage(1, "float32")
+        scaled = DeviceStorage(1, "float32", stream=stream)
         lib.call("qmoe_scale_f32", mean_aux.ptr, scaled.ptr, 0, self._aux_coef.ptr, 1, 1, stream)
         lib.call("qmoe_add", lm.storage.ptr, scaled.ptr, total.ptr, lib.QMOE_F32, 1, stream)
         self.last_lm_loss, self.last_auxiliary_loss = lm, Tensor(mean_aux, ())
@@ -444,7 +444,7 @@ class Decoder:
         held = [p for p in self.replicated_parameters() if p.grad is not None]
         if not held:
             return
-        flat = DeviceStorage(sum(p.grad.storage.size for p in held), "float32")
+        flat = DeviceStorage(sum(p.grad.storage.size for p in held), "float32", stream=stream)
         offset = 0
         for parameter in held:
             size = parameter.grad.storage.size

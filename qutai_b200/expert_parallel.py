@@ -26,6 +26,7 @@ import ctypes
 import hashlib
 import os
 import time
+from functools import partial
 from math import sqrt
 
 from . import lib
@@ -280,13 +281,13 @@ class ExpertParallelMoE:
         self.local_experts = L = E // world
         self.engine = {"auto": lib.ENGINE_AUTO, "simt": lib.ENGINE_SIMT, "tcgen05": lib.ENGINE_TCGEN05}[engine]
         self._down_std = 0.02 / sqrt(2 * config.n_layers)
-        router = DeviceStorage(E * d, "float32")
+        router = DeviceStorage(E * d, "float32", stream=stream)
         router.fill_normal(0.0, 0.02, 0x5EED if seed is None else seed, stream)
         self.router = Projection(Tensor(router, (E, d), requires_grad=True))
         self._set_placement(contiguous_placement(E, world) if placement is None else list(placement))
-        self._gate = DeviceStorage(L * h * d, "float32")
-        self._up = DeviceStorage(L * h * d, "float32")
-        self._down = DeviceStorage(L * d * h, "float32")
+        self._gate = DeviceStorage(L * h * d, "float32", stream=stream)
+        self._up = DeviceStorage(L * h * d, "float32", stream=stream)
+        self._down = DeviceStorage(L * d * h, "float32", stream=stream)
         self._make_experts()
         for j, i in enumerate(self.expert_ids):   # the model's expert number decides the generator key, as on one GPU
             base = None if seed is None else seed + 1 + 3 * i
@@ -320,7 +321,7 @@ class ExpertParallelMoE:
             ints = lambda values: DeviceStorage.from_bytes(b"".join(int(v).to_bytes(4, "little") for v in values), "int32")
             self._to_physical = ints(self._logical_of_physical)   # gather index: physical row p <- logical row
             self._to_logical = ints(self._physical_of_logical)    # gather index: logical row e <- physical row
-            self._router_physical = DeviceStorage(E * self.d_model, "float32")
+            self._router_physical = DeviceStorage(E * self.d_model, "float32", stream=self.stream)
 
     def _make_experts(self):
         L, h, d = self.local_experts, self.d_expert, self.d_model
@@ -382,7 +383,7 @@ class ExpertParallelMoE:
         """One stacked fp32 buffer of per-expert blocks (``rows`` x ``width`` each, in the slot order of
         ``old_ids``) re-sharded to the layer's current placement; returns the new stacked storage."""
         s = self.stream
-        out = DeviceStorage(stacked.size, "float32")
+        out = DeviceStorage(stacked.size, "float32", stream=s)
         sends = [(self.placement[e], j * rows, rows) for j, e in enumerate(old_ids)]
         recvs = [(old_owner[e], j * rows, rows) for j, e in enumerate(self.expert_ids)]
         (sa, sn), (ra, rn) = _segments(sends), _segments(recvs)
@@ -411,7 +412,7 @@ class ExpertParallelMoE:
         Rt = lib.rows_bound(tokens, E, k)
         Rx = lib.rows_bound(tokens * N, L, k)
         blocks = lib.route_blocks(tokens)
-        S = DeviceStorage
+        S = partial(DeviceStorage, stream=self.stream)
         buf = dict(
             probs=S(tokens * E, "float32"), gate_weights=S(A, "float32"), expert_index=S(A, "int32"),
             dest_row=S(A, "int32"), row_source=S(Rt, "int32"), counts=S(E, "int32"), offsets=S(E + 1, "int32"),
@@ -427,8 +428,8 @@ class ExpertParallelMoE:
             router_partials=S(int(lib.load().qmoe_router_grad_partials(tokens, E, d)), "float32"),
             d_w_router=S(E * d, "float32"), d_w_gate=S(L * h * d, "float32"), d_w_up=S(L * h * d, "float32"),
             d_w_down=S(L * d * h, "float32"), aux_grad=S(1, "float32"),
-            ret_table=S(Rx, "int32"), dest_base=S(E, "int32"), barrier=S.zeros(1, "int32"),
-            flags=S.zeros(lib.EP_MAX_RANKS, "int32"),
+            ret_table=S(Rx, "int32"), dest_base=S(E, "int32"), barrier=DeviceStorage.zeros(1, "int32"),
+            flags=DeviceStorage.zeros(lib.EP_MAX_RANKS, "int32"),
         )
         if not self._identity:   # the expert-indexed outputs in the model's numbering
             buf.update(utilization_logical=S(E, "float32"), d_w_router_logical=S(E * d, "float32"))
@@ -666,7 +667,7 @@ class ExpertParallelMoE:
             lib.call("qmoe_ep_plan", buf["stats_all"].ptr, tr, xr, tokens * N, s)
             lib.call("qmoe_ep_zero_pad_rows", xr, buf["x_recv"].ptr, code, d, s)
 
-        out = DeviceStorage(storage.size, dtype)
+        out = DeviceStorage(storage.size, dtype, stream=s)
         acts = (buf["x_recv"].ptr, buf["g"].ptr, buf["u"].ptr, buf["h"].ptr, buf["y_recv"].ptr)
         if self.transport == "p2p":
             peers = w["peers"]
@@ -818,7 +819,7 @@ class ExpertParallelMoE:
             lib.call("qmoe_expert_backward", xr, ex, buf["dy_recv"].ptr, *saved, buf["dy_recv"].ptr, *grads, s)  # dX reuses dY's buffer
             lib.call("qmoe_ep_exchange", buf["dy_recv"].ptr, ra, rn, buf["dy_send"].ptr, sa, sn, d, code, s)
             router_backward()
-        dx = DeviceStorage(x_storage.size, dtype)
+        dx = DeviceStorage(x_storage.size, dtype, stream=s)
         lib.call("qmoe_unpermute_reduce", tr, buf["dy_send"].ptr, buf["dx_router"].ptr, dx.ptr, code, d, s)
         # the status word at the end of the step leaves on the side stream; it is looked at together with the next
         # step's counts (or by check_status), so the host still waits for nothing here

@@ -28,7 +28,7 @@ class Generator:
             raise ValueError("a cache is bfloat16 or int8")
         self.decoder, self.cache_dtype, self.stream = decoder, cache_dtype, decoder.stream
         self.prefix = self.caches = None
-        self._operand = DeviceStorage(decoder.embedding.weight.size, "bfloat16")
+        self._operand = DeviceStorage(decoder.embedding.weight.size, "bfloat16", stream=self.stream)
 
     def _cache(self, batch, capacity):
         attention = self.decoder.blocks[0].attn
@@ -36,7 +36,7 @@ class Generator:
 
     def _embedded(self, ids, rows):
         c = self.decoder.config
-        x = DeviceStorage(rows * c.d_model, "bfloat16")
+        x = DeviceStorage(rows * c.d_model, "bfloat16", stream=self.stream)
         lib.call("qmoe_embedding", self.decoder.embedding.weight.storage.ptr, ids.ptr, x.ptr, lib.QMOE_BF16, rows, c.d_model, c.vocab_size, self.stream)
         return x
 
@@ -47,7 +47,7 @@ class Generator:
             lib.call("qmoe_cast_bf16", table.ptr, self._operand.ptr, table.size, self.stream)
             self._operand.mark_derived_from(table)
         hidden, _ = _rms_norm(x, self.decoder.norm, rows, c.d_model, self.stream)
-        logits = DeviceStorage(rows * c.vocab_size, "float32")
+        logits = DeviceStorage(rows * c.vocab_size, "float32", stream=self.stream)
         lib.call("qmoe_gemm", hidden.ptr, lib.QMOE_BF16, self._operand.ptr, lib.QMOE_BF16, logits.ptr, lib.QMOE_F32, rows, c.d_model, c.vocab_size,
                  0, 1, 0, self.stream)
         return Tensor(logits, (rows, c.vocab_size))
@@ -109,11 +109,11 @@ class Generator:
         vocab = first.shape[1]
         # the first draw of every continuation is from the prompt's last row
         zeros = DeviceStorage.zeros(samples, "int32", self.stream)
-        logits = Tensor(DeviceStorage(samples * vocab, "float32"), (samples, vocab))
+        logits = Tensor(DeviceStorage(samples * vocab, "float32", stream=self.stream), (samples, vocab))
         lib.call("qmoe_gather_rows", first.storage.ptr, logits.storage.ptr, zeros.ptr, samples, 1, 4 * vocab, self.stream)
         if new_tokens > 1:
             self.start(samples, new_tokens - 1)
-        tokens, log_probs = DeviceStorage(samples * new_tokens, "int64"), DeviceStorage(samples * new_tokens, "float32")
+        tokens, log_probs = DeviceStorage(samples * new_tokens, "int64", stream=self.stream), DeviceStorage(samples * new_tokens, "float32", stream=self.stream)
         for i in range(new_tokens):
             out = tokens.view(i * samples, samples), log_probs.view(i * samples, samples)
             sample(logits, uniforms.view(i * samples, samples), temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p, out=out, stream=self.stream)

@@ -43,7 +43,7 @@ class LMHead:
     def _buffer(self, name, size, dtype):
         current = self._buffers.get(name)
         if current is None or current.size < size or current.dtype != dtype:
-            current = self._buffers[name] = DeviceStorage(size, dtype)
+            current = self._buffers[name] = DeviceStorage(size, dtype, stream=self.stream)
         return current
 
     def _weight_operand(self, weight, dtype):
@@ -53,7 +53,7 @@ class LMHead:
             raise ValueError("the head's weight must have the activations' dtype, or be float32 with bfloat16 activations")
         shadow = self._operand
         if shadow is None or shadow.size != weight.storage.size:
-            shadow = self._operand = DeviceStorage(weight.storage.size, "bfloat16")
+            shadow = self._operand = DeviceStorage(weight.storage.size, "bfloat16", stream=self.stream)
         if not shadow.is_derived_from(weight.storage):
             lib.call("qmoe_cast_bf16", weight.storage.ptr, shadow.ptr, weight.storage.size, self.stream)
             shadow.mark_derived_from(weight.storage)
@@ -85,7 +85,7 @@ class LMHead:
         h.logits = self._buffer("logits", bound * vocab, dtype).ptr
         h.row_loss = self._buffer("row_loss", rows, "float32").ptr
         h.meta = self._buffer("meta", 8, "float32").ptr
-        loss = DeviceStorage(1, "float32")
+        loss = DeviceStorage(1, "float32", stream=self.stream)
         h.loss = loss.ptr
         lib.call("qmoe_head_forward", ctypes.byref(h), self.stream)
         self._call = (h, hidden, weight, labels, loss)
@@ -102,11 +102,11 @@ class LMHead:
         d_hidden = d_weight = None
         h.d_inputs = h.d_hidden = h.d_weight = 0
         if need_hidden:
-            d_hidden = DeviceStorage(hidden.storage.size, dtype)
+            d_hidden = DeviceStorage(hidden.storage.size, dtype, stream=self.stream)
             h.d_inputs = self._buffer("d_inputs", h.rows_bound * h.width, dtype).ptr
             h.d_hidden = d_hidden.ptr
         if need_weight:
-            d_weight = DeviceStorage(weight.storage.size, "float32")
+            d_weight = DeviceStorage(weight.storage.size, "float32", stream=self.stream)
             h.d_weight = d_weight.ptr
         if not (need_hidden or need_weight):
             return None, None

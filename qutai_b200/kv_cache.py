@@ -42,7 +42,7 @@ class KVCache:
         self.k_scale = self.v_scale = None
         for name, storage, size, kind in wanted:
             if storage is None:
-                storage = DeviceStorage(size, kind)
+                storage = DeviceStorage(size, kind, stream=stream)
             elif storage.size != size or storage.dtype != kind:
                 raise ValueError(f"{name} must hold {size} values of {kind}")
             setattr(self, name, storage)
@@ -82,7 +82,7 @@ class KVCache:
             raise ValueError("k and v must be float32 or bfloat16, both the same")
         if counts is not None and (counts.dtype != "int32" or counts.size != self.batch):
             raise ValueError("counts must hold one int32 value for each sequence")
-        after, = outputs(None if lengths_out is None else (lengths_out,), ((self.batch, "int32"),))
+        after, = outputs(None if lengths_out is None else (lengths_out,), ((self.batch, "int32"),), self.stream)
         lib.call("qmoe_cache_append", ctypes.byref(self._struct), k_ptr, v_ptr, lib.DTYPE_CODES[dtype], k_pitch, v_pitch, time,
                  0 if counts is None else counts.ptr, after.ptr, self.stream)
         self.rewind(after, self.longest + time)
@@ -95,7 +95,7 @@ class KVCache:
         if start < 0 or count < 0 or start + count > self.capacity:
             raise ValueError("positions outside the cache")
         size = self.batch * count * self.kv_heads * self.dim
-        k, v = outputs(out, ((size, dtype), (size, dtype)))
+        k, v = outputs(out, ((size, dtype), (size, dtype)), self.stream)
         lib.call("qmoe_cache_read", ctypes.byref(self._struct), start, count, k.ptr, v.ptr, lib.DTYPE_CODES[dtype], self.stream)
         shape = (self.batch, count, self.kv_heads * self.dim)
         return Tensor(k, shape), Tensor(v, shape)
@@ -112,14 +112,14 @@ def prefix_attention(q, heads, cache, prefix=None, *, out=None, stream=0):
     if q.storage.dtype != "bfloat16":
         raise ValueError("prefix_attention takes bfloat16 queries")
     rows = cache.batch * q.shape[1] * heads
-    result = outputs(out, ((rows * cache.dim, "bfloat16"), (rows, "float32")))
+    result = outputs(out, ((rows * cache.dim, "bfloat16"), (rows, "float32")), stream)
     q_ptr, out_ptr = q.storage.ptr, result[0].ptr
     if (q_ptr | out_ptr) & 15:
         raise ValueError("q and the output must be 16-byte aligned")
     a = lib.PrefixAttention(q.shape[1], heads, 0, 0 if prefix is None else prefix.longest, cache.longest, q_ptr, out_ptr, result[1].ptr)
     own, shared = ctypes.byref(cache._struct), None if prefix is None else ctypes.byref(prefix._struct)
     nbytes = lib.load().qmoe_prefix_attention_scratch(ctypes.byref(a), own, shared)
-    scratch = DeviceStorage(nbytes // 4, "float32") if nbytes else None
+    scratch = DeviceStorage(nbytes // 4, "float32", stream=stream) if nbytes else None
     a.scratch = scratch.ptr if nbytes else 0
     lib.call("qmoe_prefix_attention", ctypes.byref(a), own, shared, stream)
     return result

@@ -18,6 +18,7 @@ until the next ``backward`` of the same layer (which first copies out any gradie
 from __future__ import annotations
 
 import ctypes
+from functools import partial
 from math import prod, sqrt
 
 from . import lib
@@ -105,7 +106,7 @@ def _accumulate(parameter, view, stream):
     if parameter.grad is None:
         parameter.grad = view
         return
-    out = DeviceStorage(view.size, view.storage.dtype)
+    out = DeviceStorage(view.size, view.storage.dtype, stream=stream)
     lib.call("qmoe_add", parameter.grad.storage.ptr, view.storage.ptr, out.ptr,
              lib.DTYPE_CODES[view.storage.dtype], view.size, stream)
     parameter.grad = Tensor(out, parameter.shape)
@@ -123,10 +124,10 @@ class SparseMoE:
         self.top_k, self.n_experts, self.d_model, self.d_expert = config.top_k, E, d, h
         self.stream = stream
         self.engine = {"auto": lib.ENGINE_AUTO, "simt": lib.ENGINE_SIMT, "tcgen05": lib.ENGINE_TCGEN05}[engine]
-        self._gate = DeviceStorage(E * h * d, "float32")
-        self._up = DeviceStorage(E * h * d, "float32")
-        self._down = DeviceStorage(E * d * h, "float32")
-        router = DeviceStorage(E * d, "float32")
+        self._gate = DeviceStorage(E * h * d, "float32", stream=stream)
+        self._up = DeviceStorage(E * h * d, "float32", stream=stream)
+        self._down = DeviceStorage(E * d * h, "float32", stream=stream)
+        router = DeviceStorage(E * d, "float32", stream=stream)
         down_std = 0.02 / sqrt(2 * config.n_layers)
 
         def fill(storage, std, tensor_seed):
@@ -204,7 +205,7 @@ class SparseMoE:
         A = tokens * k
         R = lib.rows_bound(tokens, E, k)
         blocks = lib.route_blocks(tokens)
-        S = DeviceStorage
+        S = partial(DeviceStorage, stream=self.stream)
         buf = dict(
             probs=S(tokens * E, "float32"), gate_weights=S(A, "float32"), expert_index=S(A, "int32"),
             dest_row=S(A, "int32"), row_source=S(R, "int32"), counts=S(E, "int32"), offsets=S(E + 1, "int32"),
@@ -290,7 +291,7 @@ class SparseMoE:
         tokens = storage.size // self.d_model
         work = self._workspace(tokens, storage.dtype)
         layer, buf = work["layer"], work["buf"]
-        out = DeviceStorage(storage.size, storage.dtype)
+        out = DeviceStorage(storage.size, storage.dtype, stream=self.stream)
         layer.x, layer.out = storage.ptr, out.ptr
         masters = (layer.master_gate, layer.master_up, layer.master_down)
         keep = self._operands_current(work)
@@ -333,7 +334,7 @@ class SparseMoE:
         storage = x.storage if hasattr(x, "storage") else x
         work, _, shape = self._saved
         layer, buf = work["layer"], work["buf"]
-        out = DeviceStorage(storage.size, storage.dtype)   # allocated before the capture starts
+        out = DeviceStorage(storage.size, storage.dtype, stream=self.stream)   # allocated before the capture starts
         lib.call("qmoe_event_sync", self._counts_event)
         layer.x, layer.out = storage.ptr, out.ptr
         masters = (layer.master_gate, layer.master_up, layer.master_down)
@@ -369,7 +370,7 @@ class SparseMoE:
         ga = None if grad_aux is None else (grad_aux.storage if hasattr(grad_aux, "storage") else grad_aux)
         views = work["grad_views"]
         self._release_aliased_gradients(work)
-        dx = DeviceStorage(x_storage.size, x_storage.dtype)
+        dx = DeviceStorage(x_storage.size, x_storage.dtype, stream=self.stream)
         layer.grad_out, layer.grad_aux, layer.dx = g.ptr, 0 if ga is None else ga.ptr, dx.ptr
         lib.call("qmoe_layer_backward", ctypes.byref(layer), self.stream)
         # which experts get a gradient object is host logic on the forward's counts; they are read only
@@ -388,13 +389,13 @@ class SparseMoE:
         ga = grad_aux.storage if hasattr(grad_aux, "storage") else grad_aux
         tokens, d, E = x_storage.size // self.d_model, self.d_model, self.n_experts
         code = lib.DTYPE_CODES[x_storage.dtype]
-        d_router = DeviceStorage(E * d, "float32")
-        dx32 = DeviceStorage(tokens * d, "float32")
+        d_router = DeviceStorage(E * d, "float32", stream=self.stream)
+        dx32 = DeviceStorage(tokens * d, "float32", stream=self.stream)
         lib.call("qmoe_route_backward", ctypes.byref(layer.route), 0, ga.ptr, buf["d_scores"].ptr, self.stream)
         lib.call("qmoe_router_backward", buf["d_scores"].ptr, x_storage.ptr, code, self.router.weight.storage.ptr,
                  dx32.ptr, d_router.ptr, buf["router_partials"].ptr, tokens, d, E, self.stream)
         if x_storage.dtype == "bfloat16":
-            dx = DeviceStorage(tokens * d, "bfloat16")
+            dx = DeviceStorage(tokens * d, "bfloat16", stream=self.stream)
             lib.call("qmoe_cast_bf16", dx32.ptr, dx.ptr, tokens * d, self.stream)
         else:
             dx = dx32
@@ -453,7 +454,7 @@ class MoEFeedForward:
         if block is None:
             moe = self.ffn
             E, d = moe.n_experts, moe.d_model
-            S = DeviceStorage
+            S = partial(DeviceStorage, stream=moe.stream)
             extra = dict(inverse=S(tokens, "float32"), w_router_folded=S(E * d, "float32"),
                          norm_partials=S(int(lib.load().qmoe_norm_backward_partials(tokens, d)), "float32"))
             block = dict(struct=lib.Block(), extra=extra, work=work)
@@ -476,7 +477,7 @@ class MoEFeedForward:
         work = moe._workspace(tokens, storage.dtype)
         block = self._block(work, tokens)
         layer, buf, struct = work["layer"], work["buf"], block["struct"]
-        out = DeviceStorage(storage.size, storage.dtype)
+        out = DeviceStorage(storage.size, storage.dtype, stream=moe.stream)
         layer.x, layer.out = storage.ptr, out.ptr
         masters = (layer.master_gate, layer.master_up, layer.master_down)
         keep = moe._operands_current(work)
@@ -509,11 +510,11 @@ class MoEFeedForward:
             raise ValueError("grad_out must match the output's size and dtype")
         ga = None if grad_aux is None else (grad_aux.storage if hasattr(grad_aux, "storage") else grad_aux)
         moe._release_aliased_gradients(work)
-        dx = DeviceStorage(x_storage.size, x_storage.dtype)
+        dx = DeviceStorage(x_storage.size, x_storage.dtype, stream=moe.stream)
         layer.x, layer.grad_out, layer.grad_aux, layer.dx = x_storage.ptr, g.ptr, 0 if ga is None else ga.ptr, dx.ptr
         struct.layer = layer
         struct.norm_weight, struct.norm_eps = self.ffn_norm.weight.storage.ptr, self.ffn_norm.eps
-        d_norm = DeviceStorage(moe.d_model, "float32")     # handed out below: a buffer of the block would have to be copied
+        d_norm = DeviceStorage(moe.d_model, "float32", stream=moe.stream)     # handed out below: a buffer of the block would have to be copied
         struct.d_norm_weight = d_norm.ptr
         lib.call("qmoe_block_backward", ctypes.byref(struct), moe.stream)
         views = work["grad_views"]

@@ -31,14 +31,14 @@ _ITEM = "5Q2q2f"       # lib.OptimItem: values, grad, exp_avg, exp_avg_sq, shado
 class _Table:
     """Host item array plus the device buffer it is copied into, grown on demand."""
 
-    def __init__(self):
-        self.capacity, self.items, self.device = 0, None, None
+    def __init__(self, stream):
+        self.capacity, self.items, self.device, self.stream = 0, None, None, stream
 
     def fill(self, rows):
         if len(rows) > self.capacity:
             self.capacity = max(64, 2 * len(rows))
             self.items = (lib.OptimItem * self.capacity)()
-            self.device = DeviceStorage(int(lib.load().qmoe_optim_table_bytes(self.capacity)) // 4, "int32")
+            self.device = DeviceStorage(int(lib.load().qmoe_optim_table_bytes(self.capacity)) // 4, "int32", stream=self.stream)
         struct.pack_into(_ITEM * len(rows), self.items, 0, *chain.from_iterable(rows))
         return self.items, len(rows), self.device.ptr
 
@@ -53,9 +53,9 @@ def clip_grad_norm(parameters, max_norm=1.0, *, stream=0, scratch=None):
         return 0.0
     if any(g.dtype != "float32" for g in gradients):
         raise ValueError("gradients must be float32")
-    table = _Table()
+    table = _Table(stream)
     items, count, device = table.fill([(0, g.storage.ptr, 0, 0, 0, g.storage.size, 0, 1.0, 1.0) for g in gradients])
-    scratch = scratch or DeviceStorage(int(lib.load().qmoe_clip_scratch_bytes()) // 4, "int32")
+    scratch = scratch or DeviceStorage(int(lib.load().qmoe_clip_scratch_bytes()) // 4, "int32", stream=stream)
     lib.call("qmoe_clip_grad_norm", items, count, device, float(max_norm), scratch.ptr, stream)
     host = (ctypes.c_double * 2)()
     lib.call("qmoe_memcpy_d2h", ctypes.cast(host, ctypes.c_void_p), scratch.ptr, 16, stream)
@@ -109,7 +109,7 @@ class AdamW:
         self.shadows = dict(shadows or {})
         self.stream = stream
         self.steps, self.averages, self.square_averages = {}, {}, {}
-        self._table = _Table()
+        self._table = _Table(self.stream)
 
     def zero_grad(self):
         for parameter in self.parameters:

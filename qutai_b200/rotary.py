@@ -61,10 +61,10 @@ def _describe(q, k, q_weight, k_weight, heads, kv_heads, eps, theta, starts, off
     return a, dtype, dim
 
 
-def outputs(given, wanted):
-    """``given`` storages, checked against ``wanted`` [(size, dtype), ...], or new ones."""
+def outputs(given, wanted, stream):
+    """``given`` storages, checked against ``wanted`` [(size, dtype), ...], or new ones for ``stream``."""
     if given is None:
-        return tuple(DeviceStorage(size, dtype) for size, dtype in wanted)
+        return tuple(DeviceStorage(size, dtype, stream=stream) for size, dtype in wanted)
     given = tuple(given)
     if len(given) != len(wanted) or any(s.size != size or s.dtype != dtype for s, (size, dtype) in zip(given, wanted)):
         raise ValueError("out must be storages of " + ", ".join(f"{size} x {dtype}" for size, dtype in wanted))
@@ -77,7 +77,7 @@ def norm_rope_forward(q, k, q_weight, k_weight, heads, kv_heads, *, eps=1e-6, th
     storages of the normalised, rotated queries and keys (dense); ``out``: two storages to write to instead of new ones."""
     a, dtype, dim = _describe(q, k, q_weight, k_weight, heads, kv_heads, eps, theta, starts, offset)
     rows = a.batch * a.time
-    q_out, k_out = outputs(out, ((rows * heads * dim, dtype), (rows * kv_heads * dim, dtype)))
+    q_out, k_out = outputs(out, ((rows * heads * dim, dtype), (rows * kv_heads * dim, dtype)), stream)
     a.q_out, a.k_out = q_out.ptr, k_out.ptr
     lib.call("qmoe_norm_rope_forward", ctypes.byref(a), stream)
     return q_out, k_out
@@ -93,8 +93,8 @@ def norm_rope_backward(grad_q, grad_k, q, k, q_weight, k_weight, heads, kv_heads
     gradients = [getattr(g, "storage", g) for g in (grad_q, grad_k)]
     if any(g.size != size or g.dtype != dtype for g, (size, dtype) in zip(gradients, wanted)):
         raise ValueError("the gradients must have the sizes and the dtype of the forward's outputs")
-    results = outputs(out, (*wanted, (dim, "float32"), (dim, "float32")))
-    partials = DeviceStorage(int(lib.load().qmoe_norm_rope_partials(a.batch, a.time, heads, kv_heads, dim)), "float32")
+    results = outputs(out, (*wanted, (dim, "float32"), (dim, "float32")), stream)
+    partials = DeviceStorage(int(lib.load().qmoe_norm_rope_partials(a.batch, a.time, heads, kv_heads, dim)), "float32", stream=stream)
     a.grad_q, a.grad_k = (g.ptr for g in gradients)
     a.dq, a.dk, a.d_q_weight, a.d_k_weight = (s.ptr for s in results)
     a.partials = partials.ptr

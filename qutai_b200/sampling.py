@@ -33,7 +33,7 @@ def sample(logits, uniforms, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, 
             raise ValueError(f"{name} must be a number or hold one {dtype} value for each row")
         else:
             setattr(a, name + "s", value.ptr)
-    tokens, log_probs = outputs(out, ((rows, "int64"), (rows, "float32")))
+    tokens, log_probs = outputs(out, ((rows, "int64"), (rows, "float32")), stream)
     a.tokens, a.log_probs = tokens.ptr, log_probs.ptr
     lib.call("qmoe_sample", ctypes.byref(a), stream)
     return tokens, log_probs

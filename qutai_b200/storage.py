@@ -12,6 +12,10 @@ Every storage carries a ``generation`` counter that the host-visible write paths
 parent's counter.  A reader that keeps something derived from the contents (the layer's bf16 operand
 copies of the fp32 weights) compares generations instead of rebuilding it on every use.  Code that
 writes through the raw ``ptr`` calls ``touch()`` afterwards.
+
+A released block is kept for reuse while kernels that use it may still be running, so it goes to storages of the
+same ``stream`` alone, whose work comes behind those kernels.  A storage used on another stream than
+the one it was made for has to be held until that use is over.
 """
 from __future__ import annotations
 
@@ -23,7 +27,7 @@ from array import array
 from . import lib
 
 _FORMATS = {"int8": "b", "float32": "f", "float64": "d", "int32": "i", "int64": "q"}
-_cache: dict[int, list[int]] = {}
+_cache: dict[tuple[int, int], list[int]] = {}      # (stream, size of the block): released blocks
 _cached_bytes = 0
 # Freed blocks are kept for reuse up to this many bytes (a B200 has 180 GB; activations and gradients of the
 # benchmark shapes are hundreds of MB each, and a block that is really freed costs a device-wide synchronisation:
@@ -32,16 +36,16 @@ _cached_bytes = 0
 CACHE_LIMIT_BYTES = int(os.environ.get("QUTAI_MOE_CACHE_BYTES", 64 << 30))
 
 
-def _allocate(nbytes):
+def _allocate(nbytes, stream):
     global _cached_bytes
     step = 512 if nbytes < (1 << 16) else 1 << 16
     size = (nbytes + step - 1) // step * step or step
-    free = _cache.get(size)
+    free = _cache.get((stream, size))
     if free:
         _cached_bytes -= size
         address = free.pop()
         if not free:
-            del _cache[size]
+            del _cache[stream, size]
         return address, size
     address = ctypes.c_uint64()
     try:
@@ -52,7 +56,7 @@ def _allocate(nbytes):
     return address.value, size
 
 
-def _release(address, size):
+def _release(address, size, stream):
     """Keep the block for reuse.  Over the limit the blocks that have waited longest go first (the one just released
     is the likeliest to be asked for again: a gradient buffer of the next step)."""
     global _cached_bytes
@@ -60,15 +64,15 @@ def _release(address, size):
         lib.load().qmoe_free(address)
         return
     while _cached_bytes + size > CACHE_LIMIT_BYTES and _cache:
-        oldest = next(iter(_cache))            # dicts keep insertion order: the size that entered the cache first
+        oldest = next(iter(_cache))            # dicts keep insertion order: the stream and size that entered the cache first
         blocks = _cache[oldest]
         lib.load().qmoe_free(blocks.pop(0))
-        _cached_bytes -= oldest
+        _cached_bytes -= oldest[1]
         if not blocks:
             del _cache[oldest]
-    free = _cache.get(size)
+    free = _cache.get((stream, size))
     if free is None:
-        _cache[size] = [address]
+        _cache[stream, size] = [address]
     else:
         free.append(address)
     _cached_bytes += size
@@ -95,7 +99,8 @@ def bf16_bits(value):
 class DeviceStorage:
     device = "cuda"
 
-    def __init__(self, size, dtype="float32", *, ptr=None, owner=None):
+    def __init__(self, size, dtype="float32", *, ptr=None, owner=None, stream=0):
+        """``stream``: the one whose work uses the storage, if it is made here (see the module's docstring)."""
         item = lib.ITEM_BYTES.get(dtype)
         if item is None:
             raise ValueError(f"unsupported dtype {dtype!r}")
@@ -111,7 +116,8 @@ class DeviceStorage:
         self._generation = 0
         self._synced = {}          # id(source root) -> generation of the source this storage was last derived from
         if ptr is None:
-            self.ptr, self._block = _allocate(self.nbytes)
+            self._stream = stream
+            self.ptr, self._block = _allocate(self.nbytes, stream)
         else:
             self.ptr = int(ptr)
 
@@ -119,7 +125,7 @@ class DeviceStorage:
         block, self._block = getattr(self, "_block", None), None
         if block is not None:
             try:
-                _release(self.ptr, block)
+                _release(self.ptr, block, self._stream)
             except Exception:
                 pass
 
@@ -161,7 +167,7 @@ class DeviceStorage:
 
     @classmethod
     def zeros(cls, size, dtype="float32", stream=0):
-        out = cls(size, dtype)
+        out = cls(size, dtype, stream=stream)
         out.fill_zero(stream)
         return out
 
@@ -170,7 +176,7 @@ class DeviceStorage:
         item = lib.ITEM_BYTES[dtype]
         if len(data) % item:
             raise ValueError("byte length is not a multiple of the item size")
-        out = cls(len(data) // item, dtype)
+        out = cls(len(data) // item, dtype, stream=stream)
         out.upload_bytes(data, stream)
         return out
 
@@ -227,7 +233,7 @@ class DeviceStorage:
         return out.tolist()
 
     def copy(self, stream=0):
-        out = DeviceStorage(self.size, self.dtype)
+        out = DeviceStorage(self.size, self.dtype, stream=stream)
         lib.call("qmoe_memcpy_d2d", out.ptr, self.ptr, self.nbytes, stream)
         return out
 
