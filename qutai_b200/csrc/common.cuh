@@ -4,6 +4,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <mutex>
+
 #include "../../include/qutai_moe.h"
 
 namespace qmoe {
@@ -97,14 +99,18 @@ inline void chained(void (*kernel)(Parameters...), dim3 grid, dim3 block, size_t
     (void)cudaLaunchKernelEx(&config, kernel, arguments...);
 }
 
-// Dynamic shared memory beyond 48 KB, asked for once per kernel and device (about a microsecond a call).
+// Dynamic shared memory beyond 48 KB, asked for once per kernel and device (about a microsecond a call).  A limit only ever grows: between host threads
+// that ask for different amounts the setting and the note of it are one step.
 template <auto Kernel> inline cudaError_t allow_shared(int bytes) {
+    static std::mutex mutex;
     static int allowed[64] = {};
     int device = 0;
     if (cudaError_t code = cudaGetDevice(&device)) return code;
-    if (device < 64 && allowed[device] >= bytes) return cudaSuccess;
+    if (device >= 64) return cudaErrorInvalidDevice;
+    const std::lock_guard<std::mutex> lock(mutex);
+    if (allowed[device] >= bytes) return cudaSuccess;
     const cudaError_t code = cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-    if (code == cudaSuccess && device < 64) allowed[device] = bytes;
+    if (code == cudaSuccess) allowed[device] = bytes;
     return code;
 }
 
