@@ -236,7 +236,8 @@ norm_rope_backward_kernel(const __grid_constant__ NormRopeParams p) {
                 unpack8<T>(raw_g[u], g);
 #pragma unroll
                 for (int i = 0; i < 8; ++i) square = fmaf(x[i], x[i], square);
-                const float inverse = rsqrtf(head_sum<BITS>(square, p.lane_bits) * p.one_over_dim + p.eps);
+                const float mean = head_sum<BITS>(square, p.lane_bits) * p.one_over_dim + p.eps;
+                const float inverse = h >= 0 ? rsqrtf(mean) : 0.f;       // a place without a head has zeros, and 0 / sqrt(0) were eps zero
                 me.weight(at + u, w);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {          // turned back
