@@ -57,19 +57,23 @@ class Generator:
         return block.feed_forward(Tensor(middle, (rows, block.width)))[0].storage
 
     def prefill(self, prompt):
-        """Run ``prompt`` (token ids) and keep its keys and values as the prefix.  Returns the logits [1, vocab] behind its last token."""
+        """Run ``prompt`` (token ids) and keep its keys and values as the prefix; the continuations of a prompt before it are gone, and ``start`` makes
+        room for new ones.  Returns the logits [1, vocab] behind its last token."""
         tokens, c = [int(t) for t in prompt], self.decoder.config
         if not tokens or any(not 0 <= t < c.vocab_size for t in tokens):
             raise ValueError("the prompt must be a non-empty list of token ids")
         time, width = len(tokens), c.d_model
-        self.prefix = self._cache(1, time)
+        self.prefix = self.caches = None        # until all blocks have run there is nothing to go on from
+        held = self._cache(1, time)
         x = self._embedded(DeviceStorage.from_bytes(array("q", tokens).tobytes(), "int64", self.stream), time)
-        for block, prefix in zip(self.decoder.blocks, self.prefix):
+        for block, prefix in zip(self.decoder.blocks, held):
             normed, _ = _rms_norm(x, block.attn_norm, time, width, self.stream)
             y, (_, _, k, v, *_) = block.attn.forward(normed, 1, time)
             prefix.append(k, v)
             x = self._feed_forward(block, x, y, time)
-        return self._logits(x.view((time - 1) * width, width), 1)
+        logits = self._logits(x.view((time - 1) * width, width), 1)
+        self.prefix = held
+        return logits
 
     def start(self, batch, new_tokens):
         """Empty caches for ``batch`` continuations of up to ``new_tokens`` positions each."""
