@@ -101,12 +101,13 @@ class KVCache:
         return Tensor(k, shape), Tensor(v, shape)
 
 
-def prefix_attention(q, heads, cache, prefix=None, *, out=None, stream=0):
+def prefix_attention(q, heads, cache, prefix=None, *, out=None, stream=None):
     """``q`` [batch, time, heads * dim] (bfloat16), the queries of the last ``time`` positions of every sequence of ``cache``, whose keys
     and values are in it already: query ``t`` sees all of ``prefix`` (a ``KVCache`` of batch 1, or none) and the first
     ``length - time + t + 1`` positions of its own sequence.  Returns ``(out, lse)``, storages of bfloat16 [batch * time * heads * dim] and float32
     [batch * time * heads]; a query that sees nothing gives zeros and -infinity, one with a score that is NaN or +infinity NaN.  Head
-    width 64 or 128."""
+    width 64 or 128.  ``stream``: by default the cache's, behind what was appended to it."""
+    stream = cache.stream if stream is None else stream
     if len(q.shape) != 3 or q.shape[0] != cache.batch or heads <= 0 or q.shape[2] != heads * cache.dim:
         raise ValueError("q must be [batch, time, heads * dim] with the batch and head width of the cache")
     if q.storage.dtype != "bfloat16":
