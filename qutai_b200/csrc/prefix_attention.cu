@@ -113,6 +113,16 @@ template <int DIM, bool INT8, bool A, bool B> constexpr int shared_of() {
 
 // of the threads that attend, in whatever block
 __device__ __forceinline__ void attend_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kThreads) : "memory"); }
+__device__ __forceinline__ bool attend_any(bool mine) {
+    uint32_t any;
+    asm volatile("{\n\t.reg .pred one, all;\n\tsetp.ne.u32 one, %1, 0;\n\tbarrier.cta.red.or.pred all, 1, %2, one;\n\tselp.u32 %0, 1, 0, all;\n\t}"
+                 : "=r"(any) : "r"((uint32_t)mine), "n"(kThreads) : "memory");
+    return any != 0;
+}
+// Of two bf16 numbers those that are NaN or an infinity, all bits of a half set for one that is
+__device__ __forceinline__ uint32_t not_finite(uint32_t v) {
+    return ((v & 0x7f80u) == 0x7f80u ? 0xffffu : 0u) | ((v & 0x7f800000u) == 0x7f800000u ? 0xffff0000u : 0u);
+}
 
 // Rows of a tile: 16 to a warp (BY_KEYS false: 64 rows, every warp walks all keys) or the same 16 for all warps (BY_KEYS: a
 // quarter of every tile of keys each, joined at the end), for the few rows of one sequence.
@@ -156,6 +166,9 @@ __device__ __forceinline__ void attend(const PrefixParams& p, const Keys& keys, 
     int limit[2];                        // keys that the two rows see
 #pragma unroll
     for (int i = 0; i < 2; ++i) limit[i] = at[i] < 0 ? 0 : own ? min(end, length - p.time + step[i] + 1) : end;
+    // A key from `hidden` on is not seen by every row of the tile.  Its probability is zero there, but zero times a NaN or an infinity is not: such values
+    // are taken out of the tiles that hold hidden keys.  (Behind `end` lie zeros.)
+    const int earliest = length - p.time + row_tile * ROWS / p.group + 1, hidden = own && p.time > 1 && earliest < end ? earliest : 0x7fffffff;
 
     const uint32_t base = smem_u32(smem);
     const long long head = ((own ? (long long)b * p.kv_heads : 0) + g) * keys.capacity;
@@ -276,6 +289,45 @@ __device__ __forceinline__ void attend(const PrefixParams& p, const Keys& keys, 
                 l[i] += p0 + p1;
                 s[n][2 * i] = INT8 ? p0 * vs.x : p0;
                 s[n][2 * i + 1] = INT8 ? p1 * vs.y : p1;
+            }
+        }
+        if (begin + (j + 1) * KEYS > hidden) {         // for all threads alike
+            if constexpr (INT8) {                      // the numbers are finite, their scale may not be
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (first + 8 * n + 2 * t4 + (i & 1) >= limit[i >> 1]) s[n][i] = 0.f;
+            } else {
+                uint8_t* const values = smem + (v_tile - base);
+                auto each = [&](auto use) __attribute__((always_inline)) {
+#pragma unroll 1
+                    for (int i = threadIdx.x; i < KEYS * (L::kRowBytes / 16); i += kThreads)
+                        use(*reinterpret_cast<uint4*>(values + i / (L::kRowBytes / 16) * L::kPitch + i % (L::kRowBytes / 16) * 16));
+                };
+                uint32_t mine = 0;
+                each([&](const uint4& v) { mine |= not_finite(v.x) | not_finite(v.y) | not_finite(v.z) | not_finite(v.w); });
+                if (attend_any(mine != 0)) {
+                    // to the rows that see one it goes as it is, whatever its probability
+#pragma unroll 1
+                    for (int key = 0; key < NT * 8; ++key) {
+                        const uint32_t row = v_tile + (key0 + key) * L::kPitch + 4 * t4;
+#pragma unroll
+                        for (int c = 0; c < COLS; ++c) {
+                            const uint32_t v = load_shared(row + 16 * c), which = not_finite(v);
+                            if (!which) continue;
+#pragma unroll
+                            for (int i = 0; i < 2; ++i) {
+                                if (first + key >= limit[i]) continue;
+                                if (which & 0xffffu) o[c][2 * i] += __uint_as_float(v << 16);
+                                if (which >> 16) o[c][2 * i + 1] += __uint_as_float(v & 0xffff0000u);
+                            }
+                        }
+                    }
+                    attend_sync();       // all warps have looked
+                    if (mine) each([&](uint4& v) { v.x &= ~not_finite(v.x); v.y &= ~not_finite(v.y); v.z &= ~not_finite(v.z); v.w &= ~not_finite(v.w); });
+                    attend_sync();
+                }
             }
         }
 #pragma unroll
