@@ -596,7 +596,7 @@ int qmoe_prefix_attention(const qmoe_prefix_attention_t* attention, const qmoe_c
  * exp((logit - largest) / temperature), held as a whole number of 2^-31 (a weight below 2^-32 of the largest is none), so that sums
  * do not depend on their order.  Kept are the top_k largest logits (0 or at least vocab: all; of equal ones those of lower
  * index), of these the shortest run from the largest that holds top_p of their weight, of these the ones of at least
- * min_p times the largest's weight; the token is the first at which the running sum of the kept weights, by index, passes
+ * min_p times the largest's weight (a row's own min_p that is NaN lets all pass); the token is the first at which the running sum of the kept weights, by index, passes
  * uniform * their sum.  Temperature 0 (and whatever is not above it): the first of the largest.  NaN logits count as -infinity; a row without
  * another gives token -1.  log_prob: of the token among ALL of the row's at its temperature (at 1 for temperature 0).
  * ------------------------------------------------------------------------------------------- */

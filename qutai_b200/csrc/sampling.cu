@@ -259,7 +259,8 @@ sample_kernel(const __grid_constant__ SampleParams p) {
         }
     }
     const float temperature = p.temperatures ? p.temperatures[row] : p.temperature;
-    const float top_p = p.top_ps ? p.top_ps[row] : p.top_p, min_p = fminf(p.min_ps ? p.min_ps[row] : p.min_p, 1.f);
+    const float top_p = p.top_ps ? p.top_ps[row] : p.top_p, given_min = p.min_ps ? p.min_ps[row] : p.min_p;
+    const float min_p = given_min > 1.f ? 1.f : given_min;       // NaN stays: no weight is below it
     const bool greedy = !(temperature > 0.f);
     const float inverse = greedy ? 1.f : __fdiv_rn(1.f, temperature);
     const int top_k = greedy ? 1 : p.top_ks ? p.top_ks[row] : p.top_k;
