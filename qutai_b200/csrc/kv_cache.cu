@@ -148,8 +148,11 @@ CacheParams cache_params(const qmoe_cache_t* c) {
     return p;
 }
 
-template <bool APPEND> int launch(CacheParams& p, const qmoe_cache_t* c, long long units, int dtype, cudaStream_t stream) {
-    if (units > 0x7fffffff / kThreads) return fail_arg("cache: too many positions in one call");
+template <bool APPEND> int launch(CacheParams& p, const qmoe_cache_t* c, long long positions, int dtype, cudaStream_t stream) {
+    // (the kernels number the heads of positions in 32 bits, with a block's worth of room behind the last)
+    if (positions > 0x7fffffffll / c->batch || positions * c->batch > 0x7fffffffll / c->kv_heads)
+        return fail_arg("cache: more than 2147483647 heads of positions in one call");
+    const long long units = c->batch * positions * c->kv_heads;
     p.units = (unsigned)units;
     const dim3 grid((unsigned)ceil_div(units, kThreads >> p.lane_bits), 2);
     auto go = [&](auto value, auto int8, auto values) {
@@ -209,7 +212,7 @@ extern "C" int qmoe_cache_append(const qmoe_cache_t* c, uint64_t k, uint64_t v, 
     CacheParams p = cache_params(c);
     p.k_in = (const void*)k; p.v_in = (const void*)v; p.k_pitch = k_pitch; p.v_pitch = v_pitch;
     p.counts = (const int*)counts; p.lengths_out = (int*)lengths_out; p.time = (int)time;
-    return launch<true>(p, c, c->batch * time * c->kv_heads, dtype, stream);
+    return launch<true>(p, c, time, dtype, stream);
 }
 
 extern "C" int qmoe_cache_read(const qmoe_cache_t* c, int64_t start, int64_t count, uint64_t k_out, uint64_t v_out, int32_t dtype, uint64_t stream_) {
@@ -222,5 +225,5 @@ extern "C" int qmoe_cache_read(const qmoe_cache_t* c, int64_t start, int64_t cou
     TimedScope timed(KC_ELEMENTWISE, stream);
     CacheParams p = cache_params(c);
     p.k_read = (void*)k_out; p.v_read = (void*)v_out; p.start = start; p.count = count;
-    return launch<false>(p, c, c->batch * count * c->kv_heads, dtype, stream);
+    return launch<false>(p, c, count, dtype, stream);
 }
