@@ -566,7 +566,7 @@ typedef struct qmoe_cache {
     uint64_t lengths;                    /* i32 [batch], read on the device */
 } qmoe_cache_t;
 /* Rows [b, t < counts[b]] of k and v ([batch, time, kv_heads, dim], rows `pitch` elements apart; counts i32 [batch], 0: time) go to positions
- * lengths[b] + t, and lengths_out[b] = lengths[b] + counts[b].  lengths_out is another buffer than lengths.  What would
+ * lengths[b] + t, and lengths_out[b] = lengths[b] + counts[b].  lengths_out is another buffer than lengths and counts.  What would
  * lie behind `capacity` is dropped, and lengths_out[b] ends there.  batch * time * kv_heads up to 2^31 - 1 in a call, of qmoe_cache_read batch * count * kv_heads. */
 int qmoe_cache_append(const qmoe_cache_t* cache, uint64_t k, uint64_t v, int32_t dtype, int64_t k_pitch, int64_t v_pitch, int64_t time,
                       uint64_t counts, uint64_t lengths_out, uint64_t stream);

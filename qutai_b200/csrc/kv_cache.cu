@@ -198,7 +198,9 @@ extern "C" int qmoe_cache_append(const qmoe_cache_t* c, uint64_t k, uint64_t v, 
     if (dtype != QMOE_F32 && dtype != QMOE_BF16) return fail_arg("cache_append: dtype must be QMOE_F32 or QMOE_BF16");
     if (time < 0 || time > c->capacity) return fail_arg("cache_append: time must lie between 0 and the capacity");
     if (!lengths_out || lengths_out & 3u || counts & 3u) return fail_arg("cache_append: null or misaligned lengths");
-    if (lengths_out == c->lengths) return fail_arg("cache_append: the new lengths need a buffer of their own");
+    // blocks read the old lengths and the counts while others write the new lengths
+    auto overlaps = [&](uint64_t read) { return read && read < lengths_out + c->batch * sizeof(int) && lengths_out < read + c->batch * sizeof(int); };
+    if (overlaps(c->lengths) || overlaps(counts)) return fail_arg("cache_append: the new lengths need a buffer of their own");
     cudaStream_t stream = (cudaStream_t)stream_;
     if (!time) {
         QMOE_CUDA(cudaMemcpyAsync((void*)lengths_out, (const void*)c->lengths, c->batch * sizeof(int), cudaMemcpyDeviceToDevice, stream));
