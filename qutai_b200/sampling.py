@@ -28,7 +28,8 @@ def sample(logits, uniforms, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, 
     a = lib.Sample(rows, vocab, lib.DTYPE_CODES[logits.storage.dtype], 0, 1.0, 1.0, 0.0, 0.0, logits.storage.ptr, uniforms.ptr)
     for name, value, dtype in (("temperature", temperature, "float32"), ("top_k", top_k, "int32"), ("top_p", top_p, "float32"), ("min_p", min_p, "float32")):
         if not hasattr(value, "ptr"):
-            setattr(a, name, value)
+            # (the field holds 32 bits: a count beyond the vocabulary is all of it, a negative one is refused whatever its size)
+            setattr(a, name, max(-1, min(value, vocab)) if name == "top_k" else value)
         elif value.dtype != dtype or value.size != rows:
             raise ValueError(f"{name} must be a number or hold one {dtype} value for each row")
         else:
