@@ -527,6 +527,7 @@ int qmoe_attention_backward(const qmoe_attention_t* attention, uint64_t stream);
  *     y = R(p) (w * x / sqrt(mean(x^2) + eps)),   p = offset + starts[b] + t,
  * R(p) turning the pairs (2 i, 2 i + 1) by p theta^(-2 i / dim) as qmoe_rope does; one weight for the query heads, one for the key
  * heads.  Any number of rows, none included; dim a multiple of 8 up to 256; rows may lie `pitch` elements apart (a fused projection's output).
+ * An output may be its own operand (q_out q, k_out k, dq q or grad_q, dk k or grad_k) where that is dense, and overlaps no operand else.
  * ------------------------------------------------------------------------------------------- */
 typedef struct qmoe_norm_rope {
     int64_t batch, time;

@@ -359,6 +359,21 @@ int norm_rope_check(const qmoe_norm_rope_t* a, bool backward) {
     const long long align = a->dtype == QMOE_BF16 ? 8 : 4;
     if (a->q_pitch % align || a->k_pitch % align || a->q_pitch < (long long)a->heads * a->dim || a->k_pitch < (long long)a->kv_heads * a->dim)
         return fail_arg("norm_rope: a row pitch must be a multiple of 16 bytes and not below the row's width");
+    // A lane writes where it has read or somewhere else altogether: rows of another pitch, or of the other heads, would be written before they are read
+    struct Span { uint64_t at, bytes; };
+    const uint64_t item = a->dtype == QMOE_BF16 ? 2 : 4, rows = (uint64_t)a->batch * (uint64_t)a->time;
+    const uint64_t widths[2] = {(uint64_t)a->heads * a->dim, (uint64_t)a->kv_heads * a->dim}, pitches[2] = {(uint64_t)a->q_pitch, (uint64_t)a->k_pitch};
+    const uint64_t in[2] = {a->q, a->k}, grad[2] = {a->grad_q, a->grad_k}, out[2] = {backward ? a->dq : a->q_out, backward ? a->dk : a->k_out};
+    auto dense = [&](const uint64_t* of, int i) { return Span{of[i], rows * widths[i] * item}; };
+    auto overlap = [](const Span& x, const Span& y) { return x.at < y.at + y.bytes && y.at < x.at + x.bytes; };
+    bool apart = !rows || !overlap(dense(out, 0), dense(out, 1));
+    for (int i = 0; rows && i < 2; ++i)
+        for (int j = 0; j < 2; ++j) {
+            const Span read = {in[j], ((rows - 1) * pitches[j] + widths[j]) * item};
+            apart = apart && ((i == j && out[i] == in[j] && pitches[j] == widths[j]) || !overlap(dense(out, i), read));
+            if (backward) apart = apart && ((i == j && out[i] == grad[j]) || !overlap(dense(out, i), dense(grad, j)));
+        }
+    if (!apart) return fail_arg("norm_rope: an output may lie on its own operand, row on row, and on no other");
     return 0;
 }
 
