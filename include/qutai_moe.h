@@ -584,7 +584,7 @@ typedef struct qmoe_prefix_attention {
     int32_t reserved;
     int64_t prefix_longest, longest;     /* bounds on the prefix's length and on the sequences', known to the host */
     uint64_t q;                          /* [batch, time, heads, dim] */
-    uint64_t out;                        /* like q */
+    uint64_t out;                        /* like q, in another buffer */
     uint64_t lse;                        /* f32 [batch, time, heads] */
     uint64_t scratch;                    /* qmoe_prefix_attention_scratch bytes */
 } qmoe_prefix_attention_t;

@@ -44,6 +44,7 @@ struct PrefixParams {
     long long rows;                      // batch * time * heads
     int batch, time, kv_heads, group, slots;
     int prefix_items;
+    int checks;                          // some rows do not see all keys of their sequence (see row_again)
     float scale;                         // 1 / sqrt(dim)
 };
 
@@ -113,16 +114,6 @@ template <int DIM, bool INT8, bool A, bool B> constexpr int shared_of() {
 
 // of the threads that attend, in whatever block
 __device__ __forceinline__ void attend_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kThreads) : "memory"); }
-__device__ __forceinline__ bool attend_any(bool mine) {
-    uint32_t any;
-    asm volatile("{\n\t.reg .pred one, all;\n\tsetp.ne.u32 one, %1, 0;\n\tbarrier.cta.red.or.pred all, 1, %2, one;\n\tselp.u32 %0, 1, 0, all;\n\t}"
-                 : "=r"(any) : "r"((uint32_t)mine), "n"(kThreads) : "memory");
-    return any != 0;
-}
-// Of two bf16 numbers those that are NaN or an infinity, all bits of a half set for one that is
-__device__ __forceinline__ uint32_t not_finite(uint32_t v) {
-    return ((v & 0x7f80u) == 0x7f80u ? 0xffffu : 0u) | ((v & 0x7f800000u) == 0x7f800000u ? 0xffff0000u : 0u);
-}
 
 // Rows of a tile: 16 to a warp (BY_KEYS false: 64 rows, every warp walks all keys) or the same 16 for all warps (BY_KEYS: a
 // quarter of every tile of keys each, joined at the end), for the few rows of one sequence.
@@ -166,9 +157,6 @@ __device__ __forceinline__ void attend(const PrefixParams& p, const Keys& keys, 
     int limit[2];                        // keys that the two rows see
 #pragma unroll
     for (int i = 0; i < 2; ++i) limit[i] = at[i] < 0 ? 0 : own ? min(end, length - p.time + step[i] + 1) : end;
-    // A key from `hidden` on is not seen by every row of the tile.  Its probability is zero there, but zero times a NaN or an infinity is not: such values
-    // are taken out of the tiles that hold hidden keys.  (Behind `end` lie zeros.)
-    const int earliest = length - p.time + row_tile * ROWS / p.group + 1, hidden = own && p.time > 1 && earliest < end ? earliest : 0x7fffffff;
 
     const uint32_t base = smem_u32(smem);
     const long long head = ((own ? (long long)b * p.kv_heads : 0) + g) * keys.capacity;
@@ -289,45 +277,6 @@ __device__ __forceinline__ void attend(const PrefixParams& p, const Keys& keys, 
                 l[i] += p0 + p1;
                 s[n][2 * i] = INT8 ? p0 * vs.x : p0;
                 s[n][2 * i + 1] = INT8 ? p1 * vs.y : p1;
-            }
-        }
-        if (begin + (j + 1) * KEYS > hidden) {         // for all threads alike
-            if constexpr (INT8) {                      // the numbers are finite, their scale may not be
-#pragma unroll
-                for (int n = 0; n < NT; ++n)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        if (first + 8 * n + 2 * t4 + (i & 1) >= limit[i >> 1]) s[n][i] = 0.f;
-            } else {
-                uint8_t* const values = smem + (v_tile - base);
-                auto each = [&](auto use) __attribute__((always_inline)) {
-#pragma unroll 1
-                    for (int i = threadIdx.x; i < KEYS * (L::kRowBytes / 16); i += kThreads)
-                        use(*reinterpret_cast<uint4*>(values + i / (L::kRowBytes / 16) * L::kPitch + i % (L::kRowBytes / 16) * 16));
-                };
-                uint32_t mine = 0;
-                each([&](const uint4& v) { mine |= not_finite(v.x) | not_finite(v.y) | not_finite(v.z) | not_finite(v.w); });
-                if (attend_any(mine != 0)) {
-                    // to the rows that see one it goes as it is, whatever its probability
-#pragma unroll 1
-                    for (int key = 0; key < NT * 8; ++key) {
-                        const uint32_t row = v_tile + (key0 + key) * L::kPitch + 4 * t4;
-#pragma unroll
-                        for (int c = 0; c < COLS; ++c) {
-                            const uint32_t v = load_shared(row + 16 * c), which = not_finite(v);
-                            if (!which) continue;
-#pragma unroll
-                            for (int i = 0; i < 2; ++i) {
-                                if (first + key >= limit[i]) continue;
-                                if (which & 0xffffu) o[c][2 * i] += __uint_as_float(v << 16);
-                                if (which >> 16) o[c][2 * i + 1] += __uint_as_float(v & 0xffff0000u);
-                            }
-                        }
-                    }
-                    attend_sync();       // all warps have looked
-                    if (mine) each([&](uint4& v) { v.x &= ~not_finite(v.x); v.y &= ~not_finite(v.y); v.z &= ~not_finite(v.z); v.w &= ~not_finite(v.w); });
-                    attend_sync();
-                }
             }
         }
 #pragma unroll
@@ -836,6 +785,76 @@ prefix_tensor_kernel(const __grid_constant__ PrefixTcParams tc) {
     }
 }
 
+// A key that a row does not see has a probability of zero there, but zero times a NaN or an infinity is not.  So, of several new positions, a row that
+// comes out as no numbers, and not by its scores, is done again: by one warp, a key to a lane, as the formula says it, with no value that the row
+// does not see.  What the prefix gave it is taken from its parts.
+template <int DIM>
+__device__ __noinline__ void row_again(const PrefixParams& p, long long row) {
+    const Keys& keys = p.own;
+    const int lane = threadIdx.x & 31, heads = p.kv_heads * p.group, h = (int)(row % heads), b = (int)(row / heads / p.time), step = (int)(row / heads % p.time);
+    const int limit = min(max(keys.lengths[b], 0), keys.longest) - p.time + step + 1;
+    const long long head = ((long long)b * p.kv_heads + h / p.group) * keys.capacity;
+    const bool int8 = keys.k_scale != nullptr;
+    const float scale2 = p.scale * LOG2E;
+    const __nv_bfloat16* const q = p.q + row * DIM;
+    float m = -INFINITY, l = 0.f, o[DIM / 32] = {};
+    auto rescale = [&](float next) {     // returns the base of the exponentials
+        const float from = next == -INFINITY ? 0.f : next, alpha = exp2_fast(m - from);
+        m = next;
+        l *= alpha;
+#pragma unroll
+        for (int c = 0; c < DIM / 32; ++c) o[c] *= alpha;
+        return from;
+    };
+    for (int first = 0; first < limit; first += 32) {
+        const long long key = head + first + lane;
+        const bool sees = first + lane < limit;
+        float score = -INFINITY;
+        if (sees) {
+            score = 0.f;
+            for (int d = 0; d < DIM; ++d)
+                score = fmaf(__bfloat162float(q[d]), int8 ? (float)((const int8_t*)keys.k)[key * DIM + d] : __bfloat162float(((const __nv_bfloat16*)keys.k)[key * DIM + d]), score);
+            score *= int8 ? keys.k_scale[key] * scale2 : scale2;
+        }
+        const float from = rescale(fmaxf(m, warp_max(score))), weight = sees ? exp2_fast(score - from) : 0.f;
+        l += warp_sum(weight);
+        for (int i = 0; i < 32 && first + i < limit; ++i) {
+            const float w = __shfl_sync(0xffffffffu, weight, i) * (int8 ? keys.v_scale[head + first + i] : 1.f);
+#pragma unroll
+            for (int c = 0; c < DIM / 32; ++c) {
+                const long long at = (head + first + i) * DIM + 32 * c + lane;
+                o[c] = fmaf(w, int8 ? (float)((const int8_t*)keys.v)[at] : __bfloat162float(((const __nv_bfloat16*)keys.v)[at]), o[c]);
+            }
+        }
+    }
+    for (int slot = 0; slot < p.prefix.splits; ++slot) {
+        const float2 ml = p.part_ml[slot * p.rows + row];
+        if (ml.y == 0.f) continue;       // saw no key, its values were not written
+        const float weight = exp2_fast(ml.x - rescale(fmaxf(m, ml.x)));
+        l += weight * ml.y;
+#pragma unroll
+        for (int c = 0; c < DIM / 32; ++c) o[c] = fmaf(weight, p.part_o[(slot * p.rows + row) * DIM + 32 * c + lane], o[c]);
+    }
+    const float inverse = l != 0.f ? 1.f / l : 0.f;
+    if (lane == 0) p.lse[row] = l != 0.f ? (m + log2f(l)) * LN2 : -INFINITY;
+#pragma unroll
+    for (int c = 0; c < DIM / 32; ++c) p.out[row * DIM + 32 * c + lane] = __float2bfloat16_rn(o[c] * inverse);
+}
+
+// the same for rows that come in one part: a warp looks at one of them
+template <int DIM>
+__global__ void __launch_bounds__(kThreads)
+prefix_check_kernel(const __grid_constant__ PrefixParams p) {
+    chain_begin();
+    const int lane = threadIdx.x & 31;
+    const long long row = (long long)blockIdx.x * kWarps + (threadIdx.x >> 5);
+    if (row >= p.rows) return;
+    bool odd = false;
+#pragma unroll
+    for (int c = 0; c < DIM / 32; ++c) odd |= !(fabsf(__bfloat162float(p.out[row * DIM + 32 * c + lane])) < INFINITY);
+    if (__any_sync(0xffffffffu, odd) && p.lse[row] == p.lse[row]) row_again<DIM>(p, row);
+}
+
 // The parts of a row: WARPS warps to a row, which take every WARPS-th part, their weights a lane each, eight parts' values on their way together, and
 // meet in shared memory.  One warp to a row, four rows to a block, where that leaves enough warps or there is little to each; else eight: 16 rows in 97
 // parts of 128 values take 26 us with one and 5 with eight, 4096 rows in 10 parts 5 and 12.  What bounds it is the wait for the parts, from L2.
@@ -902,6 +921,10 @@ prefix_join_kernel(const __grid_constant__ PrefixParams p) {
     const float inverse = total != 0.f ? 1.f / total : 0.f;
     if (lane < LANES) *reinterpret_cast<uint2*>(p.out + row * DIM + lane * 4) = make_uint2(pack2(sum.x * inverse, sum.y * inverse), pack2(sum.z * inverse, sum.w * inverse));
     if (lane == 0) p.lse[row] = total != 0.f ? (top + log2f(total)) * LN2 : -INFINITY;
+    if (p.checks && total == total && __any_sync(0xffffffffu, !(fabsf(sum.x) < INFINITY && fabsf(sum.y) < INFINITY && fabsf(sum.z) < INFINITY && fabsf(sum.w) < INFINITY))) {
+        __syncwarp();
+        row_again<DIM>(p, row);
+    }
 }
 
 struct Plan { Keys prefix, own; int slots; long long prefix_items, own_items; bool tensor, together, prefix_by_keys, own_by_keys; };
@@ -947,7 +970,7 @@ Plan plan_of(const qmoe_prefix_attention_t* a, const qmoe_cache_t* c) {
 
 void keys_of(const qmoe_cache_t* c, long long longest, Keys& k) {
     k.k = (const uint8_t*)c->k; k.v = (const uint8_t*)c->v;
-    k.k_scale = (const float*)c->k_scale; k.v_scale = (const float*)c->v_scale;
+    if (c->dtype == QMOE_INT8) { k.k_scale = (const float*)c->k_scale; k.v_scale = (const float*)c->v_scale; }
     k.lengths = (const int*)c->lengths; k.capacity = c->capacity; k.longest = (int)longest;
 }
 
@@ -1008,7 +1031,13 @@ int launch(PrefixParams& p, const Plan& plan, const qmoe_cache_t* prefix, cudaSt
     else if (plan.own_by_keys && (plan.tensor || plan.prefix_by_keys)) rc = go(std::true_type(), std::true_type());
     else if (plan.own_by_keys) rc = go(std::false_type(), std::true_type());
     else rc = go(std::false_type(), std::false_type());
-    if (rc || plan.slots == 1) return rc;
+    if (rc) return rc;
+    if (plan.slots == 1) {
+        if (!p.checks) return 0;
+        chained(prefix_check_kernel<DIM>, (unsigned)((p.rows + kWarps - 1) / kWarps), kThreads, 0, stream, p);
+        QMOE_LAUNCH_CHECK("prefix_check_kernel");
+        return 0;
+    }
     if (plan.slots <= 8 || plan.slots * 32 <= p.rows) chained(prefix_join_kernel<DIM, 1>, (unsigned)((p.rows + kWarps - 1) / kWarps), kThreads, 0, stream, p);
     else chained(prefix_join_kernel<DIM, 8>, (unsigned)p.rows, 256, 0, stream, p);
     QMOE_LAUNCH_CHECK("prefix_join_kernel");
@@ -1046,6 +1075,7 @@ extern "C" int qmoe_prefix_attention(const qmoe_prefix_attention_t* a, const qmo
     p.batch = (int)c->batch; p.time = (int)a->time; p.kv_heads = c->kv_heads; p.group = a->heads / c->kv_heads; p.slots = plan.slots;
     p.prefix_items = (int)plan.prefix_items;
     p.scale = 1.f / sqrtf((float)c->dim);
+    p.checks = a->time > 1 && a->longest > 0 && a->out != a->q;      // (queries that are being written over cannot be read again)
     if (c->dim == 64) return c->dtype == QMOE_INT8 ? launch<64, true>(p, plan, prefix, stream) : launch<64, false>(p, plan, prefix, stream);
     return c->dtype == QMOE_INT8 ? launch<128, true>(p, plan, prefix, stream) : launch<128, false>(p, plan, prefix, stream);
 }
