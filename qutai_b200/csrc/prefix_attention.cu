@@ -281,7 +281,7 @@ __device__ __forceinline__ void attend(const PrefixParams& p, const Keys& keys, 
         }
 #pragma unroll
         for (int ks = 0; ks < NT / 2; ++ks) {
-            // probabilities as two bf16 numbers each, what one leaves in the other: 2^-17 of them is lost, so that the output's own rounding
+            // probabilities as two bf16 numbers each, what one leaves in the other: 2^-16 of them is lost at most, so that the output's own rounding
             // is the only one that shows
             uint32_t a[4], rest[4];
 #pragma unroll
@@ -929,7 +929,7 @@ prefix_join_kernel(const __grid_constant__ PrefixParams p) {
 
 struct Plan { Keys prefix, own; int slots; long long prefix_items, own_items; bool tensor, together, prefix_by_keys, own_by_keys; };
 
-// Chunks of keys: as long as they leave four items to an SM, but not below two tiles.
+// Chunks of keys: as long as they leave four items to an SM, but not below two tiles.  (Two and three items to an SM were not compared with that.)
 Plan plan_of(const qmoe_prefix_attention_t* a, const qmoe_cache_t* c) {
     Plan plan = {};
     const long long group = a->heads / c->kv_heads, own_rows = a->time * group, all_rows = c->batch * own_rows;
@@ -963,7 +963,8 @@ Plan plan_of(const qmoe_prefix_attention_t* a, const qmoe_cache_t* c) {
     plan.prefix_items = prefix_heads * plan.prefix.splits;
     plan.own_items = own_heads * plan.own.splits;
     // One launch for both while the sequences' items are few.  Many of them are better off with a launch of their own, whose blocks are small and
-    // three to four on an SM (128 sequences, 8 heads: 110 us, in one launch 117; 64 sequences, 4 heads: 27, in one launch 24).
+    // three to four on an SM.  In one launch and in two, 4 or 8 key/value heads over prefixes of 1003 to 32768 keys: 78 items 13.6 and 22.8 us, 256 19.7 and 19.2,
+    // 384 16.6 and 17.4, 592 33.0 and 32.8, 800 36.5 and 31.3, 888 37.6 and 31.0, 1024 30.5 and 24.9 (another such 128 and 114).
     plan.together = plan.own_items <= 4ll * sm_count();
     return plan;
 }

@@ -18,7 +18,8 @@ from .storage import DeviceStorage
 class KVCache:
     """Keys and values [batch, kv_heads, capacity, dim].  ``dtype`` "bfloat16" or "int8".  ``lengths`` (int32 [batch], on the device)
     says what each sequence holds; ``longest`` is the host's bound on it, by which the work is cut up: after ``append``
-    with ``counts`` it may lie above every sequence's length, never below.  The buffers are made here unless they are given
+    with ``counts`` it may lie above every sequence's length, never below.  ``append`` and ``read`` run on ``stream``; work on another stream that
+    reads the cache has to be over before the next ``append``, which lets go of the lengths before it.  The buffers are made here unless they are given
     (``k``, ``v``, ``lengths`` and, for int8, ``k_scale``, ``v_scale`` as storages; ``longest`` then says how long they are)."""
 
     def __init__(self, batch, capacity, kv_heads, dim, dtype="bfloat16", *, k=None, v=None, k_scale=None, v_scale=None, lengths=None,
