@@ -164,19 +164,24 @@ def packed_attention_forward(q, k, v, heads, kv_heads, sequences, *, scale=None,
     return result
 
 
-def packed_attention_backward(gradient, q, k, v, out, lse, heads, kv_heads, sequences, *, scale=None, results=None, stream=0):
-    """``gradient``: storage (or tensor) like the forward's ``out``; the other arguments are the forward's, ``out`` and ``lse`` what it returned.  Returns
-    ``(dq, dk, dv)`` as dense storages; ``results``: three storages to write to, whose rows behind the last sequence stay as they are."""
+def packed_attention_backward(gradient, q, k, v, attended, lse, heads, kv_heads, sequences, *, scale=None, out=None, results=None, stream=0):
+    """``gradient``: storage (or tensor) like the forward's output; ``attended`` and ``lse`` are what the forward returned, the other arguments the
+    forward's.  Returns ``(dq, dk, dv)`` as dense storages; ``out``: three storages to write to, whose rows behind the last sequence stay as they are
+    (``results``: another name of it)."""
+    if results is not None:
+        if out is not None:
+            raise ValueError("out and results are two names of the storages to write to")
+        out = results
     a, rows, dim = _describe_packed(q, k, v, heads, kv_heads, sequences, scale)
     gradient = getattr(gradient, "storage", gradient)
     wide, narrow = rows * heads * dim, rows * kv_heads * dim
-    for storage, size, dtype in ((gradient, wide, "bfloat16"), (out, wide, "bfloat16"), (lse, rows * heads, "float32")):
+    for storage, size, dtype in ((gradient, wide, "bfloat16"), (attended, wide, "bfloat16"), (lse, rows * heads, "float32")):
         if storage.size != size or storage.dtype != dtype:
-            raise ValueError("the gradient, out and lse must have the sizes and dtypes of the forward's results")
-    result = _made(results, ((wide, "bfloat16"), (narrow, "bfloat16"), (narrow, "bfloat16")), rows, sequences.rows, stream)
+            raise ValueError("the gradient, attended and lse must have the sizes and dtypes of the forward's results")
+    result = _made(out, ((wide, "bfloat16"), (narrow, "bfloat16"), (narrow, "bfloat16")), rows, sequences.rows, stream)
     if sequences.blocks:
         delta = DeviceStorage(sequences.rows * heads, "float32", stream=stream)
-        a.out, a.lse, a.grad_out, a.delta = out.ptr, lse.ptr, gradient.ptr, delta.ptr
+        a.out, a.lse, a.grad_out, a.delta = attended.ptr, lse.ptr, gradient.ptr, delta.ptr
         a.dq, a.dk, a.dv = (storage.ptr for storage in result)
         lib.call("qmoe_packed_attention_backward", ctypes.byref(a), stream)
         done_with(delta, stream)
