@@ -425,7 +425,7 @@ def run(state):
         out, lse = packed_attention_forward(given["q"], given["k"], given["v"], case["heads"], case["kv_heads"], state["sequences"], out=buffers[:2])
         if case["train"]:
             packed_attention_backward(given["dout"], given["q"], given["k"], given["v"], out, lse, case["heads"], case["kv_heads"], state["sequences"],
-                                      results=buffers[2:])
+                                      out=buffers[2:])
     else:
         head = state["head"]
         head.forward(*state["given"], out=buffers[0])
