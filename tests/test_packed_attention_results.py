@@ -9,10 +9,11 @@ from test_packed_training_arguments import Sequences, storage, tensor
 
 def backward(monkeypatch, **names):
     noted, plan = [], Sequences([60, 40], monkeypatch)
-    monkeypatch.setattr(lib, "call", lambda name, *args: noted.append((name, args)))
-    monkeypatch.setattr(attention, "DeviceStorage", lambda size, dtype, stream=0: storage(size, dtype, 10 << 20))
-    results = packed_attention_backward(storage(12800, ptr=4 << 20), tensor(100, 128), tensor(100, 64, ptr=2 << 20), tensor(100, 64, ptr=3 << 20),
-                                        storage(12800, ptr=5 << 20), storage(200, "float32", 6 << 20), 2, 1, plan, **names)
+    with monkeypatch.context() as m:
+        m.setattr(lib, "call", lambda name, *args: noted.append((name, args)))
+        m.setattr(attention, "DeviceStorage", lambda size, dtype, stream=0: storage(size, dtype, 10 << 20))
+        results = packed_attention_backward(storage(12800, ptr=4 << 20), tensor(100, 128), tensor(100, 64, ptr=2 << 20), tensor(100, 64, ptr=3 << 20),
+                                            storage(12800, ptr=5 << 20), storage(200, "float32", 6 << 20), 2, 1, plan, **names)
     return results, noted
 
 
