@@ -307,9 +307,9 @@ packed_forward_kernel(const __grid_constant__ PackedParams p) {
         const uint32_t lane_base = (uint32_t)(quad * 32) << 16;
         const float scale2 = p.scale * LOG2E;                // in the exponent of 2
         const uint64_t scale_pair = pair2(scale2, scale2);
-        // What is subtracted from scores: the largest so far, or one up to 2^LAG below it in the exponential.  O and the sum are rescaled only when the
+        // What is subtracted from scores: the largest so far, or one up to 2^LAG below it in the exponential (0 while all are -infinity).  O and the sum are rescaled only when the
         // largest score has risen further than that, which ordinary scores do in a row's first blocks alone.
-        float from = 0.f, l = 0.f;
+        float from = -INFINITY, l = 0.f;
         bool ok = true;
         for (int j = 0; ok && j < n; ++j) {
             const uint32_t tmem_s = tmem + (uint32_t)(j & 1) * KEYS + lane_base;
@@ -331,15 +331,16 @@ packed_forward_kernel(const __grid_constant__ PackedParams p) {
             for (int c = 4; c < KEYS; c += 2) peak4[(c >> 1) & 3] = max3(peak4[(c >> 1) & 3], __uint_as_float(s[c]), __uint_as_float(s[c + 1]));
             const float peak = fmaxf(max3(peak4[0], peak4[1], peak4[2]), peak4[3]);
             float alpha = 1.f;
-            if (j == 0) {
-                from = peak == -INFINITY ? 0.f : peak;        // a row may have nothing but -infinity so far
+            if (from == -INFINITY) {                          // nothing above -infinity so far: O and the sum are 0
+                from = peak;
             } else if ((peak - from) * scale2 > LAG) {
                 alpha = exp2_fast((from - peak) * scale2);
                 from = peak;
                 l *= alpha;
             }
+            const float against = from == -INFINITY ? 0.f : from;
             // (subtract, then multiply: a single fma would leave the base rounded, attention.cu)
-            const uint64_t minus = pair2(-from, -from);
+            const uint64_t minus = pair2(-against, -against);
             uint64_t total2[2] = {0, 0};
             uint32_t packed[KEYS / 2];
 #pragma unroll
