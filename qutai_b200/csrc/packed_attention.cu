@@ -194,6 +194,15 @@ __device__ __forceinline__ void release(uint32_t tmem, uint32_t columns) {
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(columns) : "memory");
 }
 
+// The CTA's entry of the table, by one warp beside the set-up of the others.  The kernel before this one may still be writing the table: behind the wait.
+__device__ __forceinline__ void fetch_item(const PackedParams& p, int which, int* to) {
+    chain_wait();
+    if ((threadIdx.x & 31) == 0) {
+        const int4 item = p.items[which];
+        to[0] = item.x; to[1] = item.y; to[2] = item.z;
+    }
+}
+
 // ------------------------------------------------------------------------------------------------
 // forward: a CTA to 128 queries of a head, key blocks of 64 positions.  S has two buffers, P lies over the S that it came from: the next
 // scores are formed while the rows have this block's, and a row waits for nothing but them.
@@ -206,7 +215,7 @@ template <int D> struct Forward {
     static constexpr int TILES = TILE + 2 * STAGES * KV_TILE;
     enum { Q_FULL = 0, K_FULL = 1, K_EMPTY = K_FULL + STAGES, V_FULL = K_EMPTY + STAGES, V_EMPTY = V_FULL + STAGES, S_FULL = V_EMPTY + STAGES, P_FULL = S_FULL + 2, O_DONE = P_FULL + 2, O_LAST, BARS };
     // (P_FULL is two barriers, by the parity of the block: a warp may have the next block's scores, and be done with them, before another one is done with this block's)
-    static constexpr int SMEM = TILES + 8 * BARS + 16;
+    static constexpr int SMEM = TILES + 8 * BARS + 24;
 };
 
 template <int D>
@@ -218,10 +227,10 @@ packed_forward_kernel(const __grid_constant__ PackedParams p) {
     const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     const uint32_t base = smem_u32(smem_raw);
     const uint32_t q_tile = base, k_tile = base + TILE, v_tile = k_tile + STAGES * KV_TILE, bars = base + C::TILES;
-    const int4 item = p.items[blockIdx.x / p.heads];     // on its way during the set-up: the host has waited for the table's upload
     auto bar = [&](int which) { return bars + 8u * which; };
     uint32_t& s_tmem_base = *reinterpret_cast<uint32_t*>(smem_raw + C::TILES + 8 * C::BARS);
     volatile int& s_abort = *reinterpret_cast<volatile int*>(smem_raw + C::TILES + 8 * C::BARS + 4);
+    int* s_item = reinterpret_cast<int*>(smem_raw + C::TILES + 8 * C::BARS + 8);
     if (base & 1023u) {   // the operand tiles need the alignment the declaration asks for
         chain_wait();
         if (threadIdx.x == 0) atomicExch(p.status, STATUS_ATTENTION_WAIT + 1);
@@ -234,12 +243,13 @@ packed_forward_kernel(const __grid_constant__ PackedParams p) {
         prefetch_map(&p.map_q); prefetch_map(&p.map_k); prefetch_map(&p.map_v);
     }
     if (warp == 1) allocate(&s_tmem_base, 256);
+    if (warp == 2) fetch_item(p, blockIdx.x / p.heads, s_item);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     chain_wait();
     chain_next();      // the tensor memory is this block's
-    const int start = uniform(item.x), length = uniform(item.y), i = uniform(item.z);
+    const int start = uniform(s_item[0]), length = uniform(s_item[1]), i = uniform(s_item[2]);
     const int h = (int)(blockIdx.x % p.heads), g = h / (p.heads / p.kv_heads);
     // key blocks that hold a position <= the last query of this block that there is
     const int n = (min(length, (i + 1) * BLOCK) + KEYS - 1) / KEYS;
@@ -429,7 +439,7 @@ template <int D> struct DQ {
     static constexpr int TILES = 2 * TILE + (K_STAGES + V_STAGES) * KV_TILE;
     enum { Q_FULL = 0, K_FULL = 1, K_EMPTY = K_FULL + K_STAGES, V_FULL = K_EMPTY + K_STAGES, V_EMPTY = V_FULL + V_STAGES, S_FULL = V_EMPTY + V_STAGES,
            S_TAKEN = S_FULL + 2, DP_FULL, DS_FULL, DQ_DONE, BARS };
-    static constexpr int SMEM = TILES + 8 * BARS + 16;
+    static constexpr int SMEM = TILES + 8 * BARS + 24;
 };
 
 template <int D>
@@ -441,10 +451,10 @@ packed_dq_kernel(const __grid_constant__ PackedParams p) {
     const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     const uint32_t base = smem_u32(smem_raw);
     const uint32_t q_tile = base, do_tile = base + TILE, k_tile = do_tile + TILE, v_tile = k_tile + C::K_STAGES * KV_TILE, bars = base + C::TILES;
-    const int4 item = p.items[blockIdx.x / p.heads];     // on its way during the set-up, as in the forward
     auto bar = [&](int which) { return bars + 8u * which; };
     uint32_t& s_tmem_base = *reinterpret_cast<uint32_t*>(smem_raw + C::TILES + 8 * C::BARS);
     volatile int& s_abort = *reinterpret_cast<volatile int*>(smem_raw + C::TILES + 8 * C::BARS + 4);
+    int* s_item = reinterpret_cast<int*>(smem_raw + C::TILES + 8 * C::BARS + 8);
     if (base & 1023u) {
         chain_wait();
         if (threadIdx.x == 0) atomicExch(p.status, STATUS_ATTENTION_WAIT + 1);
@@ -457,12 +467,13 @@ packed_dq_kernel(const __grid_constant__ PackedParams p) {
         prefetch_map(&p.map_q); prefetch_map(&p.map_k); prefetch_map(&p.map_v); prefetch_map(&p.map_do);
     }
     if (warp == 1) allocate(&s_tmem_base, 256);
+    if (warp == 2) fetch_item(p, blockIdx.x / p.heads, s_item);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     chain_wait();
     chain_next();      // the tensor memory is this block's
-    const int start = uniform(item.x), length = uniform(item.y), i = uniform(item.z);
+    const int start = uniform(s_item[0]), length = uniform(s_item[1]), i = uniform(s_item[2]);
     const int h = (int)(blockIdx.x % p.heads), g = h / (p.heads / p.kv_heads);
     // key blocks that hold a position <= the last query of this block that there is
     const int n = (min(length, (i + 1) * BLOCK) + KEYS - 1) / KEYS;
@@ -689,7 +700,7 @@ template <int D> struct DKV {
     enum { KV_FULL = 0, Q_FULL = 1, Q_EMPTY = Q_FULL + STAGES, DO_FULL = Q_EMPTY + STAGES, DO_EMPTY = DO_FULL + STAGES, S_FULL = DO_EMPTY + STAGES, DP_FULL = S_FULL + 2,
            P_FULL, DS_FULL = P_FULL + 2, ACC_DONE, BARS };
     static constexpr int BARS_AT = ROWS_AT + STAGES * DKV_ROW_BYTES;
-    static constexpr int SMEM = BARS_AT + 8 * BARS + 16;
+    static constexpr int SMEM = BARS_AT + 8 * BARS + 24;
 };
 
 template <int D>
@@ -710,11 +721,11 @@ packed_dkv_kernel(const __grid_constant__ PackedParams p) {
         chain_wait();
         return;
     }
-    const int4 item = p.items[job / p.kv_heads];         // on its way during the set-up, as in the forward
     // S_FULL and P_FULL are two barriers each, by the parity of the iteration (attention.cu says why)
     auto bar = [&](int which) { return bars + 8u * which; };
     uint32_t& s_tmem_base = *reinterpret_cast<uint32_t*>(smem_raw + C::BARS_AT + 8 * C::BARS);
     volatile int& s_abort = *reinterpret_cast<volatile int*>(smem_raw + C::BARS_AT + 8 * C::BARS + 4);
+    int* s_item = reinterpret_cast<int*>(smem_raw + C::BARS_AT + 8 * C::BARS + 8);
     if (base & 1023u) {
         chain_wait();
         if (threadIdx.x == 0) atomicExch(p.status, STATUS_ATTENTION_WAIT + 1);
@@ -731,13 +742,14 @@ packed_dkv_kernel(const __grid_constant__ PackedParams p) {
         prefetch_map(&p.map_q); prefetch_map(&p.map_k); prefetch_map(&p.map_v); prefetch_map(&p.map_do);
     }
     if (warp == 1) allocate(&s_tmem_base, 512);
+    if (warp == 2) fetch_item(p, job / p.kv_heads, s_item);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     chain_wait();
     chain_next();      // the tensor memory is this block's
-    const int start = uniform(item.x), length = uniform(item.y), blocks = (length + BLOCK - 1) / BLOCK;
-    const int j = blocks - 1 - uniform(item.z);                         // the list's block with the most key blocks is the one with the most query blocks
+    const int start = uniform(s_item[0]), length = uniform(s_item[1]), blocks = (length + BLOCK - 1) / BLOCK;
+    const int j = blocks - 1 - uniform(s_item[2]);                         // the list's block with the most key blocks is the one with the most query blocks
     const int g = job % p.kv_heads, group = p.heads / p.kv_heads;
     const int per_head = blocks - j;                           // query blocks j .. blocks - 1
     const int all = group * per_head;                          // iterations: head of the group (outer), query block (inner)
