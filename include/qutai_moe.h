@@ -92,6 +92,11 @@ int qmoe_event_sync(uint64_t event);                       /* host waits for the
  * of a kernel configures it).  After an error inside a capture call qmoe_graph_abandon. */
 int qmoe_graph_begin(uint64_t stream);
 int qmoe_stream_capturing(uint64_t stream);               /* 1 while what goes to the stream is recorded, else 0 */
+/* Which recording that is, a number of its own, or 0; and whether nothing is left of a recording: it was abandoned, or its graph destroyed (0 for ever for one
+ * that qmoe_graph_begin did not begin).  Buffers that a recorded call writes to belong to the recording until then.  A graph that was replayed on another
+ * stream than the recorded one is destroyed when those replays are over. */
+uint64_t qmoe_capture_number(uint64_t stream);
+int qmoe_capture_over(uint64_t number);
 int qmoe_graph_end(uint64_t stream, uint64_t* graph);
 int qmoe_graph_abandon(uint64_t stream);
 int qmoe_graph_launch(uint64_t graph, uint64_t stream);

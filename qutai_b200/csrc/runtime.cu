@@ -1,6 +1,7 @@
 // Process-wide plumbing of libqutai_moe.so: error text, launch counters, per-kernel-class event
 // timing, the device status word, and the small memory/stream helpers of the C ABI.
 #include <atomic>
+#include <iterator>
 #include <map>
 #include <mutex>
 #include <stdarg.h>
@@ -269,6 +270,25 @@ namespace {
 std::mutex g_graph_mutex;
 std::map<uint64_t, long long> g_graph_kernels;        // kernels recorded in each instantiated graph
 thread_local long long g_capture_started_at = 0;      // launch counter when this thread's capture began
+// Recordings that still are, by the runtime's number: being made or, with a graph, replayable.  One that was begun elsewhere stays here: nobody says when it ends.
+std::map<unsigned long long, uint64_t> g_recordings;  // number -> graph, 0 while it is being made
+std::map<uint64_t, unsigned long long> g_recording_of; // stream -> number, from qmoe_graph_begin to its end
+
+unsigned long long recording_on(uint64_t stream) {
+    cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+    unsigned long long number = 0;
+    if (cudaStreamGetCaptureInfo((cudaStream_t)stream, &status, &number) != cudaSuccess) { (void)cudaGetLastError(); return 0; }
+    return status == cudaStreamCaptureStatusActive ? number : 0;
+}
+// the recording of the stream is no longer being made; without a graph nothing is left of it
+void recording_ended(uint64_t stream, uint64_t graph) {
+    std::lock_guard<std::mutex> lock(g_graph_mutex);
+    auto it = g_recording_of.find(stream);
+    if (it == g_recording_of.end()) return;
+    if (graph) g_recordings[it->second] = graph;
+    else g_recordings.erase(it->second);
+    g_recording_of.erase(it);
+}
 }  // namespace
 
 extern "C" int qmoe_graph_begin(uint64_t stream) {
@@ -276,6 +296,10 @@ extern "C" int qmoe_graph_begin(uint64_t stream) {
     if (g_sync_each_launch) { set_error("graph capture is not possible with QUTAI_MOE_SYNC=1"); return QMOE_ERR_STATE; }
     QMOE_CUDA(cudaStreamBeginCapture((cudaStream_t)stream, cudaStreamCaptureModeThreadLocal));
     g_capture_started_at = g_launches.load();
+    const unsigned long long number = recording_on(stream);
+    std::lock_guard<std::mutex> lock(g_graph_mutex);
+    g_recordings[number] = 0;
+    g_recording_of[stream] = number;
     return 0;
 }
 extern "C" int qmoe_stream_capturing(uint64_t stream) {
@@ -283,14 +307,27 @@ extern "C" int qmoe_stream_capturing(uint64_t stream) {
     if (cudaStreamIsCapturing((cudaStream_t)stream, &status) != cudaSuccess) { (void)cudaGetLastError(); return 0; }
     return status != cudaStreamCaptureStatusNone;
 }
+extern "C" uint64_t qmoe_capture_number(uint64_t stream) {
+    const unsigned long long number = recording_on(stream);
+    std::lock_guard<std::mutex> lock(g_graph_mutex);
+    if (number) g_recordings.emplace(number, 0);
+    return number;
+}
+extern "C" int qmoe_capture_over(uint64_t number) {
+    std::lock_guard<std::mutex> lock(g_graph_mutex);
+    return g_recordings.find(number) == g_recordings.end();
+}
 extern "C" int qmoe_graph_end(uint64_t stream, uint64_t* graph) {
     if (!graph) return fail_arg("graph_end: graph is null");
     *graph = 0;
     cudaGraph_t recorded = nullptr;
-    QMOE_CUDA(cudaStreamEndCapture((cudaStream_t)stream, &recorded));
     cudaGraphExec_t exec = nullptr;
-    cudaError_t code = cudaGraphInstantiate(&exec, recorded, 0);
-    cudaGraphDestroy(recorded);
+    cudaError_t code = cudaStreamEndCapture((cudaStream_t)stream, &recorded);
+    if (code == cudaSuccess) {
+        code = cudaGraphInstantiate(&exec, recorded, 0);
+        cudaGraphDestroy(recorded);
+    }
+    recording_ended(stream, code == cudaSuccess ? (uint64_t)exec : 0);
     QMOE_CUDA(code);
     *graph = (uint64_t)exec;
     const long long recorded_kernels = g_launches.load() - g_capture_started_at;
@@ -304,6 +341,7 @@ extern "C" int qmoe_graph_abandon(uint64_t stream) {  // after a failed call dur
     cudaStreamEndCapture((cudaStream_t)stream, &recorded);
     if (recorded) cudaGraphDestroy(recorded);
     cudaGetLastError();
+    recording_ended(stream, 0);
     return 0;
 }
 extern "C" int qmoe_graph_launch(uint64_t graph, uint64_t stream) {
@@ -323,6 +361,7 @@ extern "C" int qmoe_graph_destroy(uint64_t graph) {
     QMOE_CUDA(cudaGraphExecDestroy((cudaGraphExec_t)graph));
     std::lock_guard<std::mutex> lock(g_graph_mutex);
     g_graph_kernels.erase(graph);
+    for (auto it = g_recordings.begin(); it != g_recordings.end();) it = it->second == graph ? g_recordings.erase(it) : std::next(it);
     return 0;
 }
 

@@ -277,6 +277,8 @@ SIGNATURES = {
     "qmoe_graph_end": (c_int, [_U, POINTER(c_uint64)]),
     "qmoe_graph_abandon": (c_int, [_U]),
     "qmoe_stream_capturing": (c_int, [_U]),
+    "qmoe_capture_number": (c_uint64, [_U]),
+    "qmoe_capture_over": (c_int, [_U]),
     "qmoe_graph_launch": (c_int, [_U, _U]),
     "qmoe_graph_destroy": (c_int, [_U]),
     "qmoe_optim_table_bytes": (c_int64, [_I32]),

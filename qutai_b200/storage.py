@@ -41,6 +41,9 @@ def _allocate(nbytes, stream):
     step = 512 if nbytes < (1 << 16) else 1 << 16
     size = (nbytes + step - 1) // step * step or step
     free = _cache.get((stream, size))
+    if not free and _recorded:
+        release_recorded()
+        free = _cache.get((stream, size))
     if free:
         _cached_bytes -= size
         address = free.pop()
@@ -78,18 +81,29 @@ def _release(address, size, stream):
     _cached_bytes += size
 
 
-_recorded = []      # scratch of recorded calls: a replay writes to it again
+_recorded = {}      # recording -> what its calls took for themselves: a replay writes to it again
 
 
 def done_with(scratch, stream):
-    """The caller's last use of ``scratch`` is in ``stream``.  While the stream's work is recorded the block stays out of the cache for good: a later call
-    could have it for something that lives when the graph is replayed."""
-    if stream and lib.load().qmoe_stream_capturing(stream):
-        _recorded.append(scratch)
+    """The caller's last use of ``scratch`` is in ``stream``.  While the stream's work is recorded the block stays out of the cache, since a later call
+    could have it for something that lives when the graph is replayed, until the recording is abandoned or its graph destroyed."""
+    recording = lib.load().qmoe_capture_number(stream) if stream else 0
+    if recording:
+        release_recorded()
+        _recorded.setdefault(recording, []).append(scratch)
+
+
+def release_recorded():
+    """Let go of what belongs to recordings of which nothing is left (done as well before the device is asked for memory)."""
+    handle = lib.load()
+    for recording in [number for number in _recorded if handle.qmoe_capture_over(number)]:
+        del _recorded[recording]
 
 
 def empty_cache():
     global _cached_bytes
+    if _recorded:
+        release_recorded()
     handle = lib.load()
     for blocks in _cache.values():
         for address in blocks:
