@@ -888,9 +888,13 @@ typedef struct qmoe_byte_item {
     int64_t first_chunk;                 /* set by the library */
     float step;                          /* lr / (1 - beta1^t) of THIS tensor's step t */
     float root_factor;                   /* 1 / sqrt(1 - beta2^t) */
+    uint64_t count;                      /* i64 [2] on the device, the steps taken and room for what follows from them, or 0: not kept there */
+    int64_t number;                      /* beside a count: this step's number, which is written to it; or 0: it is one more than the count, and the device forms
+                                          * step and root_factor from that and the call's learning rate and betas, anew at each replay of a recorded call */
 } qmoe_byte_item_t;
 int64_t qmoe_byte_table_bytes(int32_t count);
-/* `table`: qmoe_byte_table_bytes(count) bytes on the device; up to 32 items do not use it. */
+/* `table`: qmoe_byte_table_bytes(count) bytes on the device; up to 32 items do not use it, and only so many can be recorded.  A recorded call is of items with a
+ * count and the number 0: others would take the same step again at each replay, and are refused. */
 int qmoe_adamw_bytes(qmoe_byte_item_t* items, int32_t count, uint64_t table, double learning_rate, double beta1, double beta2, double eps,
                      double weight_decay, uint64_t stream);
 /* average_out = m, square_out = r r of every item; values and grad are not read. */

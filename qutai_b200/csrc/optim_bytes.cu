@@ -42,6 +42,8 @@ struct Item {  // = qmoe_byte_item_t
     long long size;
     long long first_chunk;
     float step, root_factor;
+    long long* count;                   // steps taken, then step and root_factor of the one being taken
+    long long number;
 };
 static_assert(sizeof(Item) == sizeof(qmoe_byte_item_t), "the table layout is part of the C ABI");
 
@@ -283,6 +285,21 @@ __device__ __forceinline__ bool aligned_item(const Item& it, bool step) {
     return (wide & 15u) == 0 && (((uintptr_t)it.average | (uintptr_t)it.root) & 3u) == 0 && (!step || ((uintptr_t)it.shadow & 7u) == 0);
 }
 
+// Items whose step's number the device keeps: one more, and the corrections that follow from it, a power to a thread.
+template <bool FEW>
+__global__ void __launch_bounds__(kThreads)
+next_step_kernel(const __grid_constant__ FewItems few, const Item* __restrict__ table, int count, double learning_rate, double beta1, double beta2) {
+    chain_begin();
+    const Item* items = FEW ? few.item : table;
+    for (int i = threadIdx.x; i < count; i += kThreads) {
+        long long* kept = items[i].count;
+        if (!kept || items[i].number) continue;
+        const long long t = kept[0] + 1;
+        kept[0] = t;
+        *reinterpret_cast<float2*>(kept + 1) = make_float2((float)(learning_rate / (1 - pow(beta1, (double)t))), (float)(1 / sqrt(1 - pow(beta2, (double)t))));
+    }
+}
+
 template <bool FEW>
 __global__ void __launch_bounds__(kThreads)
 adamw_bytes_kernel(const __grid_constant__ FewItems few, const Item* __restrict__ table, int count, long long total_chunks, Rates rates) {
@@ -294,7 +311,13 @@ adamw_bytes_kernel(const __grid_constant__ FewItems few, const Item* __restrict_
         if (chunk >= last) {
             it = items[find_item(items, count, chunk)];
             last = it.first_chunk + (it.size + kChunk - 1) / kChunk;
+            if (it.count && !it.number) {
+                const float2 given = *reinterpret_cast<const float2*>(it.count + 1);
+                it.step = given.x;
+                it.root_factor = given.y;
+            }
         }
+        if (chunk == it.first_chunk && threadIdx.x == 0 && it.count && it.number) it.count[0] = it.number;
         const long long base = (chunk - it.first_chunk) * kChunk + (threadIdx.x >> 5) * (2 * kBlock);
         if (base >= it.size) continue;
         if (aligned_item(it, true) && base + 2 * kBlock <= it.size) step_blocks<true>(it, base, rates);
@@ -365,23 +388,32 @@ byte_values_kernel(const __grid_constant__ FewItems few, const Item* __restrict_
 }
 
 // Validates the host's table and fills in first_chunk; a table of many items goes to `table` on the device.
-int stage(qmoe_byte_item_t* items, int count, uint64_t table, bool step, FewItems& few, long long* total, cudaStream_t stream) {
+// `counted`: some item's step has the number that follows from its count.
+int stage(qmoe_byte_item_t* items, int count, uint64_t table, bool step, FewItems& few, long long* total, bool* counted, cudaStream_t stream) {
     if (!items || count <= 0) return fail_arg("optimizer: the item table is empty");
     if (count > kFewItems && (!table || (table & 15u))) return fail_arg("optimizer: the device table address must be non-null and 16-byte aligned");
     long long chunks = 0;
+    bool given = false;
+    *counted = false;
     for (int i = 0; i < count; ++i) {
         qmoe_byte_item_t& it = items[i];
+        if (step && (it.count & 7u || it.number < 0)) return fail_arg("adamw: item %d has a misaligned count or a negative number", i);
+        const bool follows = it.count && !it.number;
+        given = given || !follows;
+        *counted = *counted || follows;
         if (it.size <= 0) return fail_arg("optimizer: item %d has size %lld", i, (long long)it.size);
         if (!it.average || !it.average_scale || !it.root || !it.root_scale || (step ? !it.values || !it.grad : !it.average_out || !it.square_out))
             return fail_arg("optimizer: item %d has a null address", i);
         if ((it.values | it.grad | it.average_scale | it.root_scale | it.average_out | it.square_out) & 3u || it.shadow & 1u)
             return fail_arg("optimizer: item %d has a misaligned address", i);
-        if (step && (!(it.step >= 0) || !(it.root_factor > 0) || isinf(it.step) || isinf(it.root_factor)))
+        if (step && !follows && (!(it.step >= 0) || !(it.root_factor > 0) || isinf(it.step) || isinf(it.root_factor)))
             return fail_arg("adamw: item %d has a bias correction that is no positive number", i);
         it.first_chunk = chunks;
         chunks += (it.size + kChunk - 1) / kChunk;
     }
     *total = chunks;
+    if (step && given && qmoe_stream_capturing((uint64_t)stream))
+        return fail_arg("adamw: a step whose number is given cannot be captured: a replay would take it again with the same bias corrections");
     if (count <= kFewItems) memcpy(few.item, items, (size_t)count * sizeof(Item));
     else if (qmoe_stream_capturing((uint64_t)stream)) return fail_arg("optimizer: more than %d items cannot be captured: a replay would copy the host's table as it is then", kFewItems);
     else QMOE_CUDA(cudaMemcpyAsync((void*)table, items, (size_t)count * sizeof(Item), cudaMemcpyHostToDevice, stream));
@@ -408,8 +440,14 @@ extern "C" int qmoe_adamw_bytes(qmoe_byte_item_t* items, int32_t count, uint64_t
     cudaStream_t stream = (cudaStream_t)stream_;
     FewItems few;
     long long chunks = 0;
-    if (int rc = stage(items, count, table, true, few, &chunks, stream)) return rc;
+    bool counted = false;
+    if (int rc = stage(items, count, table, true, few, &chunks, &counted, stream)) return rc;
     TimedScope timed(KC_OPTIMIZER, stream);
+    if (counted) {
+        if (count <= kFewItems) chained(next_step_kernel<true>, 1, kThreads, 0, stream, few, nullptr, count, learning_rate, beta1, beta2);
+        else chained(next_step_kernel<false>, 1, kThreads, 0, stream, few, (const Item*)table, count, learning_rate, beta1, beta2);
+        QMOE_LAUNCH_CHECK("next_step_kernel");
+    }
     const Rates rates = {(float)beta1, (float)(1 - beta1), (float)beta2, (float)(1 - beta2), (float)(1 - learning_rate * weight_decay), (float)eps * 0.0625f};
     if (count <= kFewItems) chained(adamw_bytes_kernel<true>, grid_for(chunks), kThreads, 0, stream, few, nullptr, count, chunks, rates);
     else chained(adamw_bytes_kernel<false>, grid_for(chunks), kThreads, 0, stream, few, (const Item*)table, count, chunks, rates);
@@ -421,7 +459,8 @@ extern "C" int qmoe_byte_values(qmoe_byte_item_t* items, int32_t count, uint64_t
     cudaStream_t stream = (cudaStream_t)stream_;
     FewItems few;
     long long chunks = 0;
-    if (int rc = stage(items, count, table, false, few, &chunks, stream)) return rc;
+    bool counted = false;
+    if (int rc = stage(items, count, table, false, few, &chunks, &counted, stream)) return rc;
     TimedScope timed(KC_OPTIMIZER, stream);
     if (count <= kFewItems) chained(byte_values_kernel<true>, grid_for(chunks), kThreads, 0, stream, few, nullptr, count, chunks);
     else chained(byte_values_kernel<false>, grid_for(chunks), kThreads, 0, stream, few, (const Item*)table, count, chunks);

@@ -62,7 +62,7 @@ class OptimItem(Structure):
 class ByteItem(Structure):
     """``qmoe_byte_item_t``."""
     _fields_ = [(name, c_uint64) for name in ("values", "grad", "average", "average_scale", "root", "root_scale", "shadow", "average_out", "square_out")] + [
-        ("size", c_int64), ("first_chunk", c_int64), ("step", c_float), ("root_factor", c_float)]
+        ("size", c_int64), ("first_chunk", c_int64), ("step", c_float), ("root_factor", c_float), ("count", c_uint64), ("number", c_int64)]
 
 
 class Layer(Structure):

@@ -18,7 +18,7 @@ from itertools import chain
 from math import isfinite
 
 from . import lib
-from .storage import DeviceStorage
+from .storage import DeviceStorage, done_with
 
 
 def _parameters(source):
@@ -29,7 +29,7 @@ def _parameters(source):
 
 
 _ITEM = "5Q2q2f"       # lib.OptimItem: values, grad, exp_avg, exp_avg_sq, shadow, size, first_chunk, c1, c2
-_BYTE_ITEM = "9Q2q2f"  # lib.ByteItem: values, grad, average, its scale, root, its scale, shadow, two outputs, size, first_chunk, step, root_factor
+_BYTE_ITEM = "9Q2q2fQq"    # lib.ByteItem: values, grad, average, its scale, root, its scale, shadow, two outputs, size, first_chunk, step, root_factor, count, number
 STATE_BLOCK = 256      # elements of an 8-bit moment that share a scale
 
 
@@ -116,7 +116,11 @@ def clip_grad_norm_sharded(replicated, sharded, max_norm=1.0, *, stream=0):
 class AdamW:
     """Adam with decoupled weight decay; state per parameter object (``steps``, ``averages``,
     ``square_averages``), created when the parameter first has a gradient.  ``state_bits``: 32, averages in float32
-    storages, or 8, averages as ``ByteState`` (learning rate and epsilon are then read as they are at each step, like the others)."""
+    storages, or 8, averages as ``ByteState`` (learning rate and epsilon are then read as they are at each step, like the others).
+
+    A step with 8-bit states on a stream of its own can be recorded (``qmoe_graph_begin``), once one has been taken by itself, for up to 32 parameters with
+    gradients.  Each replay is the next step, counted on the device, from what the same gradient storages hold then, with the recorded learning rate and
+    settings.  ``replayed()`` tells the host about replays."""
 
     def __init__(self, parameters, *, learning_rate=0.001, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01,
                  shadows=None, stream=0, state_bits=32):
@@ -136,6 +140,9 @@ class AdamW:
         self.state_bits = state_bits
         self._table = _Table(self.stream) if state_bits == 32 else _Table(self.stream, lib.ByteItem, _BYTE_ITEM)
         self._values_table = _Table(self.stream, lib.ByteItem, _BYTE_ITEM)
+        # 8 bits on a stream that can be recorded: two words on the device for each parameter, of which the first is its steps; what ``steps`` was when they were
+        # written; and whether a recording counts there, so that the host's number may be behind
+        self._counts, self._counted, self._recorded = None, {}, False
 
     def _state(self, states, parameter):
         """The parameter's moment in ``states``, zeros before its first step."""
@@ -147,7 +154,7 @@ class AdamW:
             raise ValueError("an 8-bit state must be a ByteState of its parameter's size")
         return state
 
-    def _row(self, parameter, gradient, shadow, step):
+    def _row(self, parameter, gradient, shadow, step, count=0, number=0):
         beta1, beta2 = self.betas
         average, square = self._state(self.averages, parameter), self._state(self.square_averages, parameter)
         shadow = 0 if shadow is None else shadow.ptr
@@ -155,7 +162,7 @@ class AdamW:
             return (parameter.storage.ptr, gradient.storage.ptr, average.ptr, square.ptr, shadow, parameter.storage.size, 0,
                     1 - beta1 ** step, 1 - beta2 ** step)
         return (parameter.storage.ptr, gradient.storage.ptr, average.codes.ptr, average.scales.ptr, square.codes.ptr, square.scales.ptr, shadow, 0, 0,
-                parameter.storage.size, 0, self.learning_rate / (1 - beta1 ** step), (1 - beta2 ** step) ** -0.5)
+                parameter.storage.size, 0, self.learning_rate / (1 - beta1 ** step), (1 - beta2 ** step) ** -0.5, count, number)
 
     def values_of_states(self, out=None):
         """``{parameter: (average, square average)}`` as float32 storages, what 8-bit states stand for, in one launch: what a checkpoint holds.  ``out``:
@@ -173,7 +180,7 @@ class AdamW:
             average, square, size = self._state(self.averages, parameter), self._state(self.square_averages, parameter), parameter.storage.size
             if any(s.dtype != "float32" or s.size != size for s in (average_out, square_out)):
                 raise ValueError("a state's values are float32 and as many as its parameter's")
-            rows.append((0, 0, average.codes.ptr, average.scales.ptr, square.codes.ptr, square.scales.ptr, 0, average_out.ptr, square_out.ptr, size, 0, 0.0, 0.0))
+            rows.append((0, 0, average.codes.ptr, average.scales.ptr, square.codes.ptr, square.scales.ptr, 0, average_out.ptr, square_out.ptr, size, 0, 0.0, 0.0, 0, 0))
         if rows:
             items, count, device = self._values_table.fill(rows)
             lib.call("qmoe_byte_values", items, count, device, self.stream)
@@ -189,7 +196,9 @@ class AdamW:
     def step(self):
         beta1, beta2 = self.betas
         rows, updated, steps = [], [], {}
-        for parameter in self.parameters:
+        counting = self.state_bits == 8 and self.stream != 0
+        recording = counting and bool(lib.load().qmoe_stream_capturing(self.stream))
+        for i, parameter in enumerate(self.parameters):
             gradient = parameter.grad
             if gradient is None:
                 continue
@@ -199,15 +208,41 @@ class AdamW:
             shadow = self.shadows.get(parameter)
             if shadow is not None and (shadow.dtype != "bfloat16" or shadow.size != parameter.storage.size):
                 raise ValueError("a shadow must be a bfloat16 storage of its parameter's size")
-            rows.append(self._row(parameter, gradient, shadow, step))
+            kept = number = 0
+            if counting:
+                in_step = parameter in self._counted and self._counted[parameter] == step - 1
+                if recording and not (in_step and parameter in self.averages and parameter in self.square_averages):
+                    raise RuntimeError("a step is recorded after one by itself, from the states and the number of steps that it left")
+                if self._counts is None:
+                    self._counts = DeviceStorage.zeros(2 * len(self.parameters), "int64", self.stream)
+                kept, number = self._counts.ptr + 16 * i, 0 if recording or (self._recorded and in_step) else step
+            rows.append(self._row(parameter, gradient, shadow, step, kept, number))
             steps[parameter] = step
             updated.append((parameter.storage, shadow))
         if not rows:
             return
         items, count, device = self._table.fill(rows)
-        # Change tracking (storage.py): the parameters' generation grows.  A bf16 copy that was current before the
-        # step and whose every updated part was rewritten by this launch is current afterwards as well; a copy of
-        # an allocation in which some updated parameter had no shadow is left stale for its owner to rebuild.
+        written = self._written(updated)
+        lib.call("qmoe_adamw_multi" if self.state_bits == 32 else "qmoe_adamw_bytes", items, count, device, self.learning_rate, beta1, beta2, self.eps,
+                 self.weight_decay, self.stream)
+        if recording:       # nothing has run; the states and the counts live as long as the recording
+            self._recorded = True
+            for parameter in steps:
+                for state in (self.averages[parameter], self.square_averages[parameter]):
+                    done_with(state.codes, self.stream)
+                    done_with(state.scales, self.stream)
+            done_with(self._counts, self.stream)
+            return
+        self.steps.update(steps)
+        if counting:
+            self._counted.update(steps)
+        self._mark(written)
+
+    @staticmethod
+    def _written(updated):
+        """Change tracking (storage.py), before a step is launched: the parameters' generation grows.  A bf16 copy that was current before the
+        step and whose every updated part was rewritten by this launch is current afterwards as well; a copy of
+        an allocation in which some updated parameter had no shadow is left stale for its owner to rebuild."""
         groups = {}
         for master, shadow in updated:
             group = groups.setdefault(id(master._root), dict(master=master, shadows={}, complete=True))
@@ -218,10 +253,24 @@ class AdamW:
         for group in groups.values():
             group["current"] = [s for s in group["shadows"].values() if group["complete"] and len(group["shadows"]) == 1
                                 and s.is_derived_from(group["master"])]
-        lib.call("qmoe_adamw_multi" if self.state_bits == 32 else "qmoe_adamw_bytes", items, count, device, self.learning_rate, beta1, beta2, self.eps,
-                 self.weight_decay, self.stream)
-        self.steps.update(steps)
-        for group in groups.values():
+        return list(groups.values())
+
+    @staticmethod
+    def _mark(written):
+        for group in written:
             group["master"].touch()
             for shadow in group["current"]:
                 shadow.mark_derived_from(group["master"])
+
+    def replayed(self):
+        """Behind replays of recorded steps: waits for them, brings ``steps`` up to date with the device, and marks as changed the parameters that they wrote (bf16 copies
+        in ``shadows`` were written with them)."""
+        if self._counts is None:
+            return
+        counts, updated = self._counts.tolist(self.stream), []
+        for i, parameter in enumerate(self.parameters):
+            taken = counts[2 * i]
+            if parameter in self._counted and taken != self._counted[parameter]:
+                self.steps[parameter] = self._counted[parameter] = taken
+                updated.append((parameter.storage, self.shadows.get(parameter)))
+        self._mark(self._written(updated))
