@@ -301,14 +301,17 @@ int pieces_check(const qmoe_pieces_t* a, bool backward) {
     const long long bound = bound_of(a->rows);
     const Span hidden = {a->hidden, a->rows * a->width * item}, weight = {a->weight, a->vocab * a->width * item}, targets = {a->targets, a->rows * 8};
     const Span tables = {a->tables, (8 + group_words(a->rows) + a->rows + 2 * bound) * 4}, inputs = {a->inputs, bound * a->width * item}, lse = {a->lse, bound * 4};
-    const Span gradient = {backward ? a->gradient : 0, 4};
-    const Span written[4] = {{backward ? a->d_hidden : a->loss, backward ? a->rows * a->width * item : 4},
+    const Span gradient = {backward ? a->gradient : 0, 4}, row_loss = {a->row_loss, bound * 4}, none = {0, 0};
+    const Span scratch = {a->scratch, scratch_of(a, backward)};
+    const auto forward = [&](const Span& x) { return backward ? none : x; };
+    const auto kept = [&](const Span& x) { return backward ? x : none; };        // what the forward leaves is what the backward reads
+    const Span written[7] = {{backward ? a->d_hidden : a->loss, backward ? a->rows * a->width * item : 4},
                              {backward ? a->d_weight : 0, a->vocab * a->width * (a->weight_gradient == QMOE_BF16 ? 2 : 4)},
-                             backward ? Span{0, 0} : inputs, {a->scratch, scratch_of(a, backward)}};
-    for (int i = 0; i < 4; ++i) {
-        for (const Span& read : {weight, targets, tables, lse, gradient})
-            if (overlap(written[i], read)) return fail_arg("pieces: an output overlaps an operand");
-        if (overlap(written[i], backward ? inputs : hidden)) return fail_arg("pieces: an output overlaps an operand");
+                             scratch, forward(inputs), forward(tables), forward(lse), forward(row_loss)};
+    const Span read[7] = {weight, targets, gradient, forward(hidden), kept(inputs), kept(tables), kept(lse)};
+    for (int i = 0; i < 7; ++i) {
+        for (const Span& other : read)
+            if (overlap(written[i], other)) return fail_arg("pieces: an output overlaps an operand");
         for (int j = 0; j < i; ++j)
             if (overlap(written[i], written[j])) return fail_arg("pieces: two outputs overlap");
     }
