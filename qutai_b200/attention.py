@@ -161,6 +161,7 @@ def packed_attention_forward(q, k, v, heads, kv_heads, sequences, *, scale=None,
     if sequences.blocks:
         a.out, a.lse = (storage.ptr for storage in result)
         lib.call("qmoe_packed_attention_forward", ctypes.byref(a), stream)
+        done_with(sequences.table, stream)       # a replay reads it, whether or not the plan is still there
     return result
 
 
@@ -185,6 +186,7 @@ def packed_attention_backward(gradient, q, k, v, attended, lse, heads, kv_heads,
         a.dq, a.dk, a.dv = (storage.ptr for storage in result)
         lib.call("qmoe_packed_attention_backward", ctypes.byref(a), stream)
         done_with(delta, stream)
+        done_with(sequences.table, stream)
     return result
 
 
