@@ -63,7 +63,8 @@ class LMHead:
         self._operand_of_weight = of
         if not shadow.is_derived_from(weight.storage):
             lib.call("qmoe_cast_bf16", weight.storage.ptr, shadow.ptr, weight.storage.size, self.stream)
-            shadow.mark_derived_from(weight.storage)
+            if not (self.stream and lib.load().qmoe_stream_capturing(self.stream)):      # (a recorded cast has not run)
+                shadow.mark_derived_from(weight.storage)
         return shadow
 
     def forward(self, hidden, weight, labels):
@@ -143,7 +144,8 @@ def projection_loss(hidden, weight, labels, chunk_size=None, *, prepared_labels=
 class PiecewiseHead(LMHead):
     """The mean cross-entropy of rows that have a target each, with the logits formed a piece of the vocabulary at a time, in the
     backward again, and never kept.  ``piece_bytes``: how much of them (of their gradient) there may be at a time.  ``operand_of``: an ``LMHead`` of the
-    same weight, whose bfloat16 copy of it serves both."""
+    same weight, whose bfloat16 copy of it serves both.  A recorded call (``qmoe_graph_begin``) multiplies with the copy of a float32 weight as it is at each replay:
+    after an update of the weight one plain ``forward`` renews it."""
 
     def __init__(self, stream=0, *, piece_bytes=256 << 20, operand_of=None):
         if piece_bytes <= 0:
@@ -189,10 +191,14 @@ class PiecewiseHead(LMHead):
                        hidden.storage.ptr, operand.ptr, targets.ptr, loss.ptr, *(storage.ptr for storage in kept))
         scratch = self._scratch(a, 0)
         lib.call("qmoe_pieces_forward", ctypes.byref(a), self.stream)
-        for storage in (scratch, *kept):
-            done_with(storage, self.stream)
+        self._hold(scratch, operand, weight, kept)
         self._call = (a, hidden, weight, operand, targets, loss, kept)
         return Tensor(loss, ())
+
+    def _hold(self, scratch, operand, weight, kept):
+        """What a recorded call reads and writes beside its caller's storages: also after another loss has taken its place here."""
+        for storage in (scratch, *kept, *(() if operand is weight.storage else (operand,))):
+            done_with(storage, self.stream)
 
     def _scratch(self, a, backward):
         scratch = DeviceStorage(-(-int(lib.load().qmoe_pieces_scratch_bytes(ctypes.byref(a), backward)) // 4), "float32", stream=self.stream)
@@ -223,7 +229,7 @@ class PiecewiseHead(LMHead):
         a.d_hidden, a.d_weight = (0 if result is None else result.ptr for result in results)
         scratch = self._scratch(a, 1)
         lib.call("qmoe_pieces_backward", ctypes.byref(a), self.stream)
-        done_with(scratch, self.stream)
+        self._hold(scratch, operand, weight, kept)
         return tuple(None if result is None else Tensor(result, tensor.shape) for result, tensor in zip(results, (hidden, weight)))
 
 
