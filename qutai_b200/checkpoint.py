@@ -33,7 +33,7 @@ from pathlib import Path
 
 FORMAT, VERSION = "qutai-training-sharded", 1
 CHUNK_BYTES = 4 << 20
-_WIDTHS = {"float32": 4, "bfloat16": 2, "float64": 8, "int32": 4, "int64": 8}
+_WIDTHS = {"int8": 1, "float32": 4, "bfloat16": 2, "float64": 8, "int32": 4, "int64": 8}
 
 
 def layer_tensors(layer, prefix, *, rank=0):

@@ -52,7 +52,8 @@ class _Table:
 class ByteState:
     """One moment of a parameter in 8 bits: ``codes`` (int8 storage, one for each element) and ``scales`` (float32, one for every
     ``STATE_BLOCK`` elements).  The first moment's codes are e4m3 numbers; the second moment is held by its root, whose codes are numbers of 4 exponent and
-    4 mantissa bits without a sign (``qmoe_adamw_bytes`` in the header says which).  ``AdamW.values_of_states`` gives what they stand for."""
+    4 mantissa bits without a sign (``qmoe_adamw_bytes`` in the header says which).  ``AdamW.values_of_states`` gives what they stand for; a checkpoint holds the
+    codes and scales themselves (``checkpoint.save_sharded`` takes both), since values do not lead back to their codes."""
 
     def __init__(self, codes, scales):
         if codes.dtype != "int8" or scales.dtype != "float32" or scales.size != -(-codes.size // STATE_BLOCK):
@@ -165,7 +166,7 @@ class AdamW:
                 parameter.storage.size, 0, self.learning_rate / (1 - beta1 ** step), (1 - beta2 ** step) ** -0.5, count, number)
 
     def values_of_states(self, out=None):
-        """``{parameter: (average, square average)}`` as float32 storages, what 8-bit states stand for, in one launch: what a checkpoint holds.  ``out``:
+        """``{parameter: (average, square average)}`` as float32 storages, what 8-bit states stand for, in one launch, to be looked at or compared.  ``out``:
         such a dict, of the storages to write to (all parameters that have a state, or some of them)."""
         if self.state_bits != 8:
             if out is not None:
