@@ -627,7 +627,7 @@ typedef struct qmoe_rotate {
     int32_t layout;                      /* QMOE_ROTATE_* */
     int32_t backward;
     int32_t reserved;
-    int64_t offset;                      /* added to every position */
+    int64_t offset;                      /* added to every position; within 2^37 of 0 */
     int64_t q_pitch, k_pitch;
     uint64_t q, k;                       /* [batch * time, heads (kv_heads), dim] */
     uint64_t positions;                  /* i32 [batch * time] on the device, or 0: row t of a sequence is t */

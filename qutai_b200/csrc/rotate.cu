@@ -21,6 +21,7 @@ namespace {
 constexpr int kThreads = 256, kWarps = kThreads / 32;
 constexpr int kMaxPairs = 128;
 constexpr int kInFlight = 4;
+constexpr long long kFarthest = 1ll << 37;
 
 struct RotateParams {
     const void* q;
@@ -166,6 +167,8 @@ int rotate_check(const qmoe_rotate_t* a) {
     // (heads x units^2 below 2^32 keeps the head of a unit exact; the elements of a row in 32 bits)
     if (a->heads > (1 << 16) || a->kv_heads > (1 << 16) || (a->batch && a->time > 0x7fffffff / a->batch)) return fail_arg("rotate: too many rows or heads");
     if (!a->q || !a->k || !a->q_out || !a->k_out || !a->turns) return fail_arg("rotate: null buffer address");
+    // (the table's frequencies are off by up to 2^-64 of a turn a position: 2^-27 there, half of what rounding an angle to a float takes)
+    if (a->offset <= -kFarthest || a->offset >= kFarthest) return fail_arg("rotate: the offset must lie within 2^37 of 0");
     const uint64_t item = a->dtype == QMOE_BF16 ? 2 : 4;
     if ((a->q | a->k | a->q_out | a->k_out) & (item - 1) || a->positions & 3u || a->turns & 7u) return fail_arg("rotate: misaligned address");
     const uint64_t widths[2] = {(uint64_t)a->heads * a->dim, (uint64_t)a->kv_heads * a->dim}, rows = (uint64_t)a->batch * (uint64_t)a->time;

@@ -135,6 +135,10 @@ class Scaling:
             raise ValueError("bands need an original context above 0 and 0 < low < high")
 
 
+# The table's frequencies are off by up to 2^-64 of a turn for each position: here 2^-27, half of what the kernel's rounding of an angle takes
+FARTHEST = 2 ** 37
+
+
 class Rotation:
     """How heads of ``dim`` elements are turned: the first ``width`` of them (all by default) in pairs, neighbours with ``layout``
     "interleaved" (``qmoe_rope``'s), elements ``width / 2`` apart with "halves"; pair ``i`` by theta^(-2 i / width) radians
@@ -186,8 +190,8 @@ def _rotate(q, k, heads, kv_heads, rotation, positions, offset, out, stream, bac
     rows = batch * time
     if positions is not None and (positions.dtype != "int32" or positions.size != rows):
         raise ValueError("positions must hold one int32 position for each row")
-    if not -2 ** 62 < offset < 2 ** 62:
-        raise ValueError("the offset must fit 62 bits")
+    if not -FARTHEST < offset < FARTHEST:
+        raise ValueError("the offset must lie within 2^37 of 0, where the angles are as exact as anywhere")
     q_out, k_out = outputs(out, ((rows * heads * dim, dtype), (rows * kv_heads * dim, dtype)), stream)
     if rows:
         a = lib.Rotate(batch, time, heads, kv_heads, dim, rotation.width, lib.DTYPE_CODES[dtype], rotation._code, backward, 0, int(offset), q_pitch, k_pitch,
