@@ -152,8 +152,8 @@ class Rotation:
             raise ValueError("the turned width must be an even number of a head's elements")
         if layout not in ("interleaved", "halves"):
             raise ValueError("the layout is interleaved or halves")
-        if not 0 < theta <= 1e30:
-            raise ValueError("theta must be positive and at most 1e30")
+        if not 1e-15 <= theta <= 1e30:      # (40 digits hold the turns of a position, up to 1e15, and their fraction's 64 bits)
+            raise ValueError("theta must lie between 1e-15 and 1e30")
         self.dim, self.theta, self.layout, self.width, self.scaling = dim, theta, layout, width, scaling
         # what counts of an angle is its fraction of a turn, held in 64 bits: an integer product with the position keeps all of them
         with localcontext() as context:
