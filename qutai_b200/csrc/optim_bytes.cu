@@ -18,7 +18,10 @@
 #include "common.cuh"
 
 #include <cuda_fp8.h>
+#include <algorithm>
 #include <math.h>
+#include <memory>
+#include <new>
 #include <string.h>
 
 namespace qmoe {
@@ -387,6 +390,29 @@ byte_values_kernel(const __grid_constant__ FewItems few, const Item* __restrict_
     }
 }
 
+// The numbers of all items lie apart from one another and from all codes and scales: in the order of their addresses nothing that is written reaches past the next start.
+int values_apart(const qmoe_byte_item_t* items, int count) {
+    struct Span { uint64_t at, end; bool written; };
+    const std::unique_ptr<Span[]> spans(new (std::nothrow) Span[(size_t)count * 6]);
+    if (!spans) { set_error("optimizer: no memory for a table of %d items", count); return QMOE_ERR_STATE; }
+    Span* next = spans.get();
+    for (int i = 0; i < count; ++i) {
+        const qmoe_byte_item_t& it = items[i];
+        const uint64_t n = (uint64_t)it.size, scales = (n + kBlock - 1) / kBlock * 4;
+        for (const uint64_t at : {it.average_out, it.square_out}) *next++ = {at, at + n * 4, true};
+        for (const uint64_t at : {it.average, it.root}) *next++ = {at, at + n, false};
+        for (const uint64_t at : {it.average_scale, it.root_scale}) *next++ = {at, at + scales, false};
+    }
+    std::sort(spans.get(), next, [](const Span& a, const Span& b) { return a.at < b.at; });
+    uint64_t written = 0, any = 0;          // where what came so far ends
+    for (const Span* s = spans.get(); s != next; ++s) {
+        if (s->at < written || (s->written && s->at < any)) return fail_arg("optimizer: an output overlaps another or what is read");
+        if (s->written && s->end > written) written = s->end;
+        if (s->end > any) any = s->end;
+    }
+    return 0;
+}
+
 // Validates the host's table and fills in first_chunk; a table of many items goes to `table` on the device.
 // `counted`: some item's step has the number that follows from its count.
 int stage(qmoe_byte_item_t* items, int count, uint64_t table, bool step, FewItems& few, long long* total, bool* counted, cudaStream_t stream) {
@@ -412,6 +438,8 @@ int stage(qmoe_byte_item_t* items, int count, uint64_t table, bool step, FewItem
         chunks += (it.size + kChunk - 1) / kChunk;
     }
     *total = chunks;
+    if (!step)
+        if (int rc = values_apart(items, count)) return rc;
     if (step && given && qmoe_stream_capturing((uint64_t)stream))
         return fail_arg("adamw: a step whose number is given cannot be captured: a replay would take it again with the same bias corrections");
     if (count <= kFewItems) memcpy(few.item, items, (size_t)count * sizeof(Item));
