@@ -14,7 +14,8 @@
 // copy 2: 18 against 30 with moments in 32 bits (optim.cu).
 // What bounds it: memory, and near it the issue of instructions (59 % of the cycles: codes to numbers and back).  266 million elements in 92 tensors with their bf16
 // copies, and both moments written out as numbers behind the step: 1.46 ms for 7.4 GB, 5.1 TB/s.  One block to a warp 1.61, streaming loads and stores 1.49; the last blocks'
-// loads without branches took 156 registers and 1.86.
+// loads without branches took 156 registers and 1.86.  A block in which some element has had no gradient but zeros (an expert without tokens, an unused token's
+// row) or squares beyond the range takes the longer form: 134 million elements in 419 us without such blocks, 652 with a zero in every block, 708 with nothing but zeros.
 #include "common.cuh"
 
 #include <cuda_fp8.h>

@@ -14,9 +14,9 @@
 //   * Forward and dq walk key blocks of 64 positions, so that S has two buffers in the 256 columns of a CTA and two CTAs stay on an SM: the scores of the next block are
 //     formed while the rows have this one's.  P lies over the S that it came from, and so does dS (heads of 64); with heads of 128 dq has one S, and dS lies over dP.
 //     dk, dv has 128 x 128 blocks, 16 row warps and one CTA an SM; with heads of 128 its accumulators leave one buffer each for S and dP.
-// What bounds it: the row warps' chain from a block's scores to its probabilities (the exponential unit is busy for 47 % of the forward, the tensor cores for 22 to 38 %, an
-// instruction issues in 36 to 46 % of the cycles: 17 documents of up to 2048, 16 heads of 64), and with short documents the CTAs' starts and ends.  Forward and
-// backward of 4 x 4096 tokens, 16 query heads of 64 in 4 groups: 690 us, 697 TFLOP/s; 8 heads of 128: 571 us, 842 TFLOP/s.
+// What bounds it: the row warps' chain from a block's scores to its probabilities (the exponential unit is busy for 39 % of the forward, the tensor cores for 21 to 36 %, an
+// instruction issues in 40 to 45 % of the cycles: 17 documents of up to 2048, 16 heads of 64), and with short documents the CTAs' starts and ends.  Forward and
+// backward of 4 x 4096 tokens, 16 query heads of 64 in 4 groups: 737 us, 653 TFLOP/s; 8 heads of 128: 599 us, 803 TFLOP/s.
 // No atomics, every sum in a fixed order.  Every wait is bounded; on expiry the CTA records a code in the library's status word and leaves.
 #include "common.cuh"
 #include "attention_ptx.cuh"
@@ -56,8 +56,8 @@ __device__ __forceinline__ void exp2_two(uint64_t x, float& p0, float& p1) {
     unpair2(mul2(p, pair2(__uint_as_float(__float_as_uint(t0) << 23), __uint_as_float(__float_as_uint(t1) << 23))), p0, p1);
 }
 // Forward and dq: of as many pairs of probabilities one is formed there, beside the exponential unit, which is the busiest part of the forward.  4 x 4096 tokens, 16
-// heads of 64, thousand cycles with none, one of 8, 4, 3 and 2: forward 389, 372, 368, 377 and 423, dq 443, 417, 416, 414 and 433; 8 heads of 128: forward 233,
-// 231, 238, 236 and 248, dq 331, 330, 332, 331 and 340.
+// heads of 64, with none, one of 8, 4, 3 and 2: forward 240, 230, 233, 236 and 264 us, dq 443, 417, 416, 414 and 433 thousand cycles; 8 heads of 128: forward 157,
+// 154, 153, 158 and 171 us, dq 331, 330, 332, 331 and 340 thousand cycles.
 constexpr int ON_FMA = 8;
 
 struct QuickWait {
@@ -317,7 +317,7 @@ packed_forward_kernel(const __grid_constant__ PackedParams p) {
         const float scale2 = p.scale * LOG2E;                // in the exponent of 2
         const uint64_t scale_pair = pair2(scale2, scale2);
         // What is subtracted from scores: the largest so far (0 while all are -infinity), so that a row's largest probability is an exact 1 in bf16.  A base that may stay
-        // up to 2^8 below it leaves O alone in most blocks (forward, 4 x 4096 tokens, 16 heads of 64: 197 us for 215; 8 of 128: 131 for 147), but then that
+        // up to 2^8 below it leaves O alone in most blocks (forward, 4 x 4096 tokens, 16 heads of 64: 211 us for 230; 8 of 128: 133 for 154), but then that
         // probability is rounded too: out 2.13e-3 instead of 2.06e-3 from the exact result for operands of standard deviation 1, 2.08e-3 instead of 1.74e-3 for 2.
         float from = -INFINITY, l = 0.f;
         bool ok = true;
@@ -370,7 +370,7 @@ packed_forward_kernel(const __grid_constant__ PackedParams p) {
                 if (!ok) break;
                 tc_fence_after();
                 const uint64_t alpha_pair = pair2(alpha, alpha);
-                constexpr int AT_ONCE = D == 64 ? 64 : 32;       // (64 of heads of 128 spill: 148 us to 155 at 4 x 4096; 32 of heads of 64: 215 to 222)
+                constexpr int AT_ONCE = D == 64 ? 64 : 32;       // (64 of heads of 128 spill: forward 148 us to 156 at 4 x 4096; 32 of heads of 64: 215 to 222)
 #pragma unroll
                 for (int c = 0; c < D; c += AT_ONCE) {
                     uint32_t o[AT_ONCE];
@@ -1033,7 +1033,7 @@ packed_dkv_kernel(const __grid_constant__ PackedParams p) {
 // CTA by itself, 9 and 7 for one of a cluster.  Forward and backward in us with 1, 2, 4 and 8: five documents of up to 130 positions, 8 heads of 64 in 2 groups,
 // 38, 37, 32 and 30; 17 documents of up to 2048, 16 heads of 64 in 4 groups, 170, 178, 241 and 389; six of up to 1999, 8 heads of 128, 107, 136, 222 and 432.
 // The same rule says whether all lists are cut or those alone that are longer than the longest one's share: then the second case takes 157 in clusters of 2, of which 48 lists have
-// one each and 244 half of one.
+// one each and 244 half of one.  (Measured with a forward some 5 us shorter in the second and third case.)
 struct Cut { int split; long long shared; };
 Cut packed_split(const qmoe_packed_attention_t* a) {
     const double alone = a->dim == 64 ? 4 : 3, shared = a->dim == 64 ? 9 : 7, slots = sm_count();

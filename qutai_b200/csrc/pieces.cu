@@ -11,7 +11,8 @@
 //     the hidden rows' gradient in fp32; the product with the hidden rows, which is the piece of the table's gradient.  The factor gradient / counted
 //     rows is applied to the finished sums: before the rounding to bf16 it would shift every row's -1 by the same up to 2^-9 (a share of 32000 classes is
 //     next to nothing beside it: d_hidden 0.0026 off in the 2-norm like that, 0.0017 like this).
-// 2 products forward and backward more than the 6 R V d that the gradient needs without forming logits again: 8 R V d.
+// 8 R V d operations, one product more than the 6 R V d of a head that forms its logits once: the price of cutting the vocabulary, whose first pieces' gradients wait for the
+// sums of all.  (Cut over the rows instead, a chunk's logits could become gradients at once, in three products: not built.)
 // float32 rows (the parity mode) take the CUDA-core products, a piece of logits at a time in both directions.
 // No atomics: the same inputs give the same bits.
 #include "common.cuh"
