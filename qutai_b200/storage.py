@@ -96,8 +96,9 @@ def done_with(scratch, stream):
 def release_recorded():
     """Let go of what belongs to recordings of which nothing is left (done as well before the device is asked for memory)."""
     handle = lib.load()
-    for recording in [number for number in _recorded if handle.qmoe_capture_over(number)]:
-        del _recorded[recording]
+    for recording in list(_recorded):          # (another thread may record or let go meanwhile)
+        if handle.qmoe_capture_over(recording):
+            _recorded.pop(recording, None)
 
 
 def empty_cache():

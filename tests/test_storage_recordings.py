@@ -61,3 +61,17 @@ def test_recording_again_and_again_takes_no_more_memory(device, monkeypatch):
     assert device.made <= 4
     storage.empty_cache()                                     # what is left of recordings that are over goes back to the device as well
     assert not device.live and not storage._recorded
+
+
+def test_threads_record_and_let_go_at_once(device, monkeypatch):
+    """A recording that another thread makes, or lets go of, while the list is looked through."""
+    monkeypatch.setattr(storage, "_recorded", {1: [], 2: [], 3: []})
+
+    def over(number):
+        storage._recorded.setdefault(number + 10, [])
+        storage._recorded.pop(2, None)
+        return number < 3
+
+    device.qmoe_capture_over = over
+    storage.release_recorded()
+    assert set(storage._recorded) == {3, 11, 13} or set(storage._recorded) == {3, 11, 12, 13}
