@@ -95,6 +95,58 @@ def test_replays_are_the_next_steps(shadows):
         assert everything(recorded) == everything(plain) and set(recorded.steps.values()) == {42}
 
 
+def test_more_parameters_than_travel_with_a_launch():
+    """Forty parameters of which three have gradients when the step is recorded; then all take ordinary steps, the three by the device's count."""
+    from gpu_util import to_device
+    from qutai_b200.layers import Tensor
+    from qutai_b200.optim import AdamW
+
+    def forty(stream):
+        rng = np.random.default_rng(5)
+        return AdamW([Tensor(to_device(rng.standard_normal(100 + n), "float32"), (100 + n,), requires_grad=True) for n in range(40)], learning_rate=1e-2, state_bits=8,
+                     stream=stream)
+
+    def give(optimizer, seed, count):
+        rng = np.random.default_rng(seed)
+        for i, p in enumerate(optimizer.parameters):
+            values = rng.standard_normal(p.storage.size).astype(np.float32)
+            if i >= count:
+                p.grad = None
+            elif p.grad is None:
+                p.grad = Tensor(to_device(values, "float32"), p.shape)
+            else:
+                p.grad.storage.upload_bytes(values.tobytes(), optimizer.stream)
+
+    def state(optimizer):
+        return [[s.tobytes(optimizer.stream) for s in (p.storage, optimizer.averages[p].codes, optimizer.square_averages[p].codes)] for p in optimizer.averages]
+
+    import ctypes
+
+    with Recording() as r:
+        plain, recorded = forty(r.stream), forty(r.stream)
+        for optimizer in (plain, recorded):
+            give(optimizer, 0, 3)
+            optimizer.step()
+        r.lib.call("qmoe_graph_begin", r.stream)
+        recorded.step()
+        graph = ctypes.c_uint64()
+        r.lib.call("qmoe_graph_end", r.stream, ctypes.byref(graph))
+        r.graphs.append(graph.value)
+        held = [p.grad for p in recorded.parameters]           # a replay reads them
+        for seed, count in ((1, 3), (2, 3), (3, 40), (4, 40), (5, 3)):
+            for optimizer in (plain, recorded):
+                give(optimizer, seed, count)
+            plain.step()
+            if count == 3 and seed < 5:
+                r.replay(graph.value)
+            else:
+                recorded.step()
+            assert state(recorded) == state(plain), seed
+        recorded.replayed()
+        assert list(recorded.steps.values()) == list(plain.steps.values()) and sorted(set(plain.steps.values())) == [2, 6]
+        assert held
+
+
 def test_a_first_step_or_another_number_of_steps_is_not_recorded():
     with Recording() as r:
         optimizer = made(2, r.stream)
